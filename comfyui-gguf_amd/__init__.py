@@ -14,6 +14,9 @@ fp16) -- as hand-written HIP kernels for gfx950 behind a C-ABI shared library
     loader      gguf_sd_loader & co. (reference loader.py:16-141) without the `gguf` package
     resident    opt-in cache that keeps dequantized weights resident in HBM (288 GB make it possible)
     fused       fused dequantize + linear: 1-4 rows (modulation layers) and, on the matrix cores, up to 256 rows; install()'s default
+    norms       residual + gate + the norms before and after a block + modulation in one pass, in the stream's type or as 8-bit rows
+    int8        rows in 8 bits with a scale each, and the product of 8-bit integers with a scale per token and per output channel
+    moe         a mixture-of-experts layer on packed expert weights, for a few tokens
     overlap     opt-in side-stream prefetch: layer i+1's (host->device copy and) unpack under layer i's GEMM
     sharding    tensor-list partitioning for one-process-per-GPU runs (no collectives)
     ops         GGMLTensor / GGMLLinear stand-ins for driving the path without ComfyUI
@@ -29,7 +32,7 @@ __version__ = "0.1.0"
 # package adds NO nodes -- it accelerates the ones ComfyUI-GGUF registers ("Unet Loader (GGUF)" & co. keep working unchanged).
 NODE_CLASS_MAPPINGS = {}
 NODE_DISPLAY_NAME_MAPPINGS = {}
-_LAZY = ("_native", "autoinstall", "dequant", "install", "grouped", "sharding", "ops", "manifests", "gguf_file", "gguf_adapter", "loader", "resident", "fused", "overlap")
+_LAZY = ("_native", "autoinstall", "dequant", "install", "grouped", "sharding", "ops", "manifests", "gguf_file", "gguf_adapter", "loader", "resident", "fused", "norms", "int8", "moe", "overlap")
 
 
 def _running_under_comfyui():

@@ -18,13 +18,20 @@ CSRC = os.path.join(_HERE, "csrc")
 LIB_DIR = os.path.join(_HERE, "_lib")
 # GGQ_HIP_LIB: load another build of the library (A/B measurements); default = the in-tree build
 LIB_PATH = os.environ.get("GGQ_HIP_LIB") or os.path.join(LIB_DIR, "libggq_hip.so")
-SOURCES = [os.path.join(CSRC, "ggq_capi.hip"), os.path.join(CSRC, "ggq_gguf.hip"), os.path.join(CSRC, "ggq_linear.hip"), os.path.join(CSRC, "ggq_overlap.hip")]
-HEADERS = [os.path.join(CSRC, "ggq_device.hpp"), os.path.join(CSRC, "ggq_linear.hpp"), os.path.join(CSRC, "ggq_mfma.hpp"), os.path.join(CSRC, "ggq_mfma16.hpp"), os.path.join(CSRC, "ggq_gemm.hpp"), os.path.join(CSRC, "ggq_host.hpp"), os.path.join(ROOT, "include", "ggq.h"), os.path.join(ROOT, "include", "ggq_gguf.h")]
+SOURCES = [os.path.join(CSRC, "ggq_capi.hip"), os.path.join(CSRC, "ggq_gguf.hip"), os.path.join(CSRC, "ggq_linear.hip"), os.path.join(CSRC, "ggq_overlap.hip"),
+           os.path.join(CSRC, "ggq_rows.hip"), os.path.join(CSRC, "ggq_int8.hip"), os.path.join(CSRC, "ggq_moe.hip")]
+HEADERS = [os.path.join(CSRC, "ggq_device.hpp"), os.path.join(CSRC, "ggq_linear.hpp"), os.path.join(CSRC, "ggq_mfma.hpp"), os.path.join(CSRC, "ggq_mfma16.hpp"), os.path.join(CSRC, "ggq_gemm.hpp"), os.path.join(CSRC, "ggq_host.hpp"), os.path.join(CSRC, "ggq_launch.hpp"),
+           os.path.join(CSRC, "ggq_rows.hpp"), os.path.join(CSRC, "ggq_int8.hpp"), os.path.join(CSRC, "ggq_moe.hpp"), os.path.join(ROOT, "include", "ggq.h"), os.path.join(ROOT, "include", "ggq_gguf.h")]
 ABI_VERSION = 11
 
 # -ffp-contract=off is REQUIRED for parity: hipcc otherwise fuses the reference's separately
 # rounded fp16 multiply and subtract into v_pk_fma_f16 (SURVEY.md section 0 finding 3).
 HIPCC_FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-ffp-contract=off", "-fPIC", "-shared"]
+
+# packed fp32 instructions stay out of the row, integer-product and expert kernels: some of their forms have returned wrong values on this part
+EXTRA_FLAGS = {f: ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"] for f in ("ggq_rows.hip", "ggq_int8.hip", "ggq_moe.hip")}
+# the one unit that unpacks no weights: its fp32 arithmetic has no operation sequence of the reference to keep
+FMA_ALLOWED = ("ggq_rows.hip",)
 
 # fused multiply-add mnemonics that must not appear in the dequant kernels
 _FMA_RE = re.compile(r"\b(v_(?:pk_)?(?:fma|fmac)_\w+|v_mad_(?:f16|f32|legacy_f\w+|mix\w*|mixlo\w*|mixhi\w*)\w*)")
@@ -41,6 +48,17 @@ _u64, _u32, _int, _vp = ctypes.c_uint64, ctypes.c_uint32, ctypes.c_int, ctypes.c
 class ggq_desc(ctypes.Structure):
     _fields_ = [("qtype", ctypes.c_int32), ("out_dtype", ctypes.c_int32), ("packed", _vp), ("out", _vp), ("n_blocks", _u64),
                 ("compute_dtype", ctypes.c_int32), ("reserved", ctypes.c_int32)]
+
+
+class ggq_norm_desc(ctypes.Structure):
+    _fields_ = [(n, _vp) for n in ("stream", "branch", "stream_out", "y", "y_scale", "post_weight", "gate", "weight", "bias", "scale", "shift")] \
+        + [(n, _u64) for n in ("rows", "gate_stride", "scale_stride", "shift_stride", "y_stride")] \
+        + [(n, _u32) for n in ("dim", "rows_per_mod", "params_f32")] + [(n, ctypes.c_int32) for n in ("dtype", "norm", "post_norm")] + [("eps", ctypes.c_float)]
+
+
+class ggq_moe_desc(ctypes.Structure):
+    _fields_ = [(n, _vp) for n in ("x", "ids", "weights", "gate", "up", "down", "y", "workspace")] + [("workspace_bytes", _u64)] \
+        + [(n, _u32) for n in ("tokens", "top_k", "experts", "dim", "ff")] + [(n, ctypes.c_int32) for n in ("up_qtype", "down_qtype", "act", "dtype")]
 
 
 GGUF_MAX_DIMS = 8
@@ -86,6 +104,12 @@ SYMBOLS = {
     "ggq_linear_mfma": (_int, [_int, _vp, _u32, _u32, _vp, _u32, _vp, _vp, _int, _int, _vp]),
     "ggq_linear_mfma_ws": (_int, [_int, _vp, _u32, _u32, _vp, _u32, _vp, _vp, _int, _int, _vp, _u64, _vp]),
     "ggq_linear_mfma_workspace": (_u64, [_int, _u32, _u32, _u32, _int]),
+    "ggq_block_norm": (_int, [ctypes.POINTER(ggq_norm_desc), _vp]),
+    "ggq_quantize_rows": (_int, [_vp, _u64, _u32, _vp, _u64, _vp, _int, _vp]),
+    "ggq_linear_int8": (_int, [_vp, _u64, _vp, _u32, _vp, _u64, _vp, _u32, _u32, _vp, _vp, _int, _vp]),
+    "ggq_moe_route": (_int, [_vp, _vp, _u32, _u32, _u32, _u32, _int, _vp, _vp, _int, _int, _vp]),
+    "ggq_moe_experts": (_int, [ctypes.POINTER(ggq_moe_desc), _vp]),
+    "ggq_moe_workspace": (_u64, [_u32, _u32, _u32]),
     "ggq_dequant_rows": (_int, [_int, _vp, _u64, _u32, _vp, _u64, _vp, _int, _int, _vp]),
     # include/ggq_gguf.h
     "ggq_gguf_open": (_int, [ctypes.c_char_p, ctypes.POINTER(_vp)]),
@@ -163,14 +187,14 @@ def build(force=False, verbose=False):
     os.makedirs(LIB_DIR, exist_ok=True)
     with tempfile.TemporaryDirectory(prefix="ggq_build_") as tmp:
         out = os.path.join(tmp, "libggq_hip.so")
-        # one hipcc -c per translation unit, all at once (the four take 20-40 s each), then one link
+        # one hipcc -c per translation unit, all at once, then one link
         compile_flags = [f for f in HIPCC_FLAGS if f != "-shared"]
         jobs = []
         for src in SOURCES:
             stem = os.path.splitext(os.path.basename(src))[0]
             d = os.path.join(tmp, stem)
             os.makedirs(d)
-            cmd = [hipcc_path()] + compile_flags + [f'-DGGQ_BUILD_ID="{source_id()}"', "-save-temps=obj", "-c", "-o", os.path.join(d, stem + ".o"), src]
+            cmd = [hipcc_path()] + compile_flags + EXTRA_FLAGS.get(os.path.basename(src), []) + [f'-DGGQ_BUILD_ID="{source_id()}"', "-save-temps=obj", "-c", "-o", os.path.join(d, stem + ".o"), src]
             jobs.append((cmd, d, subprocess.Popen(cmd, cwd=d, stdout=subprocess.PIPE, stderr=subprocess.PIPE, text=True)))
         failed = None
         for cmd, d, proc in jobs:
@@ -188,7 +212,8 @@ def build(force=False, verbose=False):
         for f in asm:
             with open(f) as fh:
                 text = fh.read()
-            check_no_fma(text)
+            if not os.path.basename(f).startswith(tuple(os.path.splitext(u)[0] + "-" for u in FMA_ALLOWED)):
+                check_no_fma(text)
             check_no_spills(text)
         link = [hipcc_path()] + HIPCC_FLAGS + ["-o", out] + [os.path.join(d, os.path.basename(d) + ".o") for _, d, _ in jobs]
         proc = subprocess.run(link, cwd=tmp, capture_output=True, text=True)

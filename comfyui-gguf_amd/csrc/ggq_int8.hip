@@ -1,0 +1,62 @@
+// ggq_int8.hip -- C ABI over ggq_int8.hpp: the product of 8-bit integers with a scale per row of x and per row of w.
+#include "ggq_int8.hpp"
+#include "ggq_launch.hpp"
+#include "../../include/ggq.h"
+
+namespace {
+
+using namespace ggq;
+
+constexpr uint32_t MAX_K = 131071;                 // 128 * 128 * k stays below 2^31
+
+template <int DT, int TM, int TN, int WM, int WN>
+hipError_t launch_tile(I8Args a, hipStream_t s)
+{
+    constexpr uint32_t lds = 2u * (TM + TN) * I8_BK;
+    if (lds > 64 * 1024) {
+        static std::atomic<uint64_t> raised{0};
+        const hipError_t e = allow_lds(reinterpret_cast<const void*>(&linear_i8_tile<DT, TM, TN, WM, WN>), (int)lds, raised);
+        if (e != hipSuccess) return e;
+    }
+    a.tiles_m = (a.m + TM - 1) / TM;
+    a.tiles_n = (a.n + TN - 1) / TN;
+    if ((uint64_t)a.tiles_m * a.tiles_n > 0x7FFFFFFFull) return hipErrorInvalidValue;
+    hipLaunchKernelGGL((linear_i8_tile<DT, TM, TN, WM, WN>), dim3(a.tiles_m * a.tiles_n), dim3(WM * WN * 64), lds, s, a);
+    return hipGetLastError();
+}
+
+template <int DT>
+hipError_t launch_rows16(const I8Args& a, hipStream_t s)
+{
+    hipLaunchKernelGGL((linear_i8_rows<DT>), dim3((a.n + 15u) / 16u, (a.m + 15u) / 16u), dim3(I8_ROW_WAVES * 64), 0, s, a);
+    return hipGetLastError();
+}
+
+template <int DT>
+hipError_t launch(const I8Args& a, hipStream_t s)
+{
+    if (a.m <= 16) return launch_rows16<DT>(a, s);
+    const uint64_t big = (uint64_t)((a.m + 255u) / 256u) * ((a.n + 255u) / 256u);
+    if (big >= 256) return launch_tile<DT, 256, 256, 2, 4>(a, s);
+    if (a.m > 64) return launch_tile<DT, 128, 128, 2, 2>(a, s);
+    return launch_tile<DT, 64, 64, 2, 2>(a, s);
+}
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+}  // namespace
+
+extern "C" int ggq_linear_int8(const void* xq, uint64_t x_stride, const float* x_scale, uint32_t m, const void* wq, uint64_t w_stride, const float* w_scale, uint32_t n,
+                               uint32_t k, const void* bias, void* y, int dtype, void* hip_stream)
+{
+    if (dtype < 0 || dtype > 2 || k == 0 || k > MAX_K) return GGQ_ERR_ARG;
+    if (m == 0 || n == 0) return GGQ_OK;
+    const uint64_t k16 = (k + 15u) & ~15u;
+    if (!xq || !x_scale || !wq || !w_scale || !y || x_stride % 16 != 0 || w_stride % 16 != 0 || x_stride < k16 || w_stride < k16) return GGQ_ERR_ARG;
+    if (!aligned16(xq) || !aligned16(wq) || (reinterpret_cast<uintptr_t>(y) & (dtype == GGQ_F32 ? 3u : 1u))) return GGQ_ERR_ALIGN;
+    const I8Args a{static_cast<const uint8_t*>(xq), static_cast<const uint8_t*>(wq), x_scale, w_scale, static_cast<const uint8_t*>(bias), static_cast<uint8_t*>(y),
+                   x_stride, w_stride, m, n, k, 0, 0};
+    hipStream_t s = static_cast<hipStream_t>(hip_stream);
+    const hipError_t e = dtype == GGQ_F16 ? launch<OUT_F16>(a, s) : (dtype == GGQ_BF16 ? launch<OUT_BF16>(a, s) : launch<OUT_F32>(a, s));
+    return e == hipSuccess ? GGQ_OK : hip_fail(e);
+}

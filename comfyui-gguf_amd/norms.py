@@ -1,0 +1,173 @@
+"""What a transformer block does to its rows between two linears, in one pass over memory (include/ggq.h ``ggq_block_norm``, csrc/ggq_rows.hpp):
+
+    r = stream + gate * [post_weight * N_post(branch)]            the residual sum, with the gate and the norm behind the block
+    y = (N(r) * weight + bias) * (1 + scale) + shift              the norm in front of the next block, modulated
+
+The models that the reference loads run these as separate torch operations around ``GGMLOps.Linear`` (ops.py:242-244; the layer norm itself through
+``GGMLOps.LayerNorm``, ops.py:262-266).  Here r stays in fp32 registers between the sum and the norm.  ``quantize=True`` returns y as 8-bit rows with a
+scale each, ready for ``int8.linear_int8``.
+
+As the fused linears do, the call raises GGQUnsupported for what the kernel does not take (CPU tensors, other types, a recording autograd); the caller
+keeps its torch operations then.
+"""
+import ctypes
+
+import torch
+
+from . import _native
+from .dequant import GGQUnsupported, _DEVICE_OK, _OUT_CODE, _cur_device, _device_served, _is_compiling, _raw_stream, dequantize_tensor, is_quantized
+
+NORMS = {None: 0, "none": 0, "rms": 1, "layer": 2}
+MAX_DIM = 24576                    # elements of a row: they live in the registers of one workgroup
+_call = None
+
+
+def _bind():
+    global _call
+    _call = _native.lib().ggq_block_norm
+    return _call
+
+
+def _plain(t):
+    return t if type(t) is torch.Tensor else t.as_subclass(torch.Tensor)
+
+
+def _on_gpu(x, what):
+    """x as a plain tensor on a served GPU, of a type that the row kernels take."""
+    if not isinstance(x, torch.Tensor) or not x.is_cuda or x.dtype not in _OUT_CODE:
+        raise GGQUnsupported(f"{what}: fp16 / bf16 / fp32 tensors on the GPU")
+    index = x.device.index
+    if not (_DEVICE_OK.get(index) or _device_served(index)):
+        raise GGQUnsupported(f"cuda:{index} is not a gfx950 device")
+    return _plain(x)
+
+
+def _refuse_grad(what, *tensors):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise GGQUnsupported(f"{what}: autograd is recording -- torch's operations build the graph")
+
+
+def _vector(v, dim, dtype, device, what):
+    """A parameter of `dim` values as (tensor, is fp32)."""
+    if is_quantized(v):
+        v = dequantize_tensor(v, torch.float32)
+    v = _plain(v)
+    if v.device != device or v.numel() != dim:
+        raise GGQUnsupported(f"block_norm: {what} holds {v.numel()} values on {v.device}, rows have {dim} on {device}")
+    if v.dtype is not dtype and v.dtype is not torch.float32:
+        v = v.float()
+    return v.contiguous(), v.dtype is torch.float32
+
+
+def _per_sample(v, lead, dim, dtype, device, what):
+    """A modulation vector per sample as (2-D tensor, stride between vectors, vectors, is fp32).  v's leading dimensions are the stream's, or the
+    first of them followed by ones."""
+    v = _plain(v)
+    if v.device != device or v.dim() == 0 or v.shape[-1] != dim:
+        raise GGQUnsupported(f"block_norm: {what} of shape {tuple(v.shape)} on {v.device} for rows of {dim} on {device}")
+    if v.dtype is not dtype and v.dtype is not torch.float32:
+        v = v.float()
+    own = list(v.shape[:-1])
+    while own and own[-1] == 1:
+        own.pop()
+    if own != list(lead[:len(own)]):
+        raise GGQUnsupported(f"block_norm: {what} of shape {tuple(v.shape)} does not follow the stream's leading dimensions {tuple(lead)}")
+    v = v.reshape(-1, dim)                          # a view where the vectors are one stride apart (a chunk of a modulation linear's output)
+    if v.stride(1) != 1:
+        v = v.contiguous()
+    n = v.shape[0]
+    return v, v.stride(0) if n > 1 else 0, n, v.dtype is torch.float32
+
+
+def _block_norm(stream, branch, gate, post_norm, post_weight, norm, weight, bias, scale, shift, eps, quantize):
+    stream = _on_gpu(stream, "block_norm")
+    if stream.dim() == 0 or norm not in NORMS or post_norm not in NORMS:
+        raise GGQUnsupported(f"block_norm: rows of a tensor, and norms of {sorted(k for k in NORMS if k)} or None")
+    _refuse_grad("block_norm", stream, branch, gate, post_weight, weight, bias, scale, shift)
+    kind, post_kind = NORMS[norm], NORMS[post_norm]
+    if branch is None and (gate is not None or post_kind or post_weight is not None):
+        raise GGQUnsupported("block_norm: gate and post_norm act on branch, which is not given")
+    if post_weight is not None and not post_kind:
+        raise GGQUnsupported("block_norm: post_weight belongs to post_norm, which is not given")
+    if not kind and (weight is not None or bias is not None or scale is not None or shift is not None):
+        raise GGQUnsupported("block_norm: weight, bias, scale and shift belong to norm, which is not given")
+    if not kind and branch is None and not quantize:
+        raise GGQUnsupported("block_norm: nothing to compute")
+    device, dtype, lead, dim = stream.device, stream.dtype, stream.shape[:-1], stream.shape[-1]
+    if not 1 <= dim <= MAX_DIM:
+        raise GGQUnsupported(f"block_norm: rows of 1 ... {MAX_DIM} elements")
+    rows = stream.numel() // dim
+    stream = stream if stream.is_contiguous() else stream.contiguous()
+    d = _native.ggq_norm_desc(stream=stream.data_ptr(), rows=rows, dim=dim, rows_per_mod=max(rows, 1), dtype=_OUT_CODE[dtype], norm=kind, post_norm=post_kind, eps=eps)
+    keep = []
+    if branch is not None:
+        branch = _plain(branch)
+        if branch.shape != stream.shape or branch.dtype is not dtype or branch.device != device:
+            raise GGQUnsupported(f"block_norm: branch {tuple(branch.shape)} {branch.dtype} is not like the stream {tuple(stream.shape)} {dtype}")
+        branch = branch if branch.is_contiguous() else branch.contiguous()
+        d.branch = branch.data_ptr()
+    flags = 0
+    for bit, name, v in ((1, "post_weight", post_weight), (4, "weight", weight), (8, "bias", bias)):
+        if v is not None:
+            v, is32 = _vector(v, dim, dtype, device, name)
+            keep.append(v)
+            setattr(d, name, v.data_ptr())
+            flags |= bit if is32 else 0
+    counts = set()
+    for bit, name, v in ((2, "gate", gate), (16, "scale", scale), (32, "shift", shift)):
+        if v is not None:
+            v, stride, n, is32 = _per_sample(v, lead, dim, dtype, device, name)
+            keep.append(v)
+            setattr(d, name, v.data_ptr())
+            setattr(d, name + "_stride", stride)
+            flags |= bit if is32 else 0
+            if n > 1:
+                counts.add(n)
+    if len(counts) > 1:
+        raise GGQUnsupported(f"block_norm: gate, scale and shift of {sorted(counts)} vectors: give them for the same rows")
+    if counts:
+        d.rows_per_mod = max(1, rows // counts.pop())
+    d.params_f32 = flags
+    out = stream
+    if branch is not None:
+        out = torch.empty_like(stream)
+        d.stream_out = out.data_ptr()
+    y = y_scale = None
+    if quantize:
+        pad = (dim + 15) // 16 * 16
+        y = torch.empty((*lead, pad), dtype=torch.int8, device=device)
+        y_scale = torch.empty(lead, dtype=torch.float32, device=device)
+        d.y, d.y_scale, d.y_stride = y.data_ptr(), y_scale.data_ptr(), pad
+        y = y[..., :dim] if pad != dim else y
+    elif kind:
+        y = torch.empty_like(stream)
+        d.y = y.data_ptr()
+    if rows:
+        index = device.index
+        call = _call or _bind()
+        if _cur_device() != index:
+            with torch.cuda.device(index):
+                rc = call(ctypes.byref(d), _raw_stream(index))
+        else:
+            rc = call(ctypes.byref(d), _raw_stream(index))
+        if rc:
+            _native.check(rc, "ggq_block_norm")
+    return out, ((y, y_scale) if quantize else y)
+
+
+def block_norm(stream, branch=None, *, gate=None, post_norm=None, post_weight=None, norm="rms", weight=None, bias=None, scale=None, shift=None, eps=1e-6, quantize=False):
+    """-> (r, y), see the module's formulas.
+
+    stream, branch: (..., dim), fp16 / bf16 / fp32, on the GPU.  Without ``branch`` r is ``stream`` itself.  ``norm`` / ``post_norm``: "rms", "layer" or None;
+    with ``norm=None`` y is None (the last block), or with ``quantize`` the 8-bit form of r.  ``weight``, ``bias``, ``post_weight``: dim values, fp32 or the
+    stream's type (GGUF norm weights are fp32).  ``gate``, ``scale``, ``shift``: one vector for all rows, or one per sample -- shape (batch, dim),
+    (batch, 1, dim), or the stream's own -- and may be chunks of one modulation linear's output.
+    ``quantize=True``: y is (q, q_scale), q int8 like the stream with rows 16 bytes apart, y ~ q * q_scale[..., None]; a row with an infinity or a NaN gets
+    q = 0 and scale NaN.  r and y are rounded once, from fp32."""
+    if _is_compiling():
+        return _eager(stream, branch, gate, post_norm, post_weight, norm, weight, bias, scale, shift, eps, quantize)
+    return _block_norm(stream, branch, gate, post_norm, post_weight, norm, weight, bias, scale, shift, eps, quantize)
+
+
+# while torch.compile traces, the launch is a graph break: nothing in it can be traced
+_eager = torch.compiler.disable(_block_norm)

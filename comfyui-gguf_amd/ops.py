@@ -181,3 +181,78 @@ class GGMLGroupNorm(GGMLLayer):
     def forward(self, input):
         weight, bias = self.cast_bias_weight(input)
         return torch.nn.functional.group_norm(input, self.num_groups, weight, bias, self.eps)
+
+
+class GGMLInt8Linear(torch.nn.Module):
+    """A linear layer whose weight is kept in 8 bits with a scale per output channel (int8.linear_int8): made once from a quantized (or plain) weight, a
+    byte per element from then on, the packed weight is not needed any more.  Activations are put into 8 bits token by token, so the result is another one
+    than GGMLLinear's: nothing chooses this layer by itself.  What the kernels do not take -- CPU tensors, a recording autograd -- is computed as F.linear
+    with the 8-bit weight's values."""
+
+    def __init__(self, weight, bias=None):
+        super().__init__()
+        from .int8 import quantize_rows
+        dense = dequantize_tensor(weight, torch.float16) if is_quantized(weight) else weight
+        dense = dense if type(dense) is torch.Tensor else dense.as_subclass(torch.Tensor)
+        q, scale = quantize_rows(dense.detach())
+        if bias is not None:
+            bias = dequantize_tensor(bias, torch.float32) if is_quantized(bias) else bias
+            bias = (bias if type(bias) is torch.Tensor else bias.as_subclass(torch.Tensor)).detach()
+        self.register_buffer("weight", q)
+        self.register_buffer("weight_scale", scale)
+        self.register_buffer("bias", bias)
+
+    def forward(self, input):
+        from .dequant import GGQUnsupported
+        from .int8 import linear_int8
+        try:
+            return linear_int8(input, self.weight, self.weight_scale, self.bias)
+        except GGQUnsupported:
+            weight = (self.weight.float() * self.weight_scale.float()[:, None]).to(input.dtype)
+            return torch.nn.functional.linear(input, weight, None if self.bias is None else self.bias.to(input.dtype))
+
+
+class GGMLMoE(torch.nn.Module):
+    """A mixture-of-experts layer over packed expert stacks (moe.moe_layer): ``router`` (experts, dim); ``gate``, ``up`` (experts, ff, dim) and ``down``
+    (experts, dim, ff) are GGMLTensors of three dimensions.  What the fused kernels do not take -- more than 64 tokens, CPU tensors, a recording
+    autograd -- runs one expert after the other: get_weight + F.linear, the reference's way (ops.py:242-244)."""
+
+    def __init__(self, router, gate, up, down, top_k, renormalize=True, activation="silu"):
+        super().__init__()
+        router = dequantize_tensor(router, torch.float32) if is_quantized(router) else router
+        self.router = router if type(router) is torch.Tensor else router.as_subclass(torch.Tensor)
+        self.gate, self.up, self.down = gate, up, down
+        self.top_k, self.renormalize, self.activation = top_k, renormalize, activation
+
+    def forward(self, input):
+        from .dequant import GGQUnsupported
+        from .moe import moe_layer
+        try:
+            return moe_layer(input, self.router, self.gate, self.up, self.down, top_k=self.top_k, renormalize=self.renormalize, activation=self.activation)
+        except GGQUnsupported:
+            return self._one_by_one(input)
+
+    def _one_by_one(self, input):
+        x = input.reshape(-1, input.shape[-1])
+        scores = torch.softmax(x.float() @ self.router.float().t(), -1)
+        share, ids = torch.sort(scores, dim=-1, descending=True, stable=True)
+        share, ids = share[:, :self.top_k], ids[:, :self.top_k]
+        if self.renormalize:
+            share = share / share.sum(-1, keepdim=True)
+        act = torch.nn.functional.silu if self.activation == "silu" else (lambda v: torch.nn.functional.gelu(v, approximate="tanh"))
+        y = torch.zeros(x.shape, dtype=torch.float32, device=x.device)
+        for expert in torch.unique(ids).tolist():
+            token, place = torch.nonzero(ids == expert, as_tuple=True)
+            gate, up, down = (self._expert(w, expert, x.dtype) for w in (self.gate, self.up, self.down))
+            rows = x[token]
+            out = torch.nn.functional.linear(act(torch.nn.functional.linear(rows, gate)) * torch.nn.functional.linear(rows, up), down)
+            y = y.index_add(0, token, out.float() * share[token, place][:, None])
+        return y.to(input.dtype).reshape(input.shape)
+
+    @staticmethod
+    def _expert(stack, expert, dtype):
+        plain = stack if type(stack) is torch.Tensor else stack.as_subclass(torch.Tensor)
+        experts, rows, cols = stack.tensor_shape
+        per = plain.numel() // experts
+        one = GGMLTensor(plain.reshape(-1)[expert * per:(expert + 1) * per].clone(), tensor_type=stack.tensor_type, tensor_shape=(rows, cols))
+        return dequantize_tensor(one, dtype)

@@ -208,6 +208,85 @@ int ggq_linear_mfma_ws(int qtype, const void* packed, uint32_t rows, uint32_t co
                        void* y, int dtype, int tile_rows, void* workspace, uint64_t workspace_bytes, void* hip_stream);
 uint64_t ggq_linear_mfma_workspace(int qtype, uint32_t rows, uint32_t cols, uint32_t m, int tile_rows);
 
+/* ---- the rows of a transformer block between its linears ------------------------------------------------------------------------------- */
+
+/* Residual, gate, norms and modulation of a block's rows in one pass (csrc/ggq_rows.hpp has the formulas):
+ *     r = stream + gate * [post_weight * N_post(branch)];     y = (N(r) * weight + bias) * (1 + scale) + shift
+ * for `rows` rows of `dim` contiguous elements of `dtype`.  branch NULL: r = stream, nothing is stored to stream_out.  y NULL: only the stream is
+ * computed.  N: 0 none, 1 root mean square, 2 layer norm (csrc NORM_*); eps is added to the mean square.  post_weight, weight, bias: `dim` values;
+ * gate, scale, shift: one vector of `dim` values for each rows_per_mod consecutive rows, `*_stride` ELEMENTS apart (0: one vector for all).  Any of
+ * the six may be NULL.  params_f32: bit i set = parameter i (order: post_weight, gate, weight, bias, scale, shift) holds fp32, else `dtype`.
+ * y_scale NULL: y is rows x dim of `dtype`.  y_scale given: y is int8 rows y_stride BYTES apart (a multiple of 16, >= dim; bytes past dim are
+ * written as 0) with y ~ q * y_scale[row], q = rint(127 y / max|row|), y_scale = max|row| / 127; a row with an infinity or a NaN: q = 0, scale NaN.
+ * stream_out may be stream, y may be branch.  GGQ_ERR_ARG: rows longer than 24576 elements.  Arithmetic in fp32 from load to store.
+ * Replaces: nothing of the reference's own code -- the torch operations that the models it loads run between GGMLOps.Linear calls
+ * (ops.py:242-244), and GGMLOps.LayerNorm (ops.py:262-266). */
+typedef struct ggq_norm_desc {
+    const void* stream;
+    const void* branch;
+    void* stream_out;
+    void* y;
+    float* y_scale;
+    const void* post_weight;
+    const void* gate;
+    const void* weight;
+    const void* bias;
+    const void* scale;
+    const void* shift;
+    uint64_t rows, gate_stride, scale_stride, shift_stride, y_stride;
+    uint32_t dim, rows_per_mod, params_f32;
+    int32_t dtype, norm, post_norm;
+    float eps;
+} ggq_norm_desc;
+int ggq_block_norm(const ggq_norm_desc* desc, void* hip_stream);
+
+/* Rows of `cols` values of `dtype` in 8 bits with one scale each: q[i, :] = rint(127 x[i, :] / max|x[i, :]|), scale[i] = max|x[i, :]| / 127; layout and
+ * special rows as in ggq_block_norm.  Half-way quotients of 16-bit rows go to the even integer exactly. */
+int ggq_quantize_rows(const void* x, uint64_t rows, uint32_t cols, void* q, uint64_t q_stride, float* scale, int dtype, void* hip_stream);
+
+/* ---- product of 8-bit integers -------------------------------------------------------------------------------------------------------- */
+
+/* y[i, j] = (sum_k xq[i, k] wq[j, k]) * x_scale[i] * w_scale[j] + bias[j], i < m, j < n: xq int8 rows x_stride bytes apart, wq int8 rows w_stride bytes
+ * apart (both multiples of 16, both arrays 16-byte aligned), scales fp32, bias (may be NULL) and y (m x n, contiguous) of `dtype`.  The integer sum
+ * is exact (int32; k <= 131071: GGQ_ERR_ARG above); scale, bias and the one rounding to `dtype` in fp32.  Bytes past column k of a row are read (up to
+ * the next multiple of 16) but must be 0 in xq where k is no multiple of 16.
+ * Replaces, for a weight kept in 8 bits: F.linear of GGMLOps.Linear.forward_ggml_cast_weights (ops.py:242-244). */
+int ggq_linear_int8(const void* xq, uint64_t x_stride, const float* x_scale, uint32_t m, const void* wq, uint64_t w_stride, const float* w_scale, uint32_t n,
+                    uint32_t k, const void* bias, void* y, int dtype, void* hip_stream);
+
+/* ---- mixture of experts for a few tokens ---------------------------------------------------------------------------------------------- */
+
+/* The experts of each token: p = softmax(x Wr^T) over `experts` (<= 512), the top_k (<= 16, <= experts) largest in descending order, equal ones to the
+ * lower index.  x: tokens x dim, router: experts x dim, of `dtype`
+ * (GGQ_F16 / GGQ_BF16) and router_dtype (`dtype` or GGQ_F32), contiguous, 16-byte aligned, dim % 8 == 0.  ids: int32
+ * tokens x top_k; weights: fp32, p of the chosen ones, divided by their sum if `renormalize`. */
+int ggq_moe_route(const void* x, const void* router, uint32_t tokens, uint32_t dim, uint32_t experts, uint32_t top_k, int renormalize, int32_t* ids,
+                  float* weights, int dtype, int router_dtype, void* hip_stream);
+
+/* y[t] = sum_s weights[t, s] * Wd[e] (act(Wg[e] x[t]) * (Wu[e] x[t])), e = ids[t, s], straight from packed expert weights: gate and up are packed stacks of
+ * logical shape (experts, ff, dim) in one format, down (experts, dim, ff) in its own; W = the fp16 values of the packed blocks in `dtype`, as
+ * dequantize_tensor gives.  1 <= tokens <= 64 (GGQ_ERR_ARG above), top_k <= 16, experts <= 512, dim and ff multiples of 256 (of 64 where the format that
+ * contracts over them has 32-element blocks).  An id outside [0, experts) adds nothing; the same id twice counts twice.  act: 0 silu, 1 gelu
+ * (tanh form).  x, y: tokens x dim of `dtype` (GGQ_F16 / GGQ_BF16).  workspace: ggq_moe_workspace() bytes, 16-byte aligned, used until the call's
+ * kernels have run.  Sums in fp32; the hidden vector is kept in two parts of `dtype` (its value and what rounding left), fp16 hidden values above
+ * 65504 overflow.  Deterministic.
+ * Replaces: one get_weight + F.linear (ops.py:242-244) per expert and projection. */
+typedef struct ggq_moe_desc {
+    const void* x;
+    const int32_t* ids;
+    const float* weights;
+    const void* gate;
+    const void* up;
+    const void* down;
+    void* y;
+    void* workspace;
+    uint64_t workspace_bytes;
+    uint32_t tokens, top_k, experts, dim, ff;
+    int32_t up_qtype, down_qtype, act, dtype;
+} ggq_moe_desc;
+int ggq_moe_experts(const ggq_moe_desc* desc, void* hip_stream);
+uint64_t ggq_moe_workspace(uint32_t tokens, uint32_t top_k, uint32_t ff);
+
 #ifdef __cplusplus
 }
 #endif
