@@ -1,32 +1,43 @@
 // ggq_rows.hip -- C ABI over ggq_rows.hpp: residual + gate + norms + modulation of a block's rows, and the 8-bit form of rows.
 #include "ggq_rows.hpp"
-#include "ggq_host.hpp"
+#include "ggq_launch.hpp"
 #include "../../include/ggq.h"
 
 namespace {
 
 using namespace ggq;
 
-typedef void (*rows_fn)(const RowArgs);
+typedef void (*rows_fn)(const RowArgs, uint32_t);
+typedef void (*long_fn)(const RowArgs);
 
-// rows of up to WAVES * 64 * NV * 8 elements: 24576 at most (8 vectors per lane on 8 waves would not fit the registers)
-#define GGQ_ROW_NV(DT, W) {block_norm<DT, W, 1>, block_norm<DT, W, 2>, block_norm<DT, W, 3>, block_norm<DT, W, 4>, block_norm<DT, W, 6>, block_norm<DT, W, (W == 8 ? 6 : 8)>}
-#define GGQ_ROW_DT(DT) {GGQ_ROW_NV(DT, 1), GGQ_ROW_NV(DT, 4), GGQ_ROW_NV(DT, 8)}
-const rows_fn ROWS[3][3][6] = {GGQ_ROW_DT(OUT_F16), GGQ_ROW_DT(OUT_BF16), GGQ_ROW_DT(OUT_F32)};
-constexpr uint32_t NVS[6] = {1, 2, 3, 4, 6, 8}, WAVES[3] = {1, 4, 8};
+// [dtype][dim % 8 != 0][a wave per row, a workgroup per row]
+#define GGQ_ROW_SET(DT) {{block_norm<DT, true, false>, block_norm<DT, false, false>}, {block_norm<DT, true, true>, block_norm<DT, false, true>}}
+const rows_fn ROWS[3][2][2] = {GGQ_ROW_SET(OUT_F16), GGQ_ROW_SET(OUT_BF16), GGQ_ROW_SET(OUT_F32)};
+const long_fn LONG_ROWS[3] = {block_norm_long<OUT_F16>, block_norm_long<OUT_BF16>, block_norm_long<OUT_F32>};
+constexpr uint32_t MAX_DIM = 32768;                                        // 128 KiB of LDS
 
 int launch_rows(const RowArgs& a, int dtype, hipStream_t s)
 {
     const uint64_t span = a.y_scale != nullptr ? a.y_stride : a.dim;       // elements a row's lanes have to cover (8-bit rows: their zero padding too)
+    if (span > MAX_DIM) return GGQ_ERR_ARG;
     const uint32_t vecs = (uint32_t)((span + 7) / 8);
-    int w = 0;
-    if (a.rows < 2048u || vecs > 64u * 8u) w = vecs > 4u * 64u * 8u || (a.rows < 256u && vecs > 64u) ? 2 : 1;
-    int nv = 0;
-    while (nv < 6 && (uint64_t)NVS[nv] * WAVES[w] * 64u < vecs) nv++;
-    if (nv == 6 || (w == 2 && nv == 5)) return GGQ_ERR_ARG;
-    const uint64_t grid = w == 0 ? (a.rows + 3) / 4 : a.rows;
-    if (grid > 0x7FFFFFFFull) return GGQ_ERR_ARG;
-    hipLaunchKernelGGL(ROWS[dtype][w][nv], dim3((uint32_t)grid), dim3(w == 0 ? 256u : WAVES[w] * 64u), 0, s, a);
+    if (vecs > 1024u) {
+        if (a.rows > 0x7FFFFFFFull) return GGQ_ERR_ARG;
+        static std::atomic<uint64_t> raised[3];
+        hipError_t e = allow_lds(reinterpret_cast<const void*>(LONG_ROWS[dtype]), MAX_DIM * 4, raised[dtype]);
+        if (e == hipSuccess) {
+            hipLaunchKernelGGL(LONG_ROWS[dtype], dim3((uint32_t)a.rows), dim3(ROW_LONG_THREADS), (vecs + 1023u) / 1024u * (ROW_LONG_THREADS * 32u), s, a);
+            e = hipGetLastError();
+        }
+        return e == hipSuccess ? GGQ_OK : hip_fail(e);
+    }
+    const bool solo = vecs <= 64u;
+    const uint32_t waves = solo ? 1u : (vecs + 63u) / 64u;
+    // as many teams as the chip holds at 16 waves per CU, each with as few rows as that leaves
+    const uint64_t teams = 256u * 16u / waves, per = (a.rows + teams - 1) / teams;
+    if (per > 0xFFFFFFFFull) return GGQ_ERR_ARG;
+    const uint64_t need = (a.rows + per - 1) / per, grid = solo ? (need + 3) / 4 : need;
+    hipLaunchKernelGGL(ROWS[dtype][a.dim % 8 != 0][solo ? 0 : 1], dim3((uint32_t)grid), dim3(solo ? 256u : waves * 64u), 0, s, a, (uint32_t)per);
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? GGQ_OK : hip_fail(e);
 }

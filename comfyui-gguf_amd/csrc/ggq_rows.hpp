@@ -13,8 +13,8 @@
 // formed in fp64 and rounded to fp32 before rint: in 16-bit rows |y| = a/2 is common and 63.5 has to be seen as exactly half-way, which a reciprocal in
 // fp32 misses; an fp32 product of two 24-bit values is not exact.
 //
-// What bounds it: HBM.  One pass: stream and branch are read once, r and y written once.  A row lives in the registers of one wave (long launches: no
-// barrier, no LDS) or of 4 / 8 waves (few rows: the row's latency is what counts).
+// What bounds it: HBM.  One pass: stream and branch are read once, r and y written once.  A row lives in the registers of one wave (short rows: no
+// barrier) or of the up to 16 waves of a workgroup, the longest in LDS.
 #pragma once
 
 #include "ggq_linear.hpp"
@@ -120,28 +120,33 @@ GGQ_DEV uint32_t wave_umax(uint32_t v)
     return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
 }
 
-// Sum / maximum over the WAVES waves of a row.  `slot` numbers the reductions of a kernel: each has LDS of its own, so one barrier is enough.
-template <int WAVES> GGQ_DEV float row_sum(float v, float (*red)[8], int slot)
+// Sum / maximum over the waves of a team, the same value in every lane.  SOLO: the team is one wave.  Else through red[], one slot of 16 per reduction (the
+// places of absent waves hold zeros), so that one barrier is enough: lane l reads place l % 16 and the 16 lanes of a DPP row fold them.
+template <bool SOLO> GGQ_DEV float team_sum(float v, float* red)
 {
     v = wave_sum(v);
-    if constexpr (WAVES > 1) {
-        if ((threadIdx.x & 63u) == 0) red[slot][threadIdx.x >> 6] = v;
+    if constexpr (!SOLO) {
+        if ((threadIdx.x & 63u) == 0) red[threadIdx.x >> 6] = v;
         __syncthreads();
-        v = 0.0f;
-#pragma unroll
-        for (int w = 0; w < WAVES; w++) v += red[slot][w];
+        v = red[threadIdx.x & 15u];
+        v += dpp_f<0xB1, 0xF>(v);
+        v += dpp_f<0x4E, 0xF>(v);
+        v += dpp_f<0x141, 0xF>(v);
+        v += dpp_f<0x140, 0xF>(v);
     }
     return v;
 }
-template <int WAVES> GGQ_DEV uint32_t row_umax(uint32_t v, float (*red)[8], int slot)
+template <bool SOLO> GGQ_DEV uint32_t team_umax(uint32_t v, float* red)
 {
     v = wave_umax(v);
-    if constexpr (WAVES > 1) {
-        if ((threadIdx.x & 63u) == 0) red[slot][threadIdx.x >> 6] = bits_f32(v);
+    if constexpr (!SOLO) {
+        if ((threadIdx.x & 63u) == 0) red[threadIdx.x >> 6] = bits_f32(v);
         __syncthreads();
-        v = 0;
-#pragma unroll
-        for (int w = 0; w < WAVES; w++) v = umax(v, __builtin_bit_cast(uint32_t, red[slot][w]));
+        v = __builtin_bit_cast(uint32_t, red[threadIdx.x & 15u]);
+        v = umax(v, dpp_u<0xB1, 0xF>(v));
+        v = umax(v, dpp_u<0x4E, 0xF>(v));
+        v = umax(v, dpp_u<0x141, 0xF>(v));
+        v = umax(v, dpp_u<0x140, 0xF>(v));
     }
     return v;
 }
@@ -165,130 +170,286 @@ GGQ_DEV void row_scale(uint32_t amax_bits, double& to, float& scale)
     else { to = 127.0 / (double)a; scale = a / 127.0f; }
 }
 
-// One row per WAVES waves; NV vectors of 8 elements per lane.  WAVES = 1: the four waves of a workgroup hold four rows.
-template <int DT, int WAVES, int NV>
-__global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64) void block_norm(const RowArgs a)
+// A row as it was loaded: 8 elements per lane and vector
+template <int DT> struct RowRaw { u32x4 a; };
+template <> struct RowRaw<OUT_F32> { u32x4 a, b; };
+
+template <int DT, bool TAIL> GGQ_DEV RowRaw<DT> row_raw(const uint8_t* p, uint32_t i, uint32_t dim)
 {
-    __shared__ float red[6][8];
-    const uint64_t row = WAVES == 1 ? (uint64_t)blockIdx.x * 4u + (threadIdx.x >> 6) : (uint64_t)blockIdx.x;
-    if (row >= a.rows) return;                                              // a whole wave (WAVES = 1: no barrier follows) or a whole workgroup
-    const uint32_t lane = WAVES == 1 ? threadIdx.x & 63u : threadIdx.x;
-    constexpr uint32_t STEP = WAVES * 64 * 8;
+    RowRaw<DT> r;
     constexpr int EB = DT == OUT_F32 ? 4 : 2;
-    const uint32_t dim = a.dim;
-    const float inv_dim = 1.0f / (float)dim;
-    const uint64_t at = row * dim * EB;
-    const uint64_t sample = row / a.rows_per_mod;
-
-    float r[NV][8];
+    if constexpr (TAIL) {                                       // dim is no multiple of 8: the last vector element by element
+        if (i + 8u > dim) {
+            float v[8];
+            row_load8<DT>(p, i, dim, v);
+            uint32_t w[8];
 #pragma unroll
-    for (int j = 0; j < NV; j++) row_load8<DT>(a.stream + at, lane * 8u + (uint32_t)j * STEP, dim, r[j]);
-
-    // mean and 1 / sqrt(var + eps) of the row in v; padded elements are 0 and stay out of the centred sum
-    auto moments = [&](const float (&v)[NV][8], int kind, int slot, float& mean, float& rstd) {
-        mean = 0.0f;
-        if (kind == NORM_LAYER) {
-            float s = 0.0f;
+            for (int k = 0; k < 8; k++) w[k] = __builtin_bit_cast(uint32_t, v[k]);
+            if constexpr (DT == OUT_F32) { r.a = u32x4{w[0], w[1], w[2], w[3]}; r.b = u32x4{w[4], w[5], w[6], w[7]}; }
+            else {
 #pragma unroll
-            for (int j = 0; j < NV; j++)
-#pragma unroll
-                for (int k = 0; k < 8; k++) s += v[j][k];
-            mean = row_sum<WAVES>(s, red, slot) * inv_dim;
-        }
-        float s = 0.0f;
-#pragma unroll
-        for (int j = 0; j < NV; j++)
-#pragma unroll
-            for (int k = 0; k < 8; k++) {
-                const float d = lane * 8u + (uint32_t)j * STEP + (uint32_t)k < dim ? v[j][k] - mean : 0.0f;
-                s += d * d;
-            }
-        rstd = 1.0f / __builtin_sqrtf(row_sum<WAVES>(s, red, slot + 1) * inv_dim + a.eps);
-    };
-
-    if (a.branch != nullptr) {
-        float h[NV][8];
-#pragma unroll
-        for (int j = 0; j < NV; j++) row_load8<DT>(a.branch + at, lane * 8u + (uint32_t)j * STEP, dim, h[j]);
-        if (a.post_norm != NORM_NONE) {
-            float mean, rstd;
-            moments(h, a.post_norm, 0, mean, rstd);
-#pragma unroll
-            for (int j = 0; j < NV; j++) {
-                float w[8];
-                if (a.post_weight != nullptr) row_param8<DT>(a.post_weight, a.p32 & P32_POST, 0, lane * 8u + (uint32_t)j * STEP, dim, w);
-#pragma unroll
-                for (int k = 0; k < 8; k++) {
-                    h[j][k] = (h[j][k] - mean) * rstd;
-                    if (a.post_weight != nullptr) h[j][k] *= w[k];
+                for (int k = 0; k < 4; k++) {
+                    if constexpr (DT == OUT_F16) r.a[k] = as_u32(h2{(_Float16)v[2 * k], (_Float16)v[2 * k + 1]});
+                    else r.a[k] = (w[2 * k] >> 16) | (w[2 * k + 1] & 0xFFFF0000u);
                 }
             }
+            return r;
         }
+        r.a = __builtin_bit_cast(u32x4, *reinterpret_cast<const u32x4_any*>(p + (uint64_t)i * EB));
+        if constexpr (DT == OUT_F32) r.b = __builtin_bit_cast(u32x4, *reinterpret_cast<const u32x4_any*>(p + (uint64_t)i * EB + 16));
+    } else {
+        const bool in = i < dim;                                // lanes past the row read its start and keep zeros: no branch between the loads of a row
+        const uint8_t* q = p + (uint64_t)(in ? i : 0u) * EB;
+        r.a = __builtin_bit_cast(u32x4, *reinterpret_cast<const u32x4_any*>(q));
+        if constexpr (DT == OUT_F32) r.b = __builtin_bit_cast(u32x4, *reinterpret_cast<const u32x4_any*>(q + 16));
 #pragma unroll
-        for (int j = 0; j < NV; j++) {
-            const uint32_t i = lane * 8u + (uint32_t)j * STEP;
-            if (a.gate != nullptr) {
-                float g[8];
-                row_param8<DT>(a.gate, a.p32 & P32_GATE, sample * a.gate_stride, i, dim, g);
-#pragma unroll
-                for (int k = 0; k < 8; k++) h[j][k] *= g[k];
-            }
-#pragma unroll
-            for (int k = 0; k < 8; k++) r[j][k] = i + (uint32_t)k < dim ? r[j][k] + h[j][k] : 0.0f;
-            if (i < dim) row_store8<DT>(a.stream_out + at, i, dim, r[j]);
+        for (int k = 0; k < 4; k++) {
+            r.a[k] = in ? r.a[k] : 0u;
+            if constexpr (DT == OUT_F32) r.b[k] = in ? r.b[k] : 0u;
         }
     }
-    if (a.y == nullptr) return;                                             // the last block: only the stream is wanted
+    return r;
+}
 
-    if (a.norm != NORM_NONE) {
-        float mean, rstd;
-        moments(r, a.norm, 2, mean, rstd);
+template <int DT> GGQ_DEV void row_unpack(const RowRaw<DT>& r, float (&v)[8])
+{
 #pragma unroll
-        for (int j = 0; j < NV; j++) {
-            const uint32_t i = lane * 8u + (uint32_t)j * STEP;
-            float w[8], b[8], sc[8], sh[8];
-            if (a.weight != nullptr) row_param8<DT>(a.weight, a.p32 & P32_WEIGHT, 0, i, dim, w);
-            if (a.bias != nullptr) row_param8<DT>(a.bias, a.p32 & P32_BIAS, 0, i, dim, b);
-            if (a.scale != nullptr) row_param8<DT>(a.scale, a.p32 & P32_SCALE, sample * a.scale_stride, i, dim, sc);
-            if (a.shift != nullptr) row_param8<DT>(a.shift, a.p32 & P32_SHIFT, sample * a.shift_stride, i, dim, sh);
+    for (int k = 0; k < 4; k++) {
+        if constexpr (DT == OUT_F32) { v[k] = bits_f32(r.a[k]); v[4 + k] = bits_f32(r.b[k]); }
+        else if constexpr (DT == OUT_F16) { const h2 h = as_h2(r.a[k]); v[2 * k] = (float)h.x; v[2 * k + 1] = (float)h.y; }
+        else { v[2 * k] = bits_f32(r.a[k] << 16); v[2 * k + 1] = bits_f32(r.a[k] & 0xFFFF0000u); }
+    }
+}
+
+// What a row is multiplied by, for 8 elements: G = post_weight * gate, A = weight * (1 + scale), B = bias * (1 + scale) + shift (1, 1, 0 where not given; 0
+// past the row's end).  The same for all rows of a sample.
+struct RowFactors { float g[8], a[8], b[8]; };
+
+template <int DT> GGQ_DEV void row_factors(const RowArgs& p, uint64_t sample, uint32_t i, uint32_t dim, RowFactors& f)
+{
+#pragma unroll
+    for (int k = 0; k < 8; k++) { f.g[k] = 1.0f; f.a[k] = 1.0f; f.b[k] = 0.0f; }
+    float v[8];
+    if (p.post_weight != nullptr) row_param8<DT>(p.post_weight, p.p32 & P32_POST, 0, i, dim, f.g);
+    if (p.gate != nullptr) {
+        row_param8<DT>(p.gate, p.p32 & P32_GATE, sample * p.gate_stride, i, dim, v);
+#pragma unroll
+        for (int k = 0; k < 8; k++) f.g[k] *= v[k];
+    }
+    if (p.weight != nullptr) row_param8<DT>(p.weight, p.p32 & P32_WEIGHT, 0, i, dim, f.a);
+    if (p.bias != nullptr) row_param8<DT>(p.bias, p.p32 & P32_BIAS, 0, i, dim, f.b);
+    if (p.scale != nullptr) {
+        row_param8<DT>(p.scale, p.p32 & P32_SCALE, sample * p.scale_stride, i, dim, v);
+#pragma unroll
+        for (int k = 0; k < 8; k++) { f.a[k] *= 1.0f + v[k]; f.b[k] *= 1.0f + v[k]; }
+    }
+    if (p.shift != nullptr) {
+        row_param8<DT>(p.shift, p.p32 & P32_SHIFT, sample * p.shift_stride, i, dim, v);
+#pragma unroll
+        for (int k = 0; k < 8; k++) f.b[k] += v[k];
+    }
+#pragma unroll
+    for (int k = 0; k < 8; k++)
+        if (i + (uint32_t)k >= dim) { f.g[k] = 0.0f; f.a[k] = 0.0f; f.b[k] = 0.0f; }
+}
+
+// Zeros in red[]: what the places of waves that a team does not have hold.
+GGQ_DEV void team_clear(float* red, uint32_t n)
+{
+    for (uint32_t i = threadIdx.x; i < n; i += blockDim.x) red[i] = 0.0f;
+    __syncthreads();
+}
+
+// Rows of up to 16 * 64 * 8 = 8192 elements: 8 per lane, in registers from load to store.  A team of waves takes `rows_per_team` consecutive rows.  SOLO: a team
+// is one wave, four teams to a workgroup, no barrier; else a team is a workgroup of up to 16 waves.  The next row's loads are under way while a row is
+// computed, and a sample's factors stay in registers from row to row (read for every row, they would be up to 14 bytes per element from the caches
+// beside the 8 from memory that the row itself moves).
+template <int DT, bool SOLO, bool TAIL>
+__global__ __launch_bounds__(SOLO ? 256 : 1024) void block_norm(const RowArgs a, uint32_t rows_per_team)
+{
+    constexpr int EB = DT == OUT_F32 ? 4 : 2;
+    __shared__ __attribute__((aligned(16))) float red[2][5][16];            // two rows' reductions: a wave may be one row ahead of another
+    const uint64_t team = SOLO ? (uint64_t)blockIdx.x * 4u + (threadIdx.x >> 6) : (uint64_t)blockIdx.x;
+    const uint64_t first = team * rows_per_team, last = first + rows_per_team < a.rows ? first + rows_per_team : a.rows;
+    if constexpr (!SOLO) team_clear(&red[0][0][0], 160);
+    if (first >= last) return;                                              // a whole wave (SOLO: no barrier follows) or a whole workgroup
+    const uint32_t lane = SOLO ? threadIdx.x & 63u : threadIdx.x;
+    const uint32_t dim = a.dim, i = lane * 8u;
+    const float inv_dim = 1.0f / (float)dim;
+
+    // mean of squares of the row (about its mean: NORM_LAYER) -> mean, 1 / sqrt(mean square + eps); elements past the end are zeros, and stay out of the
+    // centred sum
+    auto moments = [&](const float (&v)[8], int kind, float* at, float& mean, float& rstd) {
+        mean = 0.0f;
+        float s = 0.0f;
+        if (kind == NORM_LAYER) {
+            mean = team_sum<SOLO>(((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7])), at) * inv_dim;
 #pragma unroll
             for (int k = 0; k < 8; k++) {
-                float v = (r[j][k] - mean) * rstd;
-                if (a.weight != nullptr) v *= w[k];
-                if (a.bias != nullptr) v += b[k];
-                if (a.scale != nullptr) v *= 1.0f + sc[k];
-                if (a.shift != nullptr) v += sh[k];
-                r[j][k] = i + (uint32_t)k < dim ? v : 0.0f;
+                const float d = i + (TAIL ? (uint32_t)k : 0u) < dim ? v[k] - mean : 0.0f;
+                s = __builtin_fmaf(d, d, s);
             }
-        }
-    }
-    if (a.y_scale == nullptr) {
+        } else {
 #pragma unroll
-        for (int j = 0; j < NV; j++) {
-            const uint32_t i = lane * 8u + (uint32_t)j * STEP;
-            if (i < dim) row_store8<DT>(a.y + at, i, dim, r[j]);
+            for (int k = 0; k < 8; k++) s = __builtin_fmaf(v[k], v[k], s);
         }
-        return;
+        rstd = 1.0f / __builtin_sqrtf(team_sum<SOLO>(s, at + 16) * inv_dim + a.eps);
+    };
+
+    RowRaw<DT> rs, rb;
+    auto fetch = [&](uint64_t row) {
+        rs = row_raw<DT, TAIL>(a.stream + row * dim * EB, i, dim);
+        if (a.branch != nullptr) rb = row_raw<DT, TAIL>(a.branch + row * dim * EB, i, dim);
+    };
+    fetch(first);
+    RowFactors f;
+    uint64_t sample = first / a.rows_per_mod, sample_end = (sample + 1) * a.rows_per_mod;
+    row_factors<DT>(a, sample, i, dim, f);
+    for (uint64_t row = first; row < last; row++) {
+        float (*slot)[16] = red[(row - first) & 1u];
+        if (row == sample_end) {
+            sample++;
+            sample_end += a.rows_per_mod;
+            row_factors<DT>(a, sample, i, dim, f);
+        }
+        float r[8], h[8];
+        row_unpack<DT>(rs, r);
+        if (a.branch != nullptr) row_unpack<DT>(rb, h);
+        if (row + 1 < last) fetch(row + 1);
+        const uint64_t at = row * dim * EB;
+        if (a.branch != nullptr) {
+            float mean = 0.0f, rstd = 1.0f;
+            if (a.post_norm != NORM_NONE) moments(h, a.post_norm, slot[0], mean, rstd);
+#pragma unroll
+            for (int k = 0; k < 8; k++) r[k] = __builtin_fmaf((h[k] - mean) * rstd, f.g[k], r[k]);
+            if (i < dim) row_store8<DT>(a.stream_out + at, i, TAIL ? dim : ~0u, r);
+        }
+        if (a.y == nullptr) continue;                                       // the last block: only the stream is wanted
+        if (a.norm != NORM_NONE) {
+            float mean, rstd;
+            moments(r, a.norm, slot[2], mean, rstd);
+#pragma unroll
+            for (int k = 0; k < 8; k++) r[k] = __builtin_fmaf((r[k] - mean) * rstd, f.a[k], f.b[k]);
+        }
+        if (a.y_scale == nullptr) {
+            if (i < dim) row_store8<DT>(a.y + at, i, TAIL ? dim : ~0u, r);
+            continue;
+        }
+        uint32_t top = 0;
+#pragma unroll
+        for (int k = 0; k < 8; k++) top = umax(top, __builtin_bit_cast(uint32_t, r[k]) & 0x7FFFFFFFu);
+        double to;
+        float scale;
+        row_scale(team_umax<SOLO>(top, slot[4]), to, scale);
+        if (lane == 0) a.y_scale[row] = scale;
+        if (i < a.y_stride) {
+#pragma unroll
+            for (int k = 0; k < 8; k++) r[k] = to == 0.0 ? 0.0f : r[k];
+            *reinterpret_cast<u32x2*>(a.y + row * a.y_stride + i) = row_quant8(r, to);
+        }
     }
+}
+
+// Longer rows, up to 32768 elements: a workgroup per row, the row in LDS as fp32 (each lane reads back what it wrote itself: no barrier for that).
+constexpr uint32_t ROW_LONG_THREADS = 1024;
+template <int DT>
+__global__ __launch_bounds__(1024) void block_norm_long(const RowArgs a)
+{
+    constexpr int EB = DT == OUT_F32 ? 4 : 2;
+    __shared__ __attribute__((aligned(16))) float red[5][16];
+    extern __shared__ __attribute__((aligned(16))) uint8_t dyn[];
+    const uint32_t dim = a.dim, span = a.y_scale != nullptr ? (uint32_t)a.y_stride : dim;
+    const uint64_t row = blockIdx.x, at = row * dim * EB, sample = row / a.rows_per_mod;
+    const float inv_dim = 1.0f / (float)dim;
+    team_clear(&red[0][0], 80);
+    f32x4* mine = reinterpret_cast<f32x4*>(dyn) + threadIdx.x * 2u;         // vector j of this lane: mine[2048 j], mine[2048 j + 1]
+    auto get = [&](uint32_t i, float (&v)[8]) {
+        const f32x4 p = mine[i / (ROW_LONG_THREADS * 8u) * (ROW_LONG_THREADS * 2u)], q = mine[i / (ROW_LONG_THREADS * 8u) * (ROW_LONG_THREADS * 2u) + 1u];
+#pragma unroll
+        for (int k = 0; k < 4; k++) { v[k] = p[k]; v[4 + k] = q[k]; }
+    };
+    auto put = [&](uint32_t i, const float (&v)[8]) {
+        mine[i / (ROW_LONG_THREADS * 8u) * (ROW_LONG_THREADS * 2u)] = f32x4{v[0], v[1], v[2], v[3]};
+        mine[i / (ROW_LONG_THREADS * 8u) * (ROW_LONG_THREADS * 2u) + 1u] = f32x4{v[4], v[5], v[6], v[7]};
+    };
+    auto each = [&](auto&& f) {
+#pragma unroll 1
+        for (uint32_t i = threadIdx.x * 8u; i < span; i += ROW_LONG_THREADS * 8u) f(i);
+    };
+    auto moments = [&](auto&& load, int kind, float* slot, float& mean, float& rstd) {
+        mean = 0.0f;
+        float s = 0.0f;
+        if (kind == NORM_LAYER) {
+            each([&](uint32_t i) {
+                float v[8];
+                load(i, v);
+                s += ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
+            });
+            mean = team_sum<false>(s, slot) * inv_dim;
+            s = 0.0f;
+        }
+        each([&](uint32_t i) {
+            float v[8];
+            load(i, v);
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                const float d = i + (uint32_t)k < dim ? v[k] - mean : 0.0f;
+                s = __builtin_fmaf(d, d, s);
+            }
+        });
+        rstd = 1.0f / __builtin_sqrtf(team_sum<false>(s, slot + 16) * inv_dim + a.eps);
+    };
+    float mean = 0.0f, rstd = 1.0f;
+    auto branch = [&](uint32_t i, float (&v)[8]) { row_load8<DT>(a.branch + at, i, dim, v); };
+    if (a.branch != nullptr && a.post_norm != NORM_NONE) moments(branch, a.post_norm, red[0], mean, rstd);
+    each([&](uint32_t i) {
+        float r[8];
+        row_load8<DT>(a.stream + at, i, dim, r);
+        if (a.branch != nullptr) {
+            float h[8];
+            branch(i, h);
+            RowFactors f;
+            row_factors<DT>(a, sample, i, dim, f);
+#pragma unroll
+            for (int k = 0; k < 8; k++) r[k] = __builtin_fmaf((h[k] - mean) * rstd, f.g[k], r[k]);
+            if (i < dim) row_store8<DT>(a.stream_out + at, i, dim, r);
+        }
+        put(i, r);
+    });
+    if (a.y == nullptr) return;
+    mean = 0.0f;
+    rstd = 1.0f;
+    if (a.norm != NORM_NONE) moments(get, a.norm, red[2], mean, rstd);
     uint32_t top = 0;
+    each([&](uint32_t i) {
+        float r[8];
+        get(i, r);
+        if (a.norm != NORM_NONE) {
+            RowFactors f;
+            row_factors<DT>(a, sample, i, dim, f);
 #pragma unroll
-    for (int j = 0; j < NV; j++)
+            for (int k = 0; k < 8; k++) r[k] = __builtin_fmaf((r[k] - mean) * rstd, f.a[k], f.b[k]);
+        }
+        if (a.y_scale == nullptr) {
+            row_store8<DT>(a.y + at, i, dim, r);
+        } else {
+            put(i, r);
 #pragma unroll
-        for (int k = 0; k < 8; k++) top = umax(top, __builtin_bit_cast(uint32_t, r[j][k]) & 0x7FFFFFFFu);
+            for (int k = 0; k < 8; k++) top = umax(top, __builtin_bit_cast(uint32_t, r[k]) & 0x7FFFFFFFu);
+        }
+    });
+    if (a.y_scale == nullptr) return;
     double to;
     float scale;
-    row_scale(row_umax<WAVES>(top, red, 4), to, scale);
-    if (lane == 0) a.y_scale[row] = scale;
+    row_scale(team_umax<false>(top, red[4]), to, scale);
+    if (threadIdx.x == 0) a.y_scale[row] = scale;
+    each([&](uint32_t i) {
+        float r[8];
+        get(i, r);
 #pragma unroll
-    for (int j = 0; j < NV; j++) {
-        const uint32_t i = lane * 8u + (uint32_t)j * STEP;
-        if (i < a.y_stride) {
-            float v[8];
-#pragma unroll
-            for (int k = 0; k < 8; k++) v[k] = to == 0.0 ? 0.0f : r[j][k];
-            *reinterpret_cast<u32x2*>(a.y + row * a.y_stride + i) = row_quant8(v, to);
-        }
-    }
+        for (int k = 0; k < 8; k++) r[k] = to == 0.0 ? 0.0f : r[k];
+        *reinterpret_cast<u32x2*>(a.y + row * a.y_stride + i) = row_quant8(r, to);
+    });
 }
 
 }  // namespace ggq

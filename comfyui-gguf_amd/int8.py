@@ -54,7 +54,7 @@ def _quantize(x):
 
 def quantize_rows(x):
     """-> (q, scale): q int8 of x's shape with rows a multiple of 16 bytes apart, scale fp32 of x's leading dimensions; x ~ q * scale[..., None].
-    x: (..., k) fp16 / bf16 / fp32 on the GPU, 1 <= k <= 24576.  A row of zeros has scale 0; a row with an infinity or a NaN has q = 0 and scale NaN."""
+    x: (..., k) fp16 / bf16 / fp32 on the GPU, 1 <= k <= 32768.  A row of zeros has scale 0; a row with an infinity or a NaN has q = 0 and scale NaN."""
     if _is_compiling():
         return _eager_quantize(x)
     return _quantize_rows(x)

@@ -18,7 +18,7 @@ from . import _native
 from .dequant import GGQUnsupported, _DEVICE_OK, _OUT_CODE, _cur_device, _device_served, _is_compiling, _raw_stream, dequantize_tensor, is_quantized
 
 NORMS = {None: 0, "none": 0, "rms": 1, "layer": 2}
-MAX_DIM = 24576                    # elements of a row: they live in the registers of one workgroup
+MAX_DIM = 32768                    # elements of a row: they live in the registers or the LDS of one workgroup
 _call = None
 
 

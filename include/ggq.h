@@ -218,7 +218,7 @@ uint64_t ggq_linear_mfma_workspace(int qtype, uint32_t rows, uint32_t cols, uint
  * the six may be NULL.  params_f32: bit i set = parameter i (order: post_weight, gate, weight, bias, scale, shift) holds fp32, else `dtype`.
  * y_scale NULL: y is rows x dim of `dtype`.  y_scale given: y is int8 rows y_stride BYTES apart (a multiple of 16, >= dim; bytes past dim are
  * written as 0) with y ~ q * y_scale[row], q = rint(127 y / max|row|), y_scale = max|row| / 127; a row with an infinity or a NaN: q = 0, scale NaN.
- * stream_out may be stream, y may be branch.  GGQ_ERR_ARG: rows longer than 24576 elements.  Arithmetic in fp32 from load to store.
+ * stream_out may be stream, y may be branch.  GGQ_ERR_ARG: rows longer than 32768 elements.  Arithmetic in fp32 from load to store.
  * Replaces: nothing of the reference's own code -- the torch operations that the models it loads run between GGMLOps.Linear calls
  * (ops.py:242-244), and GGMLOps.LayerNorm (ops.py:262-266). */
 typedef struct ggq_norm_desc {

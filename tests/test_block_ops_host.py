@@ -38,7 +38,7 @@ def test_block_norm_arguments_at_the_c_entry(pkg):
     assert L.ggq_block_norm(None, None) == n.GGQ_ERR_ARG
     assert call(rows=0) == n.GGQ_OK
     for bad in (dict(dtype=3), dict(dtype=-1), dict(norm=3), dict(post_norm=-1), dict(dim=0), dict(rows_per_mod=0), dict(stream=None), dict(branch=A), dict(y=None),
-                dict(y_scale=A, y_stride=63), dict(y_scale=A, y_stride=72), dict(y_scale=A, y=None, branch=A, stream_out=A, y_stride=64), dict(dim=24577), dict(rows=1 << 40)):
+                dict(y_scale=A, y_stride=63), dict(y_scale=A, y_stride=72), dict(y_scale=A, y=None, branch=A, stream_out=A, y_stride=64), dict(dim=32769), dict(rows=1 << 40)):
         assert call(**bad) == n.GGQ_ERR_ARG, bad
     for bad in (dict(stream=A + 1), dict(y=A + 1), dict(y_scale=A, y_stride=64, y=A + 8), dict(weight=A + 1), dict(weight=A + 2, params_f32=4), dict(dtype=n.F32, stream=A + 2)):
         assert call(**bad) == n.GGQ_ERR_ALIGN, bad
@@ -48,7 +48,7 @@ def test_quantize_and_product_arguments_at_the_c_entry(pkg):
     n, L = pkg._native, _lib(pkg)
     q = lambda x=A, rows=4, cols=64, to=A, stride=64, s=A, dt=n.F16: L.ggq_quantize_rows(x, rows, cols, to, stride, s, dt, None)  # noqa: E731
     assert q(rows=0) == n.GGQ_OK
-    for rc in (q(x=None), q(to=None), q(s=None), q(cols=0), q(stride=48), q(stride=65), q(dt=3), q(cols=24577, stride=24592)):
+    for rc in (q(x=None), q(to=None), q(s=None), q(cols=0), q(stride=48), q(stride=65), q(dt=3), q(cols=32769, stride=32784)):
         assert rc == n.GGQ_ERR_ARG
     assert q(to=A + 8) == n.GGQ_ERR_ALIGN and q(x=A + 1) == n.GGQ_ERR_ALIGN
     p = lambda x=A, xs=64, sx=A, m=4, w=A, ws=64, sw=A, rows=4, k=64, b=None, y=A, dt=n.F16: L.ggq_linear_int8(x, xs, sx, m, w, ws, sw, rows, k, b, y, dt, None)  # noqa: E731

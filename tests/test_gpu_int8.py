@@ -164,7 +164,7 @@ def test_refusals_on_the_gpu(pkg):
     with pytest.raises(no, match="autograd"):
         L(x.clone().requires_grad_(), w, s)
     with pytest.raises(no):
-        pkg.int8.quantize_rows(torch.zeros(2, 24577, device=DEV))
+        pkg.int8.quantize_rows(torch.zeros(2, 32769, device=DEV))
 
 
 def test_the_layer(pkg):

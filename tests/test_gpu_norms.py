@@ -72,7 +72,11 @@ CASES = [
     (3, 700, 513, "layer", "layer", ("gate", "scale", "shift", "post_weight", "weight", "bias"), ("bias", "gate")),
     (1, 5, 1, "rms", "rms", ("weight",), ()),
     (1, 7, 7, "layer", None, ("weight", "bias", "scale"), ("scale",)),
-    (2, 2, 24576, "rms", None, ("weight", "shift"), ()),                                                # the longest rows
+    (2, 2, 24576, "rms", None, ("weight", "shift"), ()),                                                # rows in LDS, the longest below
+    (2, 3, 32768, "layer", "layer", ("gate", "weight", "bias", "scale"), ("weight", "gate")),
+    (1, 9, 8193, "rms", "rms", ("gate", "post_weight"), ("post_weight",)),
+    (5, 1001, 200, "rms", None, ("gate", "scale", "shift"), ()),                                        # a team's rows cross from sample to sample
+    (900, 7, 1032, "layer", None, ("gate", "shift", "weight"), ()),
     (1, 300, 4097, "layer", None, (), ()),
     (1, 4, 1000, None, None, ("gate",), ()),                                                            # only the stream
     (1, 2500, 4100, "rms", None, ("gate", "weight"), ("weight",)),                                      # more than a wave's registers hold
@@ -188,7 +192,7 @@ def test_refusals_on_the_gpu(pkg):
                 dict(weight=x[0]), dict(branch=x, gate=x[0, :, :32]), dict(branch=x, gate=x[0]), dict(branch=x, gate=x, scale=x[:, :1]), dict(post_weight=x[0, 0], branch=x)):
         with pytest.raises(no):
             B(x, **bad)
-    for other in (x.double(), x.cpu(), torch.zeros(2, 0, device=DEV), torch.zeros(1, 24577, device=DEV)):
+    for other in (x.double(), x.cpu(), torch.zeros(2, 0, device=DEV), torch.zeros(1, 32769, device=DEV)):
         with pytest.raises(no):
             B(other)
     with pytest.raises(no, match="autograd"):
