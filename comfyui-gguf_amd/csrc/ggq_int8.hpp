@@ -137,19 +137,45 @@ __global__ __launch_bounds__(WM * WN * 64) void linear_i8_tile(const I8Args a)
         }
     }
 
-    // D[row = 8 (i / 4) + 4 h + i % 4][column = r32] = sum of (row of w, row of x)
+    // D[row = 8 (i / 4) + 4 h + i % 4][column = r32] = sum of (row of w, row of x): four consecutive columns of y per lane and register group.  Each wave turns
+    // 32 rows x (TN / WN) columns of sums through its own part of LDS, so that a lane then holds 8 consecutive columns of a row (whose scales and bias it keeps)
+    // and a row is stored in full lines.  (Stored straight from the accumulators, 2 bytes at a time, the epilogue took longer than the product.)
+    constexpr uint32_t COLS = TN / WN, LPR = COLS / 8, RPI = 64 / LPR;      // columns of a wave, lanes per row, rows per store instruction
+    constexpr uint32_t SLOTS = COLS / 4;                                    // 16-byte places of a row in LDS, XOR-swizzled by the row
+    static_assert(WM * WN * 32 * COLS * 4 <= 2 * STAGE, "the turned sums fit the staging buffers");
+    __syncthreads();                                                        // every wave is done with the staging buffers
+    int* turn = reinterpret_cast<int*>(smem) + wave * (32u * COLS);
+    const uint32_t nc = n0 + wn * COLS + (lane % LPR) * 8u;
+    float sw[8], bias[8];
+#pragma unroll
+    for (int k = 0; k < 8; k++) {
+        const uint32_t c = nc + (uint32_t)k < a.n ? nc + (uint32_t)k : a.n - 1u;
+        sw[k] = a.w_scale[c];
+        bias[k] = i8_bias<DT>(a.bias, c);
+    }
 #pragma unroll
     for (int mt = 0; mt < MT; mt++) {
-        const uint32_t mr = m0 + wm * (TM / WM) + 32u * (uint32_t)mt + r32;
-        if (mr >= a.m) continue;
-        const float sx = a.x_scale[mr];
 #pragma unroll
         for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-            for (int i = 0; i < 16; i++) {
-                const uint32_t nc = n0 + wn * (TN / WN) + 32u * (uint32_t)nt + 8u * (uint32_t)(i >> 2) + 4u * h + (uint32_t)(i & 3);
-                if (nc < a.n) i8_store<DT>(a.y, (uint64_t)mr * a.n + nc, (float)acc[nt][mt][i] * (sx * a.w_scale[nc]) + i8_bias<DT>(a.bias, nc));
+            for (int g = 0; g < 4; g++)
+                *reinterpret_cast<i32x4*>(turn + r32 * COLS + (((uint32_t)(8 * nt + 2 * g) + h) ^ (r32 & (SLOTS - 1u))) * 4u) =
+                    i32x4{acc[nt][mt][4 * g], acc[nt][mt][4 * g + 1], acc[nt][mt][4 * g + 2], acc[nt][mt][4 * g + 3]};
+        wave_sync();
+#pragma unroll
+        for (uint32_t i = 0; i < 32u / RPI; i++) {
+            const uint32_t row = i * RPI + lane / LPR, mr = m0 + wm * (TM / WM) + 32u * (uint32_t)mt + row;
+            const i32x4 p = *reinterpret_cast<const i32x4*>(turn + row * COLS + (((lane % LPR) * 2u) ^ (row & (SLOTS - 1u))) * 4u);
+            const i32x4 q = *reinterpret_cast<const i32x4*>(turn + row * COLS + (((lane % LPR) * 2u + 1u) ^ (row & (SLOTS - 1u))) * 4u);
+            if (mr < a.m && nc < a.n) {
+                const float sx = a.x_scale[mr];
+                float v[8];
+#pragma unroll
+                for (int k = 0; k < 8; k++) v[k] = (float)(k < 4 ? p[k] : q[k - 4]) * (sx * sw[k]) + bias[k];
+                row_store8<DT>(a.y + (uint64_t)mr * a.n * (DT == OUT_F32 ? 4 : 2), nc, a.n, v);
             }
+        }
+        wave_sync();
     }
 }
 

@@ -21,7 +21,7 @@ int launch_rows(const RowArgs& a, int dtype, hipStream_t s)
     const uint64_t span = a.y_scale != nullptr ? a.y_stride : a.dim;       // elements a row's lanes have to cover (8-bit rows: their zero padding too)
     if (span > MAX_DIM) return GGQ_ERR_ARG;
     const uint32_t vecs = (uint32_t)((span + 7) / 8);
-    if (vecs > 1024u) {
+    if (vecs > (a.dim % 8 != 0 ? 512u : 1024u)) {
         if (a.rows > 0x7FFFFFFFull) return GGQ_ERR_ARG;
         static std::atomic<uint64_t> raised[3];
         hipError_t e = allow_lds(reinterpret_cast<const void*>(LONG_ROWS[dtype]), MAX_DIM * 4, raised[dtype]);

@@ -98,12 +98,6 @@ template <int DT> GGQ_DEV void row_store8(uint8_t* p, uint32_t i, uint32_t dim, 
     }
 }
 
-template <int DT> GGQ_DEV void row_param8(const uint8_t* p, bool is32, uint64_t base, uint32_t i, uint32_t dim, float (&v)[8])
-{
-    if (is32) row_load8<OUT_F32>(p + base * 4, i, dim, v);
-    else row_load8<DT>(p + base * (DT == OUT_F32 ? 4 : 2), i, dim, v);
-}
-
 template <int CTRL, int ROWS> GGQ_DEV uint32_t dpp_u(uint32_t v) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, false); }
 GGQ_DEV uint32_t umax(uint32_t a, uint32_t b) { return a > b ? a : b; }
 
@@ -225,32 +219,57 @@ template <int DT> GGQ_DEV void row_unpack(const RowRaw<DT>& r, float (&v)[8])
 // past the row's end).  The same for all rows of a sample.
 struct RowFactors { float g[8], a[8], b[8]; };
 
-template <int DT> GGQ_DEV void row_factors(const RowArgs& p, uint64_t sample, uint32_t i, uint32_t dim, RowFactors& f)
+// `n` values of a parameter, widened: the loads only (their use comes after all parameters' loads)
+struct RowParam { u32x4 a, b; };
+template <int DT, bool TAIL> GGQ_DEV RowParam row_param_raw(const uint8_t* p, bool is32, uint64_t base, uint32_t i, uint32_t dim)
 {
+    RowParam r{};
+    if (p == nullptr) return r;
+    if (DT == OUT_F32 || is32) {
+        const RowRaw<OUT_F32> w = row_raw<OUT_F32, TAIL>(p + base * 4, i, dim);
+        r.a = w.a;
+        r.b = w.b;
+    } else {
+        r.a = row_raw<DT, TAIL>(p + base * (DT == OUT_F32 ? 4 : 2), i, dim).a;
+    }
+    return r;
+}
+template <int DT> GGQ_DEV void row_param_unpack(const RowParam& r, bool is32, float (&v)[8])
+{
+    if (DT == OUT_F32 || is32) row_unpack<OUT_F32>(RowRaw<OUT_F32>{r.a, r.b}, v);
+    else if constexpr (DT != OUT_F32) row_unpack<DT>(RowRaw<DT>{r.a}, v);
+}
+
+template <int DT, bool TAIL> GGQ_DEV void row_factors(const RowArgs& p, uint64_t sample, uint32_t i, uint32_t dim, RowFactors& f)
+{
+    const RowParam post = row_param_raw<DT, TAIL>(p.post_weight, p.p32 & P32_POST, 0, i, dim), gate = row_param_raw<DT, TAIL>(p.gate, p.p32 & P32_GATE, sample * p.gate_stride, i, dim);
+    const RowParam weight = row_param_raw<DT, TAIL>(p.weight, p.p32 & P32_WEIGHT, 0, i, dim), bias = row_param_raw<DT, TAIL>(p.bias, p.p32 & P32_BIAS, 0, i, dim);
+    const RowParam scale = row_param_raw<DT, TAIL>(p.scale, p.p32 & P32_SCALE, sample * p.scale_stride, i, dim);
+    const RowParam shift = row_param_raw<DT, TAIL>(p.shift, p.p32 & P32_SHIFT, sample * p.shift_stride, i, dim);
+    float v[8];
 #pragma unroll
     for (int k = 0; k < 8; k++) { f.g[k] = 1.0f; f.a[k] = 1.0f; f.b[k] = 0.0f; }
-    float v[8];
-    if (p.post_weight != nullptr) row_param8<DT>(p.post_weight, p.p32 & P32_POST, 0, i, dim, f.g);
+    if (p.post_weight != nullptr) row_param_unpack<DT>(post, p.p32 & P32_POST, f.g);
     if (p.gate != nullptr) {
-        row_param8<DT>(p.gate, p.p32 & P32_GATE, sample * p.gate_stride, i, dim, v);
+        row_param_unpack<DT>(gate, p.p32 & P32_GATE, v);
 #pragma unroll
         for (int k = 0; k < 8; k++) f.g[k] *= v[k];
     }
-    if (p.weight != nullptr) row_param8<DT>(p.weight, p.p32 & P32_WEIGHT, 0, i, dim, f.a);
-    if (p.bias != nullptr) row_param8<DT>(p.bias, p.p32 & P32_BIAS, 0, i, dim, f.b);
+    if (p.weight != nullptr) row_param_unpack<DT>(weight, p.p32 & P32_WEIGHT, f.a);
+    if (p.bias != nullptr) row_param_unpack<DT>(bias, p.p32 & P32_BIAS, f.b);
     if (p.scale != nullptr) {
-        row_param8<DT>(p.scale, p.p32 & P32_SCALE, sample * p.scale_stride, i, dim, v);
+        row_param_unpack<DT>(scale, p.p32 & P32_SCALE, v);
 #pragma unroll
         for (int k = 0; k < 8; k++) { f.a[k] *= 1.0f + v[k]; f.b[k] *= 1.0f + v[k]; }
     }
     if (p.shift != nullptr) {
-        row_param8<DT>(p.shift, p.p32 & P32_SHIFT, sample * p.shift_stride, i, dim, v);
+        row_param_unpack<DT>(shift, p.p32 & P32_SHIFT, v);
 #pragma unroll
         for (int k = 0; k < 8; k++) f.b[k] += v[k];
     }
 #pragma unroll
     for (int k = 0; k < 8; k++)
-        if (i + (uint32_t)k >= dim) { f.g[k] = 0.0f; f.a[k] = 0.0f; f.b[k] = 0.0f; }
+        if (i + (TAIL ? (uint32_t)k : 0u) >= dim) { f.g[k] = 0.0f; f.a[k] = 0.0f; f.b[k] = 0.0f; }
 }
 
 // Zeros in red[]: what the places of waves that a team does not have hold.
@@ -260,12 +279,12 @@ GGQ_DEV void team_clear(float* red, uint32_t n)
     __syncthreads();
 }
 
-// Rows of up to 16 * 64 * 8 = 8192 elements: 8 per lane, in registers from load to store.  A team of waves takes `rows_per_team` consecutive rows.  SOLO: a team
+// Rows of up to 16 * 64 * 8 = 8192 elements (4096 where their number is no multiple of 8: the registers): 8 per lane, in registers from load to store.  A team of waves takes `rows_per_team` consecutive rows.  SOLO: a team
 // is one wave, four teams to a workgroup, no barrier; else a team is a workgroup of up to 16 waves.  The next row's loads are under way while a row is
 // computed, and a sample's factors stay in registers from row to row (read for every row, they would be up to 14 bytes per element from the caches
 // beside the 8 from memory that the row itself moves).
 template <int DT, bool SOLO, bool TAIL>
-__global__ __launch_bounds__(SOLO ? 256 : 1024) void block_norm(const RowArgs a, uint32_t rows_per_team)
+__global__ __launch_bounds__(SOLO ? 256 : TAIL ? 512 : 1024) void block_norm(const RowArgs a, uint32_t rows_per_team)
 {
     constexpr int EB = DT == OUT_F32 ? 4 : 2;
     __shared__ __attribute__((aligned(16))) float red[2][5][16];            // two rows' reductions: a wave may be one row ahead of another
@@ -304,13 +323,13 @@ __global__ __launch_bounds__(SOLO ? 256 : 1024) void block_norm(const RowArgs a,
     fetch(first);
     RowFactors f;
     uint64_t sample = first / a.rows_per_mod, sample_end = (sample + 1) * a.rows_per_mod;
-    row_factors<DT>(a, sample, i, dim, f);
+    row_factors<DT, TAIL>(a, sample, i, dim, f);
     for (uint64_t row = first; row < last; row++) {
         float (*slot)[16] = red[(row - first) & 1u];
         if (row == sample_end) {
             sample++;
             sample_end += a.rows_per_mod;
-            row_factors<DT>(a, sample, i, dim, f);
+            row_factors<DT, TAIL>(a, sample, i, dim, f);
         }
         float r[8], h[8];
         row_unpack<DT>(rs, r);
@@ -409,7 +428,7 @@ __global__ __launch_bounds__(1024) void block_norm_long(const RowArgs a)
             float h[8];
             branch(i, h);
             RowFactors f;
-            row_factors<DT>(a, sample, i, dim, f);
+            row_factors<DT, true>(a, sample, i, dim, f);
 #pragma unroll
             for (int k = 0; k < 8; k++) r[k] = __builtin_fmaf((h[k] - mean) * rstd, f.g[k], r[k]);
             if (i < dim) row_store8<DT>(a.stream_out + at, i, dim, r);
@@ -426,7 +445,7 @@ __global__ __launch_bounds__(1024) void block_norm_long(const RowArgs a)
         get(i, r);
         if (a.norm != NORM_NONE) {
             RowFactors f;
-            row_factors<DT>(a, sample, i, dim, f);
+            row_factors<DT, true>(a, sample, i, dim, f);
 #pragma unroll
             for (int k = 0; k < 8; k++) r[k] = __builtin_fmaf((r[k] - mean) * rstd, f.a[k], f.b[k]);
         }

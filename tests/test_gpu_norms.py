@@ -79,6 +79,7 @@ CASES = [
     (900, 7, 1032, "layer", None, ("gate", "shift", "weight"), ()),
     (1, 300, 4097, "layer", None, (), ()),
     (1, 4, 1000, None, None, ("gate",), ()),                                                            # only the stream
+    (2, 260, 5001, "layer", None, ("gate", "scale", "bias"), ("gate",)),                                # an odd length beyond the registers
     (1, 2500, 4100, "rms", None, ("gate", "weight"), ("weight",)),                                      # more than a wave's registers hold
 ]
 
