@@ -9,19 +9,17 @@ using namespace ggq;
 
 constexpr uint32_t MAX_K = 131071;                 // 128 * 128 * k stays below 2^31
 
-template <int DT, int TM, int TN, int WM, int WN>
+template <int DT, int TM, int TN, int WM, int WN, int KS, int NB>
 hipError_t launch_tile(I8Args a, hipStream_t s)
 {
-    constexpr uint32_t lds = 2u * (TM + TN) * I8_BK;
-    if (lds > 64 * 1024) {
-        static std::atomic<uint64_t> raised{0};
-        const hipError_t e = allow_lds(reinterpret_cast<const void*>(&linear_i8_tile<DT, TM, TN, WM, WN>), (int)lds, raised);
-        if (e != hipSuccess) return e;
-    }
+    constexpr uint32_t lds = NB * (TM + TN) * I8_BK;
+    static std::atomic<uint64_t> raised{0};
+    const hipError_t e = allow_lds(reinterpret_cast<const void*>(&linear_i8_tile<DT, TM, TN, WM, WN, KS, NB>), (int)lds, raised);
+    if (e != hipSuccess) return e;
     a.tiles_m = (a.m + TM - 1) / TM;
     a.tiles_n = (a.n + TN - 1) / TN;
     if ((uint64_t)a.tiles_m * a.tiles_n > 0x7FFFFFFFull) return hipErrorInvalidValue;
-    hipLaunchKernelGGL((linear_i8_tile<DT, TM, TN, WM, WN>), dim3(a.tiles_m * a.tiles_n), dim3(WM * WN * 64), lds, s, a);
+    hipLaunchKernelGGL((linear_i8_tile<DT, TM, TN, WM, WN, KS, NB>), dim3(a.tiles_m * a.tiles_n), dim3(WM * WN * KS * 64), lds, s, a);
     return hipGetLastError();
 }
 
@@ -36,10 +34,15 @@ template <int DT>
 hipError_t launch(const I8Args& a, hipStream_t s)
 {
     if (a.m <= 16) return launch_rows16<DT>(a, s);
-    const uint64_t big = (uint64_t)((a.m + 255u) / 256u) * ((a.n + 255u) / 256u);
-    if (big >= 256) return launch_tile<DT, 256, 256, 2, 4>(a, s);
-    if (a.m > 64) return launch_tile<DT, 128, 128, 2, 2>(a, s);
-    return launch_tile<DT, 64, 64, 2, 2>(a, s);
+    // The tile that finishes first: rounds of workgroups over the chip times what a step of 128 k takes, in ns, measured at 256 x 4096 x 4096 (a part of the
+    // chip) and 512 ... 4608 x 10240 x 4096 (all of it): 256 x 256 1550 (one workgroup per CU: 128 KiB of LDS); 128 x 128 720 alone on a CU, 1200 for two;
+    // 64 x 64 410, also for two.
+    auto tiles = [&](uint64_t t) { return ((a.m + t - 1) / t) * ((a.n + t - 1) / t); };
+    const uint64_t t128 = tiles(128);
+    const uint64_t big = (tiles(256) + 255) / 256 * 1550, mid = t128 <= 256 ? 720 : (t128 + 511) / 512 * 1200, small = (tiles(64) + 511) / 512 * 410;
+    if (small <= mid && small <= big) return launch_tile<DT, 64, 64, 1, 2, 2, 4>(a, s);
+    if (mid < big) return launch_tile<DT, 128, 128, 2, 2, 1, 2>(a, s);
+    return launch_tile<DT, 256, 256, 2, 4, 1, 2>(a, s);
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }

@@ -5,7 +5,7 @@
 //
 // Two kernels:
 //   linear_i8_tile   many rows of x: a workgroup owns TM rows of x  x  TN rows of w, both staged through LDS 128 bytes of k at a time (LDS-DMA, two
-//                    buffers), every fragment one ds_read_b128.  Bound by the matrix cores' rate.
+//                    to four buffers), every fragment one ds_read_b128.  Bound by the matrix cores' rate.
 //   linear_i8_rows   up to 16 rows of x: a workgroup owns 16 rows of w, its waves split k, operands go straight from memory to registers.  Bound by
 //                    reading w once.
 // The contraction index may be permuted as long as both operands agree; out-of-range rows are clamped and their results not stored; columns of k past
@@ -53,28 +53,40 @@ struct I8Args {
     uint32_t m, n, k, tiles_m, tiles_n;
 };
 
-// TM x TN outputs per workgroup, WM x WN waves of (TM / WM) x (TN / WN) outputs each.  w is the A operand (rows of D = columns of y), x the B operand:
-// a lane holds 4 consecutive columns of one row of y.
-template <int DT, int TM, int TN, int WM, int WN>
-__global__ __launch_bounds__(WM * WN * 64) void linear_i8_tile(const I8Args a)
+// TM x TN outputs per workgroup of WM x WN x KS waves: (TM / WM) x (TN / WN) outputs per wave, KS waves sharing them and splitting each step's k.  w is the A
+// operand (rows of D = columns of y), x the B operand.
+//
+// A step's fragments are read one k-piece ahead of the matrix instructions that use them, across the barrier too: the barrier that publishes step s + 1
+// stands BEFORE the last k-piece of step s is multiplied, so that the first fragments of s + 1 arrive under it.  At that barrier every wave has read
+// step s completely, so its buffer takes the loads of step s + 2 (NB = 2), or step s + 3's went to the buffer of step s - 1 when step s began (NB = 4).
+// With 256 x 256 the reads (24 x 64 x 16 bytes per wave and step) and the LDS-DMA writes take as long as the matrix instructions (32 per wave, 32 cycles each):
+// they have to overlap completely, hence the interleaved issue order that sched_group_barrier asks for.
+//
+// Measured (4608 x 9728 x 2432 / 4608 x 10240 x 4096, us): fragments read where they are used 151 / 206, tiles in groups of 4 rows of tiles (L2) 126 / 203, read one
+// piece ahead 130 / 193, and interleaved 122 / 188 = 1786 / 2054 TOP/s; 4 waves of 128 x 128 137 / 203; 64 bytes of k and 4 buffers 131 / 204.
+template <int DT, int TM, int TN, int WM, int WN, int KS, int NB>
+__global__ __launch_bounds__(WM * WN * KS * 64) void linear_i8_tile(const I8Args a)
 {
-    constexpr int THREADS = WM * WN * 64;
+    constexpr int THREADS = WM * WN * KS * 64;
     constexpr int MT = TM / WM / 32, NT = TN / WN / 32;
     constexpr int UNITS = (TM + TN) * 8, UN = UNITS / THREADS;
-    static_assert(UNITS % THREADS == 0 && MT >= 1 && NT >= 1 && TM % 16 == 0, "tile shape");
+    constexpr int KK = 4 / KS;                                              // k-pieces of 32 per wave and step
+    static_assert(UNITS % THREADS == 0 && MT >= 1 && NT >= 1 && TM % 16 == 0 && KK % 2 == 0 && NB >= 2, "tile shape");
     constexpr uint32_t STAGE = (TM + TN) * I8_BK;
     extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
 
     const uint32_t t = threadIdx.x, lane = t & 63u;
     const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(t >> 6));
-    // XCD x takes a contiguous eighth of the tile list (rows of x fastest): its L2 holds a few rows of w tiles and all of x
+    // XCD x takes a contiguous eighth of the tile list; in the list, 4 rows of tiles at a time run through all columns: an L2 holds their x while w streams by
     const uint32_t n_tiles = a.tiles_m * a.tiles_n;
     uint32_t tile = blockIdx.x;
     {
         const uint32_t q = n_tiles >> 3, r = n_tiles & 7u, xcd = tile & 7u, idx = tile >> 3;
         tile = (xcd < r ? xcd * (q + 1u) : r * (q + 1u) + (xcd - r) * q) + idx;
     }
-    const uint32_t tn = tile / a.tiles_m, tm = tile - tn * a.tiles_m;
+    const uint32_t group = tile / (4u * a.tiles_n), in = tile - group * 4u * a.tiles_n;
+    const uint32_t high = a.tiles_m - group * 4u < 4u ? a.tiles_m - group * 4u : 4u;
+    const uint32_t tm = group * 4u + in % high, tn = in / high;
     const uint32_t m0 = tm * TM, n0 = tn * TN;
 
     // unit u = t + THREADS i of a stage: row u / 8 (x rows, then w rows), LDS slot u % 8, which holds 16-byte column (u % 8) ^ swz(row)
@@ -87,26 +99,26 @@ __global__ __launch_bounds__(WM * WN * 64) void linear_i8_tile(const I8Args a)
         const uint32_t rl = is_x ? row : row - (uint32_t)TM;
         col[i] = ((u & 7u) ^ i8_swz(rl)) * 16u;
         const uint32_t gr = (is_x ? m0 : n0) + rl, top = is_x ? a.m : a.n;
-        src[i] = (GGQ_GLOBAL const uint8_t*)(is_x ? a.xq : a.wq) + (uint64_t)(gr < top ? gr : top - 1u) * (is_x ? a.x_stride : a.w_stride);
+        src[i] = (GGQ_GLOBAL const uint8_t*)(is_x ? a.xq : a.wq) + (uint64_t)(gr < top ? gr : top - 1u) * (is_x ? a.x_stride : a.w_stride) + col[i];
     }
     const uint32_t steps = (a.k + I8_BK - 1u) / I8_BK;
-    auto stage = [&](uint32_t step) {
-        uint8_t* dst = smem + (step & 1u) * STAGE;
+    auto stage = [&](uint32_t step, uint32_t buf) {
+        uint8_t* dst = smem + buf * STAGE;
         const uint32_t k0 = step * I8_BK;
         if (k0 + I8_BK <= a.k) {
 #pragma unroll
-            for (int i = 0; i < UN; i++) i8_dma16(src[i] + k0 + col[i], dst + (wave * 64u + (uint32_t)(THREADS * i)) * 16u);
+            for (int i = 0; i < UN; i++) i8_dma16(src[i] + k0, dst + (wave * 64u + (uint32_t)(THREADS * i)) * 16u);
         } else {                                       // the last step: columns past k are zeros of x against whatever starts the row of w
 #pragma unroll
             for (int i = 0; i < UN; i++) {
-                const bool in = k0 + col[i] < a.k, is_x = t + (uint32_t)(THREADS * i) < (uint32_t)TM * 8u;
-                const GGQ_GLOBAL uint8_t* p = in ? src[i] + k0 + col[i] : (is_x ? (const GGQ_GLOBAL uint8_t*)I8_ZEROS : src[i]);
+                const bool in_k = k0 + col[i] < a.k, is_x = t + (uint32_t)(THREADS * i) < (uint32_t)TM * 8u;
+                const GGQ_GLOBAL uint8_t* p = in_k ? src[i] + k0 : (is_x ? (const GGQ_GLOBAL uint8_t*)I8_ZEROS : src[i] - col[i]);
                 i8_dma16(p, dst + (wave * 64u + (uint32_t)(THREADS * i)) * 16u);
             }
         }
     };
 
-    const uint32_t wm = wave / WN, wn = wave % WN, r32 = lane & 31u, h = lane >> 5, fswz = i8_swz(r32);
+    const uint32_t ks = wave / (WM * WN), place = wave % (WM * WN), wm = place / WN, wn = place % WN, r32 = lane & 31u, h = lane >> 5, fswz = i8_swz(r32);
     const uint32_t xrow = wm * (TM / WM) + r32, wrow = (uint32_t)TM + wn * (TN / WN) + r32;
     i32x16 acc[NT][MT];
 #pragma unroll
@@ -115,26 +127,85 @@ __global__ __launch_bounds__(WM * WN * 64) void linear_i8_tile(const I8Args a)
         for (int mt = 0; mt < MT; mt++)
 #pragma unroll
             for (int i = 0; i < 16; i++) acc[nt][mt][i] = 0;
+    i32x4 wa[2][NT], xb[2][MT];
+    auto fragments = [&](const uint8_t* buf, int kk, int set) {
+        const uint32_t c = ((2u * (uint32_t)(KK * (int)ks + kk) + h) ^ fswz) * 16u;
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) wa[set][nt] = *reinterpret_cast<const i32x4*>(buf + (wrow + 32u * (uint32_t)nt) * I8_BK + c);
+#pragma unroll
+        for (int mt = 0; mt < MT; mt++) xb[set][mt] = *reinterpret_cast<const i32x4*>(buf + (xrow + 32u * (uint32_t)mt) * I8_BK + c);
+    };
+    // every load but the newest IN_FLIGHT of this wave has landed and its LDS reads have returned; the barrier says so to the others.  (Raw s_barrier: with
+    // __syncthreads() the compiler would wait for all loads.)
+    auto publish_keep = [&]() {
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" :: "n"(UN * (NB == 2 ? 1 : NB - 2)) : "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    };
+    auto publish_all = [&]() {
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    };
 
-    stage(0);
+    constexpr uint32_t AHEAD = NB == 2 ? 2 : NB - 1;                        // steps requested before the first is used
+#pragma unroll
+    for (uint32_t s = 0; s < AHEAD; s++)
+        if (s < steps) stage(s, s);
+    if (steps >= AHEAD) publish_keep();
+    else publish_all();
+    fragments(smem, 0, 0);
+    uint32_t cur = 0, free_buf = NB - 1;
     for (uint32_t s = 0; s < steps; s++) {
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");       // this wave's part of step s has landed; the barrier publishes it, and says that every
-        __syncthreads();                                       // wave is done reading step s - 1, whose buffer step s + 1 goes to
-        if (s + 1 < steps) stage(s + 1);
-        const uint8_t* buf = smem + (s & 1u) * STAGE;
+        const uint32_t next = cur + 1 == NB ? 0 : cur + 1;
+        if constexpr (NB > 2) {
+            if (s + NB - 1 < steps) stage(s + NB - 1, free_buf);
+        }
 #pragma unroll
-        for (int kk = 0; kk < 4; kk++) {
-            const uint32_t c = (((uint32_t)(2 * kk) + h) ^ fswz) * 16u;
-            i32x4 wa[NT], xb[MT];
-#pragma unroll
-            for (int nt = 0; nt < NT; nt++) wa[nt] = *reinterpret_cast<const i32x4*>(buf + (wrow + 32u * (uint32_t)nt) * I8_BK + c);
-#pragma unroll
-            for (int mt = 0; mt < MT; mt++) xb[mt] = *reinterpret_cast<const i32x4*>(buf + (xrow + 32u * (uint32_t)mt) * I8_BK + c);
+        for (int kk = 0; kk < KK; kk++) {
+            if (kk + 1 < KK) {
+                fragments(smem + cur * STAGE, kk + 1, (kk + 1) & 1);
+            } else if (s + 1 < steps) {
+                if (NB > 2 && s + NB - 1 < steps) publish_keep();
+                else publish_all();
+                if constexpr (NB == 2) {
+                    if (s + 2 < steps) stage(s + 2, cur);
+                }
+                fragments(smem + next * STAGE, 0, 0);
+            }
 #pragma unroll
             for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-                for (int mt = 0; mt < MT; mt++) acc[nt][mt] = __builtin_amdgcn_mfma_i32_32x32x32_i8(wa[nt], xb[mt], acc[nt][mt], 0, 0, 0);
+                for (int mt = 0; mt < MT; mt++) acc[nt][mt] = __builtin_amdgcn_mfma_i32_32x32x32_i8(wa[kk & 1][nt], xb[kk & 1][mt], acc[nt][mt], 0, 0, 0);
+            if constexpr (NT * MT >= NT + MT) {                             // one LDS read behind each of the first matrix instructions
+#pragma unroll
+                for (int q = 0; q < NT + MT; q++) {
+                    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+                }
+                __builtin_amdgcn_sched_group_barrier(0x8, NT * MT - NT - MT, 0);
+            }
         }
+        free_buf = cur;
+        cur = next;
+    }
+    if constexpr (KS > 1) {                                                 // integers: the k-parts add up to the same in any order
+        __syncthreads();
+        i32x16* part = reinterpret_cast<i32x16*>(smem);
+        static_assert((KS - 1) * WM * WN * 64 * 64 <= NB * STAGE, "partial sums fit the staging buffers");
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+            for (int mt = 0; mt < MT; mt++) {
+                if (ks) part[((ks - 1u) * (WM * WN) + place) * 64u + lane] = acc[nt][mt];
+                __syncthreads();
+                if (!ks)
+                    for (uint32_t q = 0; q < KS - 1; q++) acc[nt][mt] += part[(q * (WM * WN) + place) * 64u + lane];
+                __syncthreads();
+            }
+        if (ks) return;
+    } else {
+        __syncthreads();                                                    // every wave is done with the staging buffers
     }
 
     // D[row = 8 (i / 4) + 4 h + i % 4][column = r32] = sum of (row of w, row of x): four consecutive columns of y per lane and register group.  Each wave turns
@@ -142,9 +213,8 @@ __global__ __launch_bounds__(WM * WN * 64) void linear_i8_tile(const I8Args a)
     // and a row is stored in full lines.  (Stored straight from the accumulators, 2 bytes at a time, the epilogue took longer than the product.)
     constexpr uint32_t COLS = TN / WN, LPR = COLS / 8, RPI = 64 / LPR;      // columns of a wave, lanes per row, rows per store instruction
     constexpr uint32_t SLOTS = COLS / 4;                                    // 16-byte places of a row in LDS, XOR-swizzled by the row
-    static_assert(WM * WN * 32 * COLS * 4 <= 2 * STAGE, "the turned sums fit the staging buffers");
-    __syncthreads();                                                        // every wave is done with the staging buffers
-    int* turn = reinterpret_cast<int*>(smem) + wave * (32u * COLS);
+    static_assert(WM * WN * 32 * COLS * 4 <= NB * STAGE, "the turned sums fit the staging buffers");
+    int* turn = reinterpret_cast<int*>(smem) + place * (32u * COLS);
     const uint32_t nc = n0 + wn * COLS + (lane % LPR) * 8u;
     float sw[8], bias[8];
 #pragma unroll

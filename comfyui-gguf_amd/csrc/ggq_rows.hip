@@ -71,6 +71,16 @@ extern "C" int ggq_quantize_rows(const void* x, uint64_t rows, uint32_t cols, vo
     if (rows == 0) return GGQ_OK;
     if (!x || !q || !scale || cols == 0 || q_stride < cols || q_stride % 16 != 0) return GGQ_ERR_ARG;
     if (!aligned_to(x, dtype == GGQ_F32 ? 4 : 2) || !aligned_to(q, 16)) return GGQ_ERR_ALIGN;
+    if (q_stride <= 8192u && rows <= 0x7FFFFFFFull) {
+        typedef void (*quantize_fn)(const uint8_t*, uint64_t, uint32_t, uint8_t*, uint64_t, float*);
+#define GGQ_QUANTIZE(DT) {{quantize_rows<DT, true, false>, quantize_rows<DT, false, false>}, {quantize_rows<DT, true, true>, quantize_rows<DT, false, true>}}
+        static const quantize_fn QUANTIZE[3][2][2] = {GGQ_QUANTIZE(OUT_F16), GGQ_QUANTIZE(OUT_BF16), GGQ_QUANTIZE(OUT_F32)};
+        const bool solo = q_stride <= 512u;
+        hipLaunchKernelGGL(QUANTIZE[dtype][cols % 8 != 0][solo ? 0 : 1], dim3((uint32_t)(solo ? (rows + 3) / 4 : rows)), dim3(solo ? 256u : (uint32_t)(q_stride + 511u) / 512u * 64u), 0,
+                           static_cast<hipStream_t>(hip_stream), static_cast<const uint8_t*>(x), rows, cols, static_cast<uint8_t*>(q), q_stride, scale);
+        const hipError_t e = hipGetLastError();
+        return e == hipSuccess ? GGQ_OK : hip_fail(e);
+    }
     RowArgs a{};
     a.stream = static_cast<const uint8_t*>(x);
     a.y = static_cast<uint8_t*>(q);

@@ -87,7 +87,7 @@ def _check(y, q, sx, w, sw, bias, dtype):
 
 
 SIZES = [(1, 1, 1), (1, 17, 64), (3, 100, 1001), (16, 48, 4096), (17, 33, 129), (64, 65, 127), (65, 130, 2432), (128, 128, 128), (129, 257, 384), (333, 1501, 1001), (300, 70, 16),
-         (1, 10240, 4096), (2, 5, 20000), (1100, 1030, 640), (4100, 4099, 160), (31, 16384, 48)]
+         (1, 10240, 4096), (2, 5, 20000), (1100, 1030, 640), (4100, 4099, 160), (31, 16384, 48), (700, 5000, 200)]
 
 
 @pytest.mark.parametrize("kind", ["f16", "bf16", "f32"])
