@@ -109,7 +109,7 @@ SYMBOLS = {
     "ggq_linear_int8": (_int, [_vp, _u64, _vp, _u32, _vp, _u64, _vp, _u32, _u32, _vp, _vp, _int, _vp]),
     "ggq_moe_route": (_int, [_vp, _vp, _u32, _u32, _u32, _u32, _int, _vp, _vp, _int, _int, _vp]),
     "ggq_moe_experts": (_int, [ctypes.POINTER(ggq_moe_desc), _vp]),
-    "ggq_moe_workspace": (_u64, [_u32, _u32, _u32]),
+    "ggq_moe_workspace": (_u64, [_u32, _u32, _u32, _u32]),
     "ggq_dequant_rows": (_int, [_int, _vp, _u64, _u32, _vp, _u64, _vp, _int, _int, _vp]),
     # include/ggq_gguf.h
     "ggq_gguf_open": (_int, [ctypes.c_char_p, ctypes.POINTER(_vp)]),

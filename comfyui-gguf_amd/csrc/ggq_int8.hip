@@ -34,12 +34,12 @@ template <int DT>
 hipError_t launch(const I8Args& a, hipStream_t s)
 {
     if (a.m <= 16) return launch_rows16<DT>(a, s);
-    // The tile that finishes first: rounds of workgroups over the chip times what a step of 128 k takes, in ns, measured at 256 x 4096 x 4096 (a part of the
-    // chip) and 512 ... 4608 x 10240 x 4096 (all of it): 256 x 256 1550 (one workgroup per CU: 128 KiB of LDS); 128 x 128 720 alone on a CU, 1200 for two;
-    // 64 x 64 410, also for two.
+    // The tile that finishes first: rounds of workgroups over the chip times what a step of 128 k takes, in ns.  Measured at 256 x 4096 x 4096 (a part of
+    // the chip), 512 x 10240 x 4096 and 4608 x 10240 x 4096 (all of it, at the clock it holds then): 256 x 256 (128 KiB of LDS: one workgroup per CU) 1330 ...
+    // 1450 in one round, 1850 in several; 128 x 128 670 alone on a CU, 1050 for two; 64 x 64 350 alone, 420 for two.
     auto tiles = [&](uint64_t t) { return ((a.m + t - 1) / t) * ((a.n + t - 1) / t); };
-    const uint64_t t128 = tiles(128);
-    const uint64_t big = (tiles(256) + 255) / 256 * 1550, mid = t128 <= 256 ? 720 : (t128 + 511) / 512 * 1200, small = (tiles(64) + 511) / 512 * 410;
+    const uint64_t t256 = tiles(256), t128 = tiles(128), t64 = tiles(64);
+    const uint64_t big = t256 <= 256 ? 1450 : (t256 + 255) / 256 * 1850, mid = t128 <= 256 ? 670 : (t128 + 511) / 512 * 1050, small = t64 <= 256 ? 350 : (t64 + 511) / 512 * 420;
     if (small <= mid && small <= big) return launch_tile<DT, 64, 64, 1, 2, 2, 4>(a, s);
     if (mid < big) return launch_tile<DT, 128, 128, 2, 2, 1, 2>(a, s);
     return launch_tile<DT, 256, 256, 2, 4, 1, 2>(a, s);

@@ -62,8 +62,10 @@ struct I8Args {
 // With 256 x 256 the reads (24 x 64 x 16 bytes per wave and step) and the LDS-DMA writes take as long as the matrix instructions (32 per wave, 32 cycles each):
 // they have to overlap completely, hence the interleaved issue order that sched_group_barrier asks for.
 //
-// Measured (4608 x 9728 x 2432 / 4608 x 10240 x 4096, us): fragments read where they are used 151 / 206, tiles in groups of 4 rows of tiles (L2) 126 / 203, read one
-// piece ahead 130 / 193, and interleaved 122 / 188 = 1786 / 2054 TOP/s; 4 waves of 128 x 128 137 / 203; 64 bytes of k and 4 buffers 131 / 204.
+// Measured (4608 x 9728 x 2432 / 4608 x 10240 x 4096, us): fragments read where they are used 151 / 206; tiles in groups of 4 rows of tiles (L2) 126 / 203; read one
+// piece ahead 130 / 193, interleaved 122 / 188; the branches for a partial last step out of the loop, so that the compiler counts the reads in flight
+// instead of waiting for all, 118 / 178 = 1840 / 2172 TOP/s (the library's int8 product on these shapes: 127 / 187).  4 waves of 128 x 128: 137 / 203; 64 bytes
+// of k and 4 buffers: 131 / 204.
 template <int DT, int TM, int TN, int WM, int WN, int KS, int NB>
 __global__ __launch_bounds__(WM * WN * KS * 64) void linear_i8_tile(const I8Args a)
 {
@@ -102,12 +104,15 @@ __global__ __launch_bounds__(WM * WN * KS * 64) void linear_i8_tile(const I8Args
         src[i] = (GGQ_GLOBAL const uint8_t*)(is_x ? a.xq : a.wq) + (uint64_t)(gr < top ? gr : top - 1u) * (is_x ? a.x_stride : a.w_stride) + col[i];
     }
     const uint32_t steps = (a.k + I8_BK - 1u) / I8_BK;
+    auto stage_whole = [&](uint32_t step, uint32_t buf) {
+#pragma unroll
+        for (int i = 0; i < UN; i++) i8_dma16(src[i] + step * I8_BK, smem + buf * STAGE + (wave * 64u + (uint32_t)(THREADS * i)) * 16u);
+    };
     auto stage = [&](uint32_t step, uint32_t buf) {
         uint8_t* dst = smem + buf * STAGE;
         const uint32_t k0 = step * I8_BK;
         if (k0 + I8_BK <= a.k) {
-#pragma unroll
-            for (int i = 0; i < UN; i++) i8_dma16(src[i] + k0, dst + (wave * 64u + (uint32_t)(THREADS * i)) * 16u);
+            stage_whole(step, buf);
         } else {                                       // the last step: columns past k are zeros of x against whatever starts the row of w
 #pragma unroll
             for (int i = 0; i < UN; i++) {
@@ -156,7 +161,45 @@ __global__ __launch_bounds__(WM * WN * KS * 64) void linear_i8_tile(const I8Args
     else publish_all();
     fragments(smem, 0, 0);
     uint32_t cur = 0, free_buf = NB - 1;
-    for (uint32_t s = 0; s < steps; s++) {
+    auto multiply = [&](int set) {
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+            for (int mt = 0; mt < MT; mt++) acc[nt][mt] = __builtin_amdgcn_mfma_i32_32x32x32_i8(wa[set][nt], xb[set][mt], acc[nt][mt], 0, 0, 0);
+        if constexpr (NT * MT >= NT + MT) {                                 // one LDS read behind each of the first matrix instructions
+#pragma unroll
+            for (int q = 0; q < NT + MT; q++) {
+                __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            }
+            __builtin_amdgcn_sched_group_barrier(0x8, NT * MT - NT - MT, 0);
+        }
+    };
+    auto turn_buffers = [&]() {
+        free_buf = cur;
+        cur = cur + 1 == NB ? 0 : cur + 1;
+    };
+    uint32_t s = 0;
+    // steps whose requests are whole: no branch but the loop's
+    const uint32_t whole = a.k / I8_BK > AHEAD ? a.k / I8_BK - AHEAD : 0u;
+    for (; s < whole; s++) {
+        const uint32_t next = cur + 1 == NB ? 0 : cur + 1;
+        if constexpr (NB > 2) stage_whole(s + NB - 1, free_buf);
+#pragma unroll
+        for (int kk = 0; kk < KK; kk++) {
+            if (kk + 1 < KK) {
+                fragments(smem + cur * STAGE, kk + 1, (kk + 1) & 1);
+            } else {
+                if constexpr (NB > 2) publish_keep();
+                else publish_all();
+                if constexpr (NB == 2) stage_whole(s + 2, cur);
+                fragments(smem + next * STAGE, 0, 0);
+            }
+            multiply(kk & 1);
+        }
+        turn_buffers();
+    }
+    for (; s < steps; s++) {
         const uint32_t next = cur + 1 == NB ? 0 : cur + 1;
         if constexpr (NB > 2) {
             if (s + NB - 1 < steps) stage(s + NB - 1, free_buf);
@@ -173,21 +216,9 @@ __global__ __launch_bounds__(WM * WN * KS * 64) void linear_i8_tile(const I8Args
                 }
                 fragments(smem + next * STAGE, 0, 0);
             }
-#pragma unroll
-            for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-                for (int mt = 0; mt < MT; mt++) acc[nt][mt] = __builtin_amdgcn_mfma_i32_32x32x32_i8(wa[kk & 1][nt], xb[kk & 1][mt], acc[nt][mt], 0, 0, 0);
-            if constexpr (NT * MT >= NT + MT) {                             // one LDS read behind each of the first matrix instructions
-#pragma unroll
-                for (int q = 0; q < NT + MT; q++) {
-                    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-                    __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
-                }
-                __builtin_amdgcn_sched_group_barrier(0x8, NT * MT - NT - MT, 0);
-            }
+            multiply(kk & 1);
         }
-        free_buf = cur;
-        cur = next;
+        turn_buffers();
     }
     if constexpr (KS > 1) {                                                 // integers: the k-parts add up to the same in any order
         __syncthreads();

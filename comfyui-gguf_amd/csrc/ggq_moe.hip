@@ -7,29 +7,56 @@ namespace {
 
 using namespace ggq;
 
-typedef hipError_t (*moe_fn)(const MoeArgs&, hipStream_t);
+typedef hipError_t (*moe_fn)(MoeArgs, hipStream_t);
 
-template <class F, int OUT, int MB>
-hipError_t launch_up(const MoeArgs& a, hipStream_t s)
+// Slots of a wave's ring, given the rest of a workgroup's LDS: three where two workgroups then still fit a CU (160 KiB) or would not with two slots either.
+constexpr uint32_t HALF_LDS = 80u * 1024u, ALL_LDS = 160u * 1024u;
+uint32_t ring_slots(uint32_t rest, uint32_t slot_bytes)
 {
-    const uint32_t pairs = a.tokens * a.top_k, experts = pairs < a.experts ? pairs : a.experts;      // at most so many are chosen
-    hipLaunchKernelGGL((moe_up<F, OUT, MB>), dim3(a.ff / 16u, experts), dim3(MOE_UP_WAVES * 64), 0, s, a);
-    return hipGetLastError();
+    const uint32_t two = rest + MOE_WAVES * 2u * slot_bytes, three = rest + MOE_WAVES * 3u * slot_bytes;
+    if (three <= HALF_LDS) return 3u;
+    if (two <= HALF_LDS) return 2u;
+    return three <= ALL_LDS ? 3u : 2u;
 }
 
 template <class F, int OUT, int MB>
-hipError_t launch_down(const MoeArgs& a, hipStream_t s)
+hipError_t launch_up(MoeArgs a, hipStream_t s)
 {
-    const uint32_t lds = MOE_DOWN_WAVES * a.tokens * 64u;                                             // <= 32 KiB, beside up to 41 KiB of static LDS
+    constexpr uint32_t fixed = sizeof(MoeTable) + MOE_WAVES * MOE_MAX_TOKENS * 4 + (MB == 1 ? 2 : MB) * MOE_WAVES * 1024 + 64;
+    const uint32_t pairs = a.tokens * a.top_k, most = (pairs < a.experts ? pairs : a.experts) * (a.ff / 16u);      // tiles, if every pair chose another expert
+    const uint32_t blocks = (a.tokens + 15u) / 16u;
+    a.spare = blocks > (uint32_t)MB ? blocks - MB : 0u;
+    a.ring = ring_slots(fixed + MOE_WAVES * a.spare * 1024u, Mf16Geom<F>::SLICE);
+    const uint32_t lds = MOE_WAVES * (a.spare * 1024u + a.ring * Mf16Geom<F>::SLICE);
+    if (fixed + lds > ALL_LDS) return hipErrorInvalidConfiguration;
     static std::atomic<uint64_t> raised{0};
-    const hipError_t e = allow_lds(reinterpret_cast<const void*>(&moe_down<F, OUT, MB>), MOE_DOWN_WAVES * MOE_MAX_TOKENS * 64, raised);
+    const hipError_t e = allow_lds(reinterpret_cast<const void*>(&moe_up<F, OUT, MB>), (int)(ALL_LDS - fixed), raised);
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL((moe_down<F, OUT, MB>), dim3(a.dim / 16u), dim3(MOE_DOWN_WAVES * 64), lds, s, a);
+    // as many workgroups as the chip holds (MB > 1: their registers leave one per CU), dealt the same number of tiles
+    const uint32_t fit = MB == 1 && fixed + lds <= HALF_LDS ? 512u : 256u;
+    hipLaunchKernelGGL((moe_up<F, OUT, MB>), dim3(most < fit ? most : fit), dim3(MOE_WAVES * 64), lds, s, a);
     return hipGetLastError();
 }
 
-struct MoeEntry { int qtype, block_size; moe_fn up[2][2], down[2][2]; };                              // [dtype f16 / bf16][MB 1 / 2]
-#define GGQ_MOE_ROW(FN, F, OUT) {FN<F, OUT, 1>, FN<F, OUT, 2>}
+template <class F, int OUT, int MB>
+hipError_t launch_down(MoeArgs a, hipStream_t s)
+{
+    constexpr uint32_t fixed = sizeof(MoeTable) + MOE_MAX_TOKENS * MOE_MAX_TOPK * 4 + 2 * MOE_WAVES * MOE_MAX_TOKENS * 4 + 64;
+    const uint32_t blocks = (2u * a.tokens + 15u) / 16u;
+    a.spare = blocks > (uint32_t)MB ? blocks - MB : 0u;
+    const uint32_t sums = MOE_WAVES * (a.tokens * 64u + a.spare * 1024u);
+    a.ring = ring_slots(fixed + sums, Mf16Geom<F>::SLICE);
+    const uint32_t lds = sums + MOE_WAVES * a.ring * Mf16Geom<F>::SLICE;
+    if (fixed + lds > ALL_LDS) return hipErrorInvalidConfiguration;
+    static std::atomic<uint64_t> raised{0};
+    const hipError_t e = allow_lds(reinterpret_cast<const void*>(&moe_down<F, OUT, MB>), (int)(ALL_LDS - fixed), raised);
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL((moe_down<F, OUT, MB>), dim3(a.dim / 16u, a.parts), dim3(MOE_WAVES * 64), lds, s, a);
+    return hipGetLastError();
+}
+
+struct MoeEntry { int qtype, block_size; moe_fn up[2][3], down[2][3]; };                              // [dtype f16 / bf16][blocks of 16 columns 1 / 2 / 4]
+#define GGQ_MOE_ROW(FN, F, OUT) {FN<F, OUT, 1>, FN<F, OUT, 2>, FN<F, OUT, 4>}
 #define GGQ_MOE(F) MoeEntry { F::ID, F::BS, {GGQ_MOE_ROW(launch_up, F, OUT_F16), GGQ_MOE_ROW(launch_up, F, OUT_BF16)}, \
                               {GGQ_MOE_ROW(launch_down, F, OUT_F16), GGQ_MOE_ROW(launch_down, F, OUT_BF16)} }
 const MoeEntry MOE[] = {
@@ -43,6 +70,23 @@ const MoeEntry* entry(int qtype)
     for (const MoeEntry& e : MOE)
         if (e.qtype == qtype) return &e;
     return nullptr;
+}
+
+// Workgroups that share the (expert, span) list of moe_down's 16 rows: so many that the launch has two for every CU.
+uint32_t down_parts(uint32_t dim)
+{
+    const uint32_t tiles = dim / 16u;
+    return tiles >= 512u ? 1u : (512u / (tiles ? tiles : 1u) < 8u ? 512u / (tiles ? tiles : 1u) : 8u);
+}
+
+// Blocks of 16 columns for `per_token` columns of each token of an expert: room for three standard deviations above the mean of evenly spread choices (more
+// tokens than that on one expert are multiplied block by block, with their sums in LDS).
+int column_blocks(uint32_t tokens, uint32_t top_k, uint32_t experts, uint32_t per_token)
+{
+    const double mean = (double)tokens * top_k / experts, most = mean + 3.0 * __builtin_sqrt(mean);
+    if (per_token == 2 && tokens > 32) return 2;                    // the sums of what may overflow have to fit the LDS
+    const double cols = (most < tokens ? most : (double)tokens) * per_token;
+    return cols <= 16.0 ? 0 : (cols <= 32.0 ? 1 : 2);
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -66,7 +110,11 @@ extern "C" int ggq_moe_route(const void* x, const void* router, uint32_t tokens,
     return e == hipSuccess ? GGQ_OK : hip_fail(e);
 }
 
-extern "C" uint64_t ggq_moe_workspace(uint32_t tokens, uint32_t top_k, uint32_t ff) { return (uint64_t)tokens * top_k * ff * 4u; }
+extern "C" uint64_t ggq_moe_workspace(uint32_t tokens, uint32_t top_k, uint32_t dim, uint32_t ff)
+{
+    const uint64_t hidden = ((uint64_t)tokens * top_k * ff * 4u + 15u) & ~15ull, parts = down_parts(dim);
+    return hidden + (parts > 1 ? parts * tokens * dim * 4u : 0u);
+}
 
 extern "C" int ggq_moe_experts(const ggq_moe_desc* d, void* hip_stream)
 {
@@ -74,17 +122,25 @@ extern "C" int ggq_moe_experts(const ggq_moe_desc* d, void* hip_stream)
     const MoeEntry *up = entry(d->up_qtype), *down = entry(d->down_qtype);
     if (!up || !down) return GGQ_ERR_QTYPE;
     auto whole = [](const MoeEntry* e, uint32_t k) { return k != 0 && k % (e->block_size == 32 ? 64u : 256u) == 0; };
-    if ((d->dtype != GGQ_F16 && d->dtype != GGQ_BF16) || (d->act != 0 && d->act != 1) || !whole(up, d->dim) || !whole(down, d->ff) || d->dim % 16u != 0 || d->ff % 16u != 0 ||
+    if ((d->dtype != GGQ_F16 && d->dtype != GGQ_BF16) || (d->act != 0 && d->act != 1) || !whole(up, d->dim) || !whole(down, d->ff) || d->dim % 16u != 0 || d->ff % 16u != 0 || d->dim > (1u << 24) || d->ff > (1u << 24) ||
         d->experts == 0 || d->experts > (uint32_t)MOE_MAX_EXPERTS || d->top_k == 0 || d->top_k > (uint32_t)MOE_MAX_TOPK || d->tokens > (uint32_t)MOE_MAX_TOKENS) return GGQ_ERR_ARG;
     if (d->tokens == 0) return GGQ_OK;
-    if (!d->x || !d->ids || !d->weights || !d->gate || !d->up || !d->down || !d->y || !d->workspace || d->workspace_bytes < ggq_moe_workspace(d->tokens, d->top_k, d->ff))
+    if (!d->x || !d->ids || !d->weights || !d->gate || !d->up || !d->down || !d->y || !d->workspace || d->workspace_bytes < ggq_moe_workspace(d->tokens, d->top_k, d->dim, d->ff))
         return GGQ_ERR_ARG;
     if (!aligned16(d->x) || !aligned16(d->gate) || !aligned16(d->up) || !aligned16(d->down) || !aligned16(d->workspace) || !aligned4(d->ids) || !aligned4(d->weights) ||
-        (reinterpret_cast<uintptr_t>(d->y) & 1u)) return GGQ_ERR_ALIGN;
-    const MoeArgs a{static_cast<const uint8_t*>(d->x), d->ids, d->weights, static_cast<const uint8_t*>(d->gate), static_cast<const uint8_t*>(d->up),
-                    static_cast<const uint8_t*>(d->down), static_cast<uint8_t*>(d->y), static_cast<uint8_t*>(d->workspace), d->tokens, d->top_k, d->experts, d->dim, d->ff, d->act};
+        (reinterpret_cast<uintptr_t>(d->y) & 7u)) return GGQ_ERR_ALIGN;
+    MoeArgs a{static_cast<const uint8_t*>(d->x), d->ids, d->weights, static_cast<const uint8_t*>(d->gate), static_cast<const uint8_t*>(d->up),
+              static_cast<const uint8_t*>(d->down), static_cast<uint8_t*>(d->y), static_cast<uint8_t*>(d->workspace), nullptr, d->tokens, d->top_k, d->experts, d->dim, d->ff, d->act, 1, 0, 2};
+    a.parts = down_parts(a.dim);
+    a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(d->workspace) + (((uint64_t)a.tokens * a.top_k * a.ff * 4u + 15u) & ~15ull));
     hipStream_t s = static_cast<hipStream_t>(hip_stream);
-    hipError_t e = up->up[d->dtype][d->tokens > 16 ? 1 : 0](a, s);
-    if (e == hipSuccess) e = down->down[d->dtype][d->tokens > 8 ? 1 : 0](a, s);
+    hipError_t e = up->up[d->dtype][column_blocks(a.tokens, a.top_k, a.experts, 1)](a, s);
+    if (e == hipSuccess) e = down->down[d->dtype][column_blocks(a.tokens, a.top_k, a.experts, 2)](a, s);
+    if (e == hipSuccess && a.parts > 1) {
+        const uint32_t quads = a.tokens * a.dim / 4u;
+        if (d->dtype == GGQ_F16) hipLaunchKernelGGL((moe_combine<OUT_F16>), dim3((quads + 255u) / 256u), dim3(256), 0, s, a.part, a.y, a.parts, quads);
+        else hipLaunchKernelGGL((moe_combine<OUT_BF16>), dim3((quads + 255u) / 256u), dim3(256), 0, s, a.part, a.y, a.parts, quads);
+        e = hipGetLastError();
+    }
     return e == hipSuccess ? GGQ_OK : hip_fail(e);
 }

@@ -3,13 +3,17 @@
 // Mathematics, per token x:  l = Wr x;  p = softmax(l);  the top_k largest p (equal ones to the lower index), divided by their sum if asked;
 //     y = sum_s p_s Wd[e_s] (act(Wg[e_s] x) * (Wu[e_s] x)).
 //
-// Three kernels: the router (moe_route, a workgroup per token), the gate and up projections with the activation (moe_up), the down projection with the
-// weighted sum over experts (moe_down).  What bounds them is reading the packed bytes of the chosen experts, each ONCE for all tokens that chose it:
-//   * moe_up: a workgroup owns 16 rows of Wg and the same 16 rows of Wu of one chosen expert; half of its waves contract the gate rows, half the up
-//     rows, each a part of k; the tokens of that expert are the 16 columns of v_mfma_f32_16x16x32 (A = 16 rows of decoded weights).
-//   * moe_down: a workgroup owns 16 rows of the output for ALL tokens and walks every chosen expert, so the sum over a token's experts needs no second
-//     pass and no atomics; its waves take equal, contiguous parts of the (expert, piece of k) list.
+// Kernels: the router (moe_route, a workgroup per token), the gate and up projections with the activation (moe_up), the down projection with the weighted sum
+// over experts (moe_down), and where the output has too few rows for the chip, a sum of its parts (moe_combine).  What bounds them is reading the
+// packed bytes of the chosen experts, each ONCE for all tokens that chose it -- and, as closely, unpacking them (1100 cycles of vector instructions per 16
+// rows x 256 columns of Q4_K for bf16: at the full rate that is 18 us where reading takes 19, for two experts of 2 x 10240 x 4096):
+//   * moe_up: a workgroup owns some tiles of 16 rows of Wg and Wu of the chosen experts; half of its waves contract the gate rows, half the up rows, each a part
+//     of k; the tokens of the expert are the columns of v_mfma_f32_16x16x32 (A = 16 rows of decoded weights).
+//   * moe_down: a workgroup owns 16 rows of the output for ALL tokens and walks every chosen expert, so the sum over a token's experts needs no atomics; its
+//     waves take equal, contiguous parts of the (expert, piece of k) list.
 //   * the list of chosen experts and the tokens of each are found by every workgroup itself from the ids (at most 64 x 16 of them).
+//   * a wave requests the columns (x, hidden) of this span, then the weights of a later one, then waits for all but those.  Loads return in order: columns
+//     requested behind weights would wait for those weights.
 // A weight is the reference's value bit for bit (ggq_device.hpp: same decode, same fp16 operations, then the rounding to the activations' type).
 // The hidden vector act(g) * u is kept in two parts of the activations' type -- its rounded value and the rounded rest -- which ride as two columns of
 // the down product: about 16 (bf16) or 22 (fp16) bits, for no more weight traffic.  The fp16 rest is kept times 2^11, out of the subnormals.
@@ -19,44 +23,69 @@
 #include "ggq_mfma16.hpp"
 #include "ggq_rows.hpp"
 
+#include <type_traits>
+
 namespace ggq {
 
 constexpr int MOE_MAX_TOKENS = 64, MOE_MAX_TOPK = 16, MOE_MAX_EXPERTS = 512;
 constexpr int MOE_WORDS = MOE_MAX_EXPERTS / 32;
 
-// ---- the router: a workgroup per token, a wave per expert in turn
+// ---- the router: a workgroup per token, four experts per wave at a time
 
-// Eight products, formed and added in fp64: which of two close scores is larger decides which experts run.  RT: the router's type, fp32 in GGUF files.
-template <int OUT, int RT> GGQ_DEV double moe_dot8(const uint8_t* x, const uint8_t* w)
+// Eight products, four at a time in fp32 (a product of two 16-bit values is exact there), what follows in fp64: which of two close scores is larger decides
+// which experts run.  (All of it in fp64: 17 us for 64 experts x 2048, most of it conversions.)  RT: the router's type, fp32 in GGUF files.
+template <int OUT, int RT> GGQ_DEV double moe_dot8(const float (&u)[8], const uint8_t* w)
 {
-    float u[8], v[8];
-    row_load8<OUT>(x, 0, 8, u);
+    float v[8], s[8];
     row_load8<RT>(w, 0, 8, v);
-    double s[4];
 #pragma unroll
-    for (int k = 0; k < 4; k++) s[k] = (double)u[2 * k] * (double)v[2 * k] + (double)u[2 * k + 1] * (double)v[2 * k + 1];
-    return (s[0] + s[1]) + (s[2] + s[3]);
+    for (int k = 0; k < 8; k++) s[k] = u[k] * v[k];
+    return (double)((s[0] + s[1]) + (s[2] + s[3])) + (double)((s[4] + s[5]) + (s[6] + s[7]));
 }
 
-constexpr int MOE_ROUTE_THREADS = 512;
+constexpr int MOE_ROUTE_THREADS = 1024;
 
 template <int OUT, int RT>
 __global__ __launch_bounds__(MOE_ROUTE_THREADS) void moe_route(const uint8_t* __restrict__ x_, const uint8_t* __restrict__ router_, uint32_t dim, uint32_t experts,
                                                               uint32_t top_k, int renormalize, int32_t* __restrict__ ids, float* __restrict__ weights)
 {
+    constexpr uint32_t RB = RT == OUT_F32 ? 4 : 2;
     __shared__ double score[MOE_MAX_EXPERTS];
     __shared__ double chosen[MOE_MAX_TOPK];
     const uint32_t t = threadIdx.x, lane = t & 63u, wave = t >> 6;
     const uint8_t* x = x_ + (uint64_t)blockIdx.x * dim * 2;
-    for (uint32_t e = wave; e < experts; e += MOE_ROUTE_THREADS / 64) {
-        constexpr uint32_t RB = RT == OUT_F32 ? 4 : 2;
-        const uint8_t* w = router_ + (uint64_t)e * dim * RB;
-        double acc = 0.0;
-        for (uint32_t i = lane * 8u; i < dim; i += 512u)
-            acc += moe_dot8<OUT, RT>(x + (uint64_t)i * 2, w + (uint64_t)i * RB);
+    constexpr uint32_t WAVES = MOE_ROUTE_THREADS / 64;
+    // Q experts e0, e0 + 16, ... of a wave, U pieces of 512 elements of their rows on their way at once; absent experts repeat the last one
+    auto scores = [&](auto q_, auto u_, uint32_t e0) {
+        constexpr uint32_t Q = decltype(q_)::value, U = decltype(u_)::value;
+        double acc[Q] = {};
+        for (uint32_t i0 = lane * 8u; i0 < dim; i0 += 512u * U) {
+            float u[U][8];
 #pragma unroll
-        for (int off = 32; off > 0; off >>= 1) acc += __shfl_xor(acc, off, 64);
-        if (lane == 0) score[e] = acc;
+            for (uint32_t p = 0; p < U; p++) row_load8<OUT>(x + (uint64_t)(i0 + 512u * p < dim ? i0 + 512u * p : 0u) * 2, 0, 8, u[p]);
+#pragma unroll
+            for (uint32_t q = 0; q < Q; q++) {
+                const uint32_t e = e0 + q * WAVES < experts ? e0 + q * WAVES : experts - 1u;
+                double d[U];
+#pragma unroll
+                for (uint32_t p = 0; p < U; p++) d[p] = moe_dot8<OUT, RT>(u[p], router_ + ((uint64_t)e * dim + (i0 + 512u * p < dim ? i0 + 512u * p : 0u)) * RB);
+#pragma unroll
+                for (uint32_t p = 0; p < U; p++) acc[q] += i0 + 512u * p < dim ? d[p] : 0.0;
+            }
+        }
+#pragma unroll
+        for (int off = 32; off > 0; off >>= 1)
+#pragma unroll
+            for (uint32_t q = 0; q < Q; q++) acc[q] += __shfl_xor(acc[q], off, 64);
+        if (lane == 0)
+#pragma unroll
+            for (uint32_t q = 0; q < Q; q++)
+                if (e0 + q * WAVES < experts) score[e0 + q * WAVES] = acc[q];
+    };
+    if (experts <= WAVES) {
+        if (wave < experts) scores(std::integral_constant<uint32_t, 1>{}, std::integral_constant<uint32_t, 4>{}, wave);
+    } else {
+        for (uint32_t e0 = wave; e0 < experts; e0 += 4 * WAVES) scores(std::integral_constant<uint32_t, 4>{}, std::integral_constant<uint32_t, 2>{}, e0);
     }
     __syncthreads();
     // rank of an expert = how many come before it; a NaN comes last (its weight is NaN all the same)
@@ -86,47 +115,63 @@ __global__ __launch_bounds__(MOE_ROUTE_THREADS) void moe_route(const uint8_t* __
 
 // ---- which experts were chosen, and by whom
 
-// bit e of words[]: some token chose expert e.  Called by the whole workgroup; ends with a barrier.
-GGQ_DEV void moe_mark(uint32_t* words, const int32_t* __restrict__ ids, uint32_t pairs, uint32_t experts)
+struct MoeTable {
+    uint32_t words[MOE_WORDS];                       // bit e: some token chose expert e
+    int32_t ids[MOE_MAX_TOKENS * MOE_MAX_TOPK];
+    uint16_t list[MOE_MAX_EXPERTS];                  // the chosen experts, ascending
+    uint32_t n;                                      // how many
+};
+
+// Called by the whole workgroup; ends with a barrier.
+GGQ_DEV void moe_table(MoeTable& s, const int32_t* __restrict__ ids, uint32_t pairs, uint32_t experts)
 {
-    if (threadIdx.x < MOE_WORDS) words[threadIdx.x] = 0;
+    if (threadIdx.x < MOE_WORDS) s.words[threadIdx.x] = 0;
     __syncthreads();
     for (uint32_t p = threadIdx.x; p < pairs; p += blockDim.x) {
         const uint32_t e = (uint32_t)ids[p];
-        if (e < experts) atomicOr(&words[e >> 5], 1u << (e & 31u));
+        s.ids[p] = (int32_t)e;
+        if (e < experts) atomicOr(&s.words[e >> 5], 1u << (e & 31u));
+    }
+    __syncthreads();
+    if (threadIdx.x < 64) {
+        uint32_t b = threadIdx.x < MOE_WORDS ? s.words[threadIdx.x] : 0u;
+        uint32_t upto = (uint32_t)__builtin_popcount(b);
+        const uint32_t own = upto;
+#pragma unroll
+        for (int off = 1; off < MOE_WORDS; off <<= 1) {
+            const uint32_t o = (uint32_t)__shfl_up((int)upto, off, 64);
+            if (threadIdx.x >= (uint32_t)off) upto += o;
+        }
+        if (threadIdx.x == MOE_WORDS - 1) s.n = upto;
+        for (uint32_t at = upto - own; b != 0; b &= b - 1u) s.list[at++] = (uint16_t)(32u * threadIdx.x + (uint32_t)__builtin_ctz(b));
     }
     __syncthreads();
 }
 
-// the `a`-th chosen expert in ascending order, or -1 (wave-uniform)
-GGQ_DEV int moe_nth(const uint32_t* words, uint32_t a)
-{
-    for (int w = 0; w < MOE_WORDS; w++) {
-        uint32_t b = words[w];
-        const uint32_t n = (uint32_t)__builtin_popcount(b);
-        if (a >= n) { a -= n; continue; }
-        for (; a > 0; a--) b &= b - 1u;
-        return 32 * w + __builtin_ctz(b);
-    }
-    return -1;
-}
-
 // The tokens that chose `expert`: lane t looks at token t.  `slot`: its first place in ids, `weight`: the sum over its places (the same expert twice
-// counts twice).  Returns the mask of tokens.
-GGQ_DEV uint64_t moe_tokens(const int32_t* __restrict__ ids, const float* __restrict__ weights, uint32_t tokens, uint32_t top_k, int expert, uint32_t& slot, float& weight)
+// counts twice; weights_ may be null).  Returns the mask of tokens.
+GGQ_DEV uint64_t moe_tokens(const MoeTable& s, const float* weights, uint32_t tokens, uint32_t top_k, int expert, uint32_t& slot, float& weight)
 {
     const uint32_t t = threadIdx.x & 63u;
     bool has = false;
     slot = 0;
     weight = 0.0f;
     if (t < tokens)
-        for (uint32_t s = top_k; s-- > 0;)
-            if (ids[t * top_k + s] == expert) {
+        for (uint32_t k = top_k; k-- > 0;)
+            if (s.ids[t * top_k + k] == expert) {
                 has = true;
-                slot = t * top_k + s;
-                weight += weights[t * top_k + s];
+                slot = t * top_k + k;
+                if (weights != nullptr) weight += weights[t * top_k + k];
             }
     return __ballot(has);
+}
+
+// a barrier for LDS only: weights that are on their way to registers stay on their way
+GGQ_DEV void moe_barrier()
+{
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
 }
 
 GGQ_DEV float moe_act(float g, int act)
@@ -136,59 +181,88 @@ GGQ_DEV float moe_act(float g, int act)
     return g * __builtin_amdgcn_rcpf(1.0f + __expf(-2.0f * u));
 }
 
-// one 256-element span of 16 rows, packed bytes to registers: as in linear_mfma16 (a short last span only in the 32-element formats)
-template <class F> GGQ_DEV void moe_fetch(gcptr rows, uint64_t row_bytes, uint32_t span, uint32_t n_spans, uint32_t tail_len, u32x4 (&pf)[Mf16Geom<F>::NUW])
+// A wave's packed bytes go from memory straight into its own ring of LDS slots (LDS-DMA), one 256-element span of 16 rows per slot: row r at r * ROW_STRIDE, an
+// odd number of 16-byte units, from the aligned address below the row's span on (Mf16Geom).  With a ring of three slots two spans are on their way while one is
+// decoded, at no cost in registers; the launch takes two slots where three would leave one workgroup on a CU instead of two.
+
+template <class F> struct MoeGeom {
+    using G = Mf16Geom<F>;
+    static constexpr uint32_t PITCH_U = G::ROW_STRIDE / 16, UNITS = 16 * PITCH_U, LOADS = (UNITS + 63) / 64;       // units of a slot; DMA instructions
+};
+
+// byte offset of a row's span from the 16-byte boundary at or below the first row: 16 rows are within 32 bits of it
+GGQ_DEV uint32_t moe_offset(gcptr rows, uint32_t row, uint32_t row_bytes, uint32_t span_at) { return ((uint32_t)(uintptr_t)rows & 15u) + row * row_bytes + span_at; }
+
+// requests one span; at least one lane of every instruction loads where the span is whole (LOADS instructions), fewer for a short last one
+template <class F> GGQ_DEV void moe_request(gcptr rows, uint32_t row_bytes, uint32_t span, uint32_t span_bytes, uint8_t* slot)
 {
     using G = Mf16Geom<F>;
-    const int lane = (int)(threadIdx.x & 63u);
-    const bool tail = F::BS == 32 && span + 1 == n_spans && tail_len != (uint32_t)MF_SPAN;                 // wave-uniform
-    const uint32_t span_bytes = (tail ? tail_len : (uint32_t)MF_SPAN) / (uint32_t)F::BS * (uint32_t)F::TS;
+    using M = MoeGeom<F>;
+    const uint32_t lane = threadIdx.x & 63u;
+    const gcptr base = (gcptr)((uintptr_t)rows & ~(uintptr_t)15);
 #pragma unroll
-    for (int u = 0; u < G::NUW; u++) {
-        const uint32_t unit = (uint32_t)(lane + 64 * u), ur = unit / (uint32_t)G::U, uu = unit % (uint32_t)G::U;
-        const gcptr at = rows + (uint64_t)(ur < 16u ? ur : 0u) * row_bytes + (uint64_t)span * G::SPAN_BYTES;
-        const uint32_t a = G::SKEW ? ((uint32_t)(uintptr_t)at & 15u) : 0u;
+    for (uint32_t i = 0; i < M::LOADS; i++) {
+        const uint32_t unit = lane + 64u * i, ur = unit / M::PITCH_U, uu = unit % M::PITCH_U;
+        const uint32_t at = moe_offset(rows, ur, row_bytes, span * G::SPAN_BYTES), a = G::SKEW ? at & 15u : 0u;
         // loads start 16-byte aligned: what they read past the span lies in a unit that also holds bytes of the tensor
-        pf[u] = (ur < 16u && uu * 16u < a + span_bytes) ? gload16<true>(at - a + uu * 16u) : u32x4{0, 0, 0, 0};
-        if (tail) {                                                                                        // blocks past the end decode to zeros
-            const int32_t valid = (int32_t)(a + span_bytes) - (int32_t)(uu * 16u);
-            uint32_t d[4] = {pf[u].x, pf[u].y, pf[u].z, pf[u].w};
-#pragma unroll
-            for (int i = 0; i < 4; i++) d[i] &= valid >= 4 * i + 4 ? 0xFFFFFFFFu : (valid == 4 * i + 2 ? 0x0000FFFFu : 0u);
-            pf[u] = u32x4{d[0], d[1], d[2], d[3]};
-        }
+        if (ur < 16u && uu * 16u < a + span_bytes)
+            __builtin_amdgcn_global_load_lds((const GGQ_GLOBAL void*)(base + (at - a + uu * 16u)), (__attribute__((address_space(3))) void*)(slot + 1024u * i), 16, 0, 0);
     }
 }
 
-template <class F> GGQ_DEV void moe_stash(uint8_t* slice, const u32x4 (&pf)[Mf16Geom<F>::NUW])
+// zeros behind a short last span: blocks that do not exist decode to weights of exactly 0
+template <class F> GGQ_DEV void moe_cut(gcptr rows, uint32_t row_bytes, uint32_t span, uint32_t span_bytes, uint8_t* slot)
 {
     using G = Mf16Geom<F>;
-    const int lane = (int)(threadIdx.x & 63u);
+    using M = MoeGeom<F>;
+    for (uint32_t unit = threadIdx.x & 63u; unit < M::UNITS; unit += 64u) {
+        const uint32_t ur = unit / M::PITCH_U, uu = unit % M::PITCH_U;
+        const uint32_t a = G::SKEW ? moe_offset(rows, ur, row_bytes, span * G::SPAN_BYTES) & 15u : 0u;
+        const int32_t valid = (int32_t)(a + span_bytes) - (int32_t)(uu * 16u);
+        if (valid >= 16) continue;
+        u32x4* at = reinterpret_cast<u32x4*>(slot + unit * 16u);
+        u32x4 d = *at;
 #pragma unroll
-    for (int u = 0; u < G::NUW; u++) {
-        const uint32_t unit = (uint32_t)(lane + 64 * u), ur = unit / (uint32_t)G::U, uu = unit % (uint32_t)G::U;
-        if (ur < 16u) *reinterpret_cast<u32x4*>(slice + ur * G::ROW_STRIDE + uu * 16u) = pf[u];
+        for (int i = 0; i < 4; i++) d[i] &= valid >= 4 * i + 4 ? 0xFFFFFFFFu : (valid == 4 * i + 2 ? 0x0000FFFFu : 0u);
+        *at = d;
     }
+    wave_sync();
 }
 
-// acc += 16 rows of decoded weights (in `slice`, first row at byte `skew` of its pitch) x MB blocks of 16 columns; col[]: this lane's column at element 32 c
-template <class F, int OUT, int MB>
-GGQ_DEV void moe_span(const uint8_t* wspan, const GGQ_GLOBAL uint8_t* const (&col)[MB], uint32_t span, uint32_t k_len, f32x4 (&acc)[MB])
+// at most `KEEP` of this wave's newest loads are still under way
+template <int KEEP> GGQ_DEV void moe_wait() { asm volatile("s_waitcnt vmcnt(%0)" :: "n"(KEEP) : "memory"); }
+
+// this lane's columns of one span: element 128 g + 32 c + 8 t ... + 7 of column (block mb, r) in x[mb][4 g + t].  Lanes without a column (null) load nothing and
+// keep what they hold: a column of the product depends on that column alone.  (One token, 2 x 10240 x 4096: with every lane loading, the columns were 8 KiB
+// per span against 2.3 of weights, and cost 8 of 38 us in the vector cache.)
+template <class F, int MB>
+GGQ_DEV void moe_columns(const GGQ_GLOBAL uint8_t* const (&col)[MB], uint32_t span, uint32_t k_len, u32x4 (&x)[MB][8])
 {
-    constexpr int CPB = F::BS / 8;
     const int c = (int)(threadIdx.x & 63u) >> 4;
 #pragma unroll
-    for (int g = 0; g < 2; g++) {
-        u32x4 xf[MB][4];
+    for (int g = 0; g < 2; g++)
 #pragma unroll
         for (int mb = 0; mb < MB; mb++) {
             const GGQ_GLOBAL uint8_t* src = col[mb] + (uint64_t)span * (MF_SPAN * 2) + (uint32_t)(g * 256);
             if constexpr (F::BS == 32) {                                                                   // past the end of k: zeros
                 if (span * (uint32_t)MF_SPAN + (uint32_t)(128 * g + 32 * c) >= k_len) src = (GGQ_GLOBAL const uint8_t*)MF16_ZEROS;
             }
+            if (col[mb] != nullptr) {
 #pragma unroll
-            for (int t = 0; t < 4; t++) xf[mb][t] = *(GGQ_GLOBAL const u32x4*)(src + t * 16);
+                for (int t = 0; t < 4; t++) x[mb][4 * g + t] = *(GGQ_GLOBAL const u32x4*)(src + t * 16);
+            }
         }
+}
+
+// acc += 16 rows of weights, decoded from one span of packed bytes (`wspan`: this lane's row in LDS), times MB blocks of 16 columns
+template <class F, int OUT, int MB>
+GGQ_DEV void moe_span(const uint8_t* wspan, const u32x4 (&x)[MB][8], f32x4 (&acc)[MB])
+{
+    constexpr int CPB = F::BS / 8;
+    const int c = (int)(threadIdx.x & 63u) >> 4;
+#pragma unroll
+    for (int g = 0; g < 2; g++) {
+        if (g) __builtin_amdgcn_sched_barrier(0);                                                          // the second half's decode stays out of the first one's registers
 #pragma unroll
         for (int t = 0; t < 4; t++) {
             const int j = 16 * g + 4 * c + t;
@@ -197,7 +271,7 @@ GGQ_DEV void moe_span(const uint8_t* wspan, const GGQ_GLOBAL uint8_t* const (&co
             weights8<F, OUT>(f, w);
             const u32x4 wa{w[0], w[1], w[2], w[3]};
 #pragma unroll
-            for (int mb = 0; mb < MB; mb++) acc[mb] = mfma16<OUT>(wa, xf[mb][t], acc[mb]);
+            for (int mb = 0; mb < MB; mb++) acc[mb] = mfma16<OUT>(wa, x[mb][4 * g + t], acc[mb]);
         }
     }
 }
@@ -209,182 +283,290 @@ struct MoeArgs {
     const uint8_t *gate, *up, *down;
     uint8_t* y;
     uint8_t* hidden;                 // [2][tokens * top_k][ff] of the activations' type: the rounded value, then the rest
+    float* part;                     // [parts][tokens][dim]: moe_down's parts of y (parts > 1)
     uint32_t tokens, top_k, experts, dim, ff;
     int act;
+    uint32_t parts, spare, ring;     // spare: blocks of 16 columns beyond the kernel's MB that the tokens could fill (their sums live in LDS); ring: slots of a wave
 };
 
-constexpr int MOE_UP_WAVES = 8, MOE_DOWN_WAVES = 8;
+constexpr int MOE_WAVES = 8;
+// waves per SIMD that the registers are asked to leave room for: with one block of columns 4, two workgroups per CU
+#define MOE_OCC(MB) __attribute__((amdgpu_waves_per_eu((MB) == 1 ? 4 : 2, 8)))
 
-// hidden = act(Wg x) * (Wu x) for 16 hidden rows of one chosen expert.  Waves 0, 2, 4, ... contract gate rows, waves 1, 3, 5, ... up rows.
+// this wave's list of the columns' places: `per` columns for each token of the expert; returns how many columns
+GGQ_DEV uint32_t moe_list(const MoeTable& s, const float* weights, const MoeArgs& a, int expert, uint32_t* slots, float* shares)
+{
+    const uint32_t lane = threadIdx.x & 63u;
+    uint32_t slot;
+    float weight;
+    const uint64_t mask = moe_tokens(s, weights, a.tokens, a.top_k, expert, slot, weight);
+    if ((mask >> lane) & 1u) {
+        const uint32_t at = (uint32_t)__builtin_popcountll(mask & ((1ull << lane) - 1ull));
+        slots[at] = slot;
+        if (shares != nullptr) shares[at] = weight;
+    }
+    wave_sync();
+    return (uint32_t)__builtin_popcountll(mask);
+}
+
+// hidden = act(Wg x) * (Wu x), 16 hidden rows of a chosen expert at a time.  The (expert, tile of 16 rows) list is dealt out evenly: the first workgroups take
+// one tile more.  Waves 0, 2, 4, 6 contract gate rows, waves 1, 3, 5, 7 up rows, every fourth span each.
 template <class F, int OUT, int MB>
-__global__ __launch_bounds__(MOE_UP_WAVES * 64) void moe_up(const MoeArgs a)
+__global__ __launch_bounds__(MOE_WAVES * 64) MOE_OCC(MB) void moe_up(const MoeArgs a)
 {
     using G = Mf16Geom<F>;
-    __shared__ uint32_t words[MOE_WORDS];
-    __shared__ uint32_t slots[MOE_MAX_TOKENS];                                     // per column: where its hidden row goes (= token * top_k + place)
-    constexpr int WORK = MOE_UP_WAVES * G::SLICE > MOE_UP_WAVES * MB * 1024 ? MOE_UP_WAVES * G::SLICE : MOE_UP_WAVES * MB * 1024;
-    __shared__ __attribute__((aligned(16))) uint8_t work[WORK];
+    // per wave: the sums of columns beyond MB blocks ([spare][64] f32x4), then, for all waves, the rings
+    extern __shared__ __attribute__((aligned(16))) uint8_t dyn[];
+    __shared__ MoeTable table;
+    __shared__ uint32_t slots_[MOE_WAVES][MOE_MAX_TOKENS];                         // per column: where its hidden row goes (= token * top_k + place)
+    constexpr int TURNS = MB == 1 ? 2 : 1;                                         // two tiles' partial sums: the next tile's are written while one is added up
+    __shared__ f32x4 red[TURNS][MOE_WAVES][MB][64];
     const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const uint32_t lane = threadIdx.x & 63u, r = lane & 15u, c = lane >> 4;
     const uint32_t pairs = a.tokens * a.top_k;
+    moe_table(table, a.ids, pairs, a.experts);
 
-    moe_mark(words, a.ids, pairs, a.experts);
-    const int expert = moe_nth(words, blockIdx.y);
-    if (expert < 0) return;                                                        // fewer experts than the grid allows for
-    uint32_t slot;
-    float weight;
-    const uint64_t mask = moe_tokens(a.ids, a.weights, a.tokens, a.top_k, expert, slot, weight);
-    const uint32_t n_cols = (uint32_t)__builtin_popcountll(mask);
-    if (wave == 0 && ((mask >> lane) & 1u)) slots[__builtin_popcountll(mask & ((1ull << lane) - 1ull))] = slot;
-    __syncthreads();
-
-    const uint32_t row0 = blockIdx.x * 16u;
+    const uint32_t tiles = a.ff / 16u, total = table.n * tiles, each = total / gridDim.x, more = total - each * gridDim.x;
+    const uint32_t t0 = blockIdx.x * each + (blockIdx.x < more ? blockIdx.x : more), t1 = t0 + each + (blockIdx.x < more ? 1u : 0u);
     const uint64_t row_bytes = (uint64_t)(a.dim / F::BS) * F::TS;
-    const uint32_t n_spans = (a.dim + MF_SPAN - 1) / MF_SPAN, tail_len = a.dim - (n_spans - 1) * (uint32_t)MF_SPAN;
-    const gcptr rows = (gcptr)((wave & 1u) ? a.up : a.gate) + ((uint64_t)(uint32_t)expert * a.ff + row0) * row_bytes;
-    uint8_t* slice = work + wave * G::SLICE;
-    for (uint32_t c0 = 0; c0 < n_cols; c0 += MB * 16) {                            // more columns than fit: the rows are read again, from the caches
+    const uint32_t n_spans = (a.dim + MF_SPAN - 1) / MF_SPAN, tail_len = a.dim - (n_spans - 1) * (uint32_t)MF_SPAN, span0 = wave >> 1;
+    const gcptr weights = (gcptr)((wave & 1u) ? a.up : a.gate);
+    uint8_t* ring = dyn + MOE_WAVES * a.spare * 1024u + wave * a.ring * (uint32_t)G::SLICE;
+    uint32_t* slots = slots_[wave];
+    f32x4* spare = reinterpret_cast<f32x4*>(dyn) + (uint64_t)wave * a.spare * 64u;
+    uint32_t turn = 0;
+    for (uint32_t t = t0; t < t1;) {                                               // one expert at a time: tiles [t, stop) of the list
+        const uint32_t nth = t / tiles, stop = (nth + 1) * tiles < t1 ? (nth + 1) * tiles : t1;
+        const uint32_t n_cols = moe_list(table, nullptr, a, table.list[nth], slots, nullptr);
+        const gcptr base = weights + (uint64_t)table.list[nth] * a.ff * row_bytes;
+        auto weights_at = [&](uint32_t i) { return base + (uint64_t)(i - nth * tiles) * 16u * row_bytes; };        // tile i of the list
+        auto column = [&](uint32_t v) { return v < n_cols ? (GGQ_GLOBAL const uint8_t*)a.x + (uint64_t)(slots[v] / a.top_k) * a.dim * 2 + c * 64u : nullptr; };
         const GGQ_GLOBAL uint8_t* col[MB];
 #pragma unroll
-        for (int mb = 0; mb < MB; mb++) {
-            const uint32_t v = c0 + (uint32_t)(mb * 16) + r;
-            col[mb] = (GGQ_GLOBAL const uint8_t*)a.x + (uint64_t)(slots[v < n_cols ? v : 0u] / a.top_k) * a.dim * 2 + c * 64u;
-        }
+        for (int mb = 0; mb < MB; mb++) col[mb] = column((uint32_t)(mb * 16) + r);
+        const uint32_t blocks = (n_cols + 15u) / 16u;
+
+        uint32_t ft = t, fs = span0, in = 0, out = 0;                              // the next span to request; ring slots
+        auto request = [&]() {                                                     // -> 2: a whole span, 1: a short one, 0: nothing left
+            if (ft >= stop || fs >= n_spans) return 0;
+            const bool tail = F::BS == 32 && fs + 1 == n_spans && tail_len != (uint32_t)MF_SPAN;
+            moe_request<F>(weights_at(ft), (uint32_t)row_bytes, fs, (tail ? tail_len : (uint32_t)MF_SPAN) / (uint32_t)F::BS * (uint32_t)F::TS, ring + in * G::SLICE);
+            in = in + 1 == a.ring ? 0 : in + 1;
+            fs += MOE_WAVES / 2;
+            if (fs >= n_spans) { fs = span0; ft++; }
+            return tail ? 1 : 2;
+        };
+        request();
+        if (a.ring > 2) request();
         f32x4 acc[MB];
+        auto clear = [&]() {
 #pragma unroll
-        for (int mb = 0; mb < MB; mb++) acc[mb] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        u32x4 pf[G::NUW];
-        uint32_t span = wave >> 1;
-        if (span < n_spans) moe_fetch<F>(rows, row_bytes, span, n_spans, tail_len, pf);
-        for (; span < n_spans; span += MOE_UP_WAVES / 2) {
-            moe_stash<F>(slice, pf);
-            wave_sync();
-            if (span + MOE_UP_WAVES / 2 < n_spans) moe_fetch<F>(rows, row_bytes, span + MOE_UP_WAVES / 2, n_spans, tail_len, pf);
-            const uint32_t skew = G::SKEW ? (uint32_t)(uintptr_t)(rows + (uint64_t)r * row_bytes + (uint64_t)span * G::SPAN_BYTES) & 15u : 0u;
-            moe_span<F, OUT, MB>(slice + r * G::ROW_STRIDE + skew, col, span, a.dim, acc);
-            wave_sync();
-        }
-        __syncthreads();
-        f32x4* red = reinterpret_cast<f32x4*>(work);
-#pragma unroll
-        for (int mb = 0; mb < MB; mb++) red[(wave * MB + (uint32_t)mb) * 64u + lane] = acc[mb];
-        __syncthreads();
-        if (wave < (uint32_t)MB) {
-            f32x4 g = red[wave * 64u + lane], u = red[(MB + wave) * 64u + lane];
-            for (uint32_t w = 2; w < MOE_UP_WAVES; w += 2) {
-                g += red[(w * MB + wave) * 64u + lane];
-                u += red[((w + 1) * MB + wave) * 64u + lane];
+            for (int mb = 0; mb < MB; mb++) acc[mb] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            for (uint32_t q = MB; q < blocks; q++) spare[(q - MB) * 64u + lane] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        };
+        uint32_t tile = t - nth * tiles, span = span0;
+        const uint32_t tile_end = stop - nth * tiles;
+        auto one = [&]() {
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");                     // the slot that is filled next has been read
+            u32x4 x[MB][8];
+            moe_columns<F, MB>(col, span, a.dim, x);
+            asm volatile("" ::: "memory");
+            if (request() == 2) moe_wait<(int)MoeGeom<F>::LOADS>();                // all but the span just requested
+            else moe_wait<0>();
+            uint8_t* slot = ring + out * G::SLICE;
+            out = out + 1 == a.ring ? 0 : out + 1;
+            const gcptr rows = weights_at(nth * tiles + tile);
+            if (F::BS == 32 && span + 1 == n_spans && tail_len != (uint32_t)MF_SPAN) moe_cut<F>(rows, (uint32_t)row_bytes, span, tail_len / (uint32_t)F::BS * (uint32_t)F::TS, slot);
+            const uint32_t skew = G::SKEW ? moe_offset(rows, r, (uint32_t)row_bytes, span * G::SPAN_BYTES) & 15u : 0u;
+            moe_span<F, OUT, MB>(slot + r * G::ROW_STRIDE + skew, x, acc);
+            for (uint32_t q = MB; q < blocks; q++) {                               // more tokens on one expert than the kernel was picked for
+                const GGQ_GLOBAL uint8_t* const late[1] = {column(q * 16u + r)};
+                u32x4 lx[1][8];
+                f32x4 sum[1] = {spare[(q - MB) * 64u + lane]};
+                moe_columns<F, 1>(late, span, a.dim, lx);
+                moe_span<F, OUT, 1>(slot + r * G::ROW_STRIDE + skew, lx, sum);
+                spare[(q - MB) * 64u + lane] = sum[0];
             }
-            const uint32_t v = c0 + wave * 16u + r;                                // D[row = 4c + i][column = r]
-            if (v < n_cols) {
-                uint32_t hi[2], lo[2];
+            wave_sync();
+            span += MOE_WAVES / 2;
+        };
+        // the sums of a tile over the waves, the activation, the two parts of the hidden value; the waves take turns at it
+        auto finish = [&]() {
 #pragma unroll
-                for (int p = 0; p < 2; p++) {
-                    float h0 = moe_act(g[2 * p], a.act) * u[2 * p], h1 = moe_act(g[2 * p + 1], a.act) * u[2 * p + 1];
-                    asm volatile("" : "+v"(h0), "+v"(h1));                         // the product rounded to fp32 (no v_fma_mix with the conversion): both parts see it
-                    if constexpr (OUT == OUT_F16) {
-                        const h2 q{(_Float16)h0, (_Float16)h1};
-                        hi[p] = as_u32(q);
-                        lo[p] = as_u32(h2{(_Float16)__builtin_ldexpf(h0 - (float)q.x, 11), (_Float16)__builtin_ldexpf(h1 - (float)q.y, 11)});
-                    } else {
-                        hi[p] = pack_bf16(h0, h1);
-                        lo[p] = pack_bf16(h0 - bits_f32(hi[p] << 16), h1 - bits_f32(hi[p] & 0xFFFF0000u));
+            for (int mb = 0; mb < MB; mb++) red[turn][wave][mb][lane] = acc[mb];
+            moe_barrier();
+            for (uint32_t q = (wave - tile * MB) % MOE_WAVES; q < blocks; q += MOE_WAVES) {
+                auto sum = [&](uint32_t w) { return q < (uint32_t)MB ? red[turn][w][q][lane] : reinterpret_cast<const f32x4*>(dyn)[(uint64_t)(w * a.spare + q - MB) * 64u + lane]; };
+                f32x4 g = sum(0), u = sum(1);
+                for (uint32_t w = 2; w < MOE_WAVES; w += 2) { g += sum(w); u += sum(w + 1); }
+                const uint32_t v = q * 16u + r;                                    // D[row = 4c + i][column = r]
+                if (v < n_cols) {
+                    uint32_t hi[2], lo[2];
+#pragma unroll
+                    for (int p = 0; p < 2; p++) {
+                        float h0 = moe_act(g[2 * p], a.act) * u[2 * p], h1 = moe_act(g[2 * p + 1], a.act) * u[2 * p + 1];
+                        asm volatile("" : "+v"(h0), "+v"(h1));                     // the product rounded to fp32 (no v_fma_mix with the conversion): both parts see it
+                        if constexpr (OUT == OUT_F16) {
+                            const h2 n{(_Float16)h0, (_Float16)h1};
+                            hi[p] = as_u32(n);
+                            lo[p] = as_u32(h2{(_Float16)__builtin_ldexpf(h0 - (float)n.x, 11), (_Float16)__builtin_ldexpf(h1 - (float)n.y, 11)});
+                        } else {
+                            hi[p] = pack_bf16(h0, h1);
+                            lo[p] = pack_bf16(h0 - bits_f32(hi[p] << 16), h1 - bits_f32(hi[p] & 0xFFFF0000u));
+                        }
                     }
+                    uint8_t* dst = a.hidden + ((uint64_t)slots[v] * a.ff + tile * 16u + 4u * c) * 2;
+                    *reinterpret_cast<u32x2*>(dst) = u32x2{hi[0], hi[1]};
+                    *reinterpret_cast<u32x2*>(dst + (uint64_t)pairs * a.ff * 2) = u32x2{lo[0], lo[1]};
                 }
-                uint8_t* dst = a.hidden + ((uint64_t)slots[v] * a.ff + row0 + 4u * c) * 2;
-                *reinterpret_cast<u32x2*>(dst) = u32x2{hi[0], hi[1]};
-                *reinterpret_cast<u32x2*>(dst + (uint64_t)pairs * a.ff * 2) = u32x2{lo[0], lo[1]};
             }
+            if (TURNS == 1 || blocks > (uint32_t)MB) moe_barrier();                // the same sums' place is written next
+            else turn ^= 1u;
+            tile++;
+            span = span0;
+            clear();
+        };
+        clear();
+        while (tile < tile_end) {
+            if (span < n_spans) one();
+            if (span >= n_spans) finish();
         }
-        __syncthreads();                                                           // the partial sums become weight slices again
+        t = stop;
     }
 }
 
-// 16 rows of y for every token.  A wave's columns are (token, part of the hidden vector): column 2 i the value, 2 i + 1 the rest of token i of the expert.
+// 16 rows of y for every token; of gridDim.y = `parts` workgroups each takes a part of the (expert, span) list, and each of its waves an equal part of
+// that, one wave after the other.  A wave's columns are (token, part of the hidden vector): column 2 i the value, 2 i + 1 the rest of token i of the expert.
 template <class F, int OUT, int MB>
-__global__ __launch_bounds__(MOE_DOWN_WAVES * 64) void moe_down(const MoeArgs a)
+__global__ __launch_bounds__(MOE_WAVES * 64) MOE_OCC(MB) void moe_down(const MoeArgs a)
 {
     using G = Mf16Geom<F>;
-    extern __shared__ __attribute__((aligned(16))) uint8_t dyn[];                  // y of each wave: [wave][token][16] floats
-    __shared__ uint32_t words[MOE_WORDS];
-    __shared__ uint32_t slots[MOE_DOWN_WAVES][MOE_MAX_TOKENS];
-    __shared__ float shares[MOE_DOWN_WAVES][MOE_MAX_TOKENS];
-    __shared__ __attribute__((aligned(16))) uint8_t work[MOE_DOWN_WAVES * G::SLICE];
+    // y of each wave ([wave][token][16] floats), sums of columns beyond MB blocks ([wave][spare][64] f32x4), the rings
+    extern __shared__ __attribute__((aligned(16))) uint8_t dyn[];
+    __shared__ MoeTable table;
+    __shared__ float shares_all[MOE_MAX_TOKENS * MOE_MAX_TOPK];
+    __shared__ uint32_t slots_[MOE_WAVES][MOE_MAX_TOKENS];
+    __shared__ float shares_[MOE_WAVES][MOE_MAX_TOKENS];
     const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const uint32_t lane = threadIdx.x & 63u, r = lane & 15u, c = lane >> 4;
     const uint32_t pairs = a.tokens * a.top_k;
     float* part = reinterpret_cast<float*>(dyn) + (uint64_t)wave * a.tokens * 16u;
+    f32x4* spare = reinterpret_cast<f32x4*>(dyn + (uint64_t)MOE_WAVES * a.tokens * 64u) + (uint64_t)wave * a.spare * 64u;
     for (uint32_t i = lane; i < a.tokens * 16u; i += 64u) part[i] = 0.0f;
+    for (uint32_t p = threadIdx.x; p < pairs; p += MOE_WAVES * 64) shares_all[p] = a.weights[p];
+    moe_table(table, a.ids, pairs, a.experts);
 
-    moe_mark(words, a.ids, pairs, a.experts);
-    uint32_t n_experts = 0;
-    for (int w = 0; w < MOE_WORDS; w++) n_experts += (uint32_t)__builtin_popcount(words[w]);
     const uint32_t row0 = blockIdx.x * 16u;
-    const uint64_t row_bytes = (uint64_t)(a.ff / F::BS) * F::TS;
+    const uint64_t row_bytes = (uint64_t)(a.ff / F::BS) * F::TS, expert_bytes = (uint64_t)a.dim * row_bytes;
     const uint32_t n_spans = (a.ff + MF_SPAN - 1) / MF_SPAN, tail_len = a.ff - (n_spans - 1) * (uint32_t)MF_SPAN;
-    const uint32_t items = n_experts * n_spans, each = (items + MOE_DOWN_WAVES - 1) / MOE_DOWN_WAVES;
-    const uint32_t last = (wave + 1) * each < items ? (wave + 1) * each : items;
-    uint8_t* slice = work + wave * G::SLICE;
+    const gcptr base = (gcptr)a.down + (uint64_t)row0 * row_bytes;
+    const uint64_t items = (uint64_t)table.n * n_spans, share = blockIdx.y * MOE_WAVES + wave, all = (uint64_t)a.parts * MOE_WAVES;
+    const uint32_t first = (uint32_t)(items * share / all), last = (uint32_t)(items * (share + 1) / all);
+    uint8_t* ring = dyn + MOE_WAVES * (a.tokens * 64u + a.spare * 1024u) + wave * a.ring * (uint32_t)G::SLICE;
+    uint32_t* slots = slots_[wave];
+    float* shares = shares_[wave];
 
-    for (uint32_t item = wave * each; item < last;) {                              // one expert at a time: items [item, stop)
-        const uint32_t nth = item / n_spans, span0 = item - nth * n_spans;
-        const uint32_t stop = (nth + 1) * n_spans < last ? (nth + 1) * n_spans : last, span1 = span0 + (stop - item);
-        const int expert = moe_nth(words, nth);
-        uint32_t slot;
-        float weight;
-        const uint64_t mask = moe_tokens(a.ids, a.weights, a.tokens, a.top_k, expert, slot, weight);
-        const uint32_t n_cols = 2u * (uint32_t)__builtin_popcountll(mask);
-        if ((mask >> lane) & 1u) {
-            const uint32_t at = (uint32_t)__builtin_popcountll(mask & ((1ull << lane) - 1ull));
-            slots[wave][at] = slot;
-            shares[wave][at] = weight;
+    uint32_t fi = first, fn = first / n_spans, fs = first % n_spans, in = 0, out = 0;      // the next span to request, also of the next expert; ring slots
+    auto request = [&]() {                                                         // -> 2: a whole span, 1: a short one, 0: nothing left
+        if (fi >= last) return 0;
+        const bool tail = F::BS == 32 && fs + 1 == n_spans && tail_len != (uint32_t)MF_SPAN;
+        moe_request<F>(base + (uint64_t)table.list[fn] * expert_bytes, (uint32_t)row_bytes, fs, (tail ? tail_len : (uint32_t)MF_SPAN) / (uint32_t)F::BS * (uint32_t)F::TS, ring + in * G::SLICE);
+        in = in + 1 == a.ring ? 0 : in + 1;
+        fi++;
+        if (++fs == n_spans) { fs = 0; fn++; }
+        return tail ? 1 : 2;
+    };
+    request();
+    if (a.ring > 2) request();
+
+    uint32_t item = first, nth = first / n_spans, span = first % n_spans, n_cols = 0, blocks = 0;
+    gcptr rows = base;
+    const GGQ_GLOBAL uint8_t* col[MB];
+    f32x4 acc[MB];
+    auto column = [&](uint32_t v) {
+        return v < n_cols ? (GGQ_GLOBAL const uint8_t*)a.hidden + ((uint64_t)(v & 1u) * pairs + slots[v >> 1]) * a.ff * 2 + c * 64u : nullptr;
+    };
+    auto start = [&]() {                                                           // the columns of the next expert
+        n_cols = 2u * moe_list(table, shares_all, a, table.list[nth], slots, shares);
+        blocks = (n_cols + 15u) / 16u;
+        rows = base + (uint64_t)table.list[nth] * expert_bytes;
+#pragma unroll
+        for (int mb = 0; mb < MB; mb++) {
+            col[mb] = column((uint32_t)(mb * 16) + r);
+            acc[mb] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+        for (uint32_t q = MB; q < blocks; q++) spare[(q - MB) * 64u + lane] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    };
+    auto one = [&]() {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");                         // the slot that is filled next has been read
+        u32x4 x[MB][8];
+        moe_columns<F, MB>(col, span, a.ff, x);
+        asm volatile("" ::: "memory");
+        if (request() == 2) moe_wait<(int)MoeGeom<F>::LOADS>();                    // all but the span just requested
+        else moe_wait<0>();
+        uint8_t* slot = ring + out * G::SLICE;
+        out = out + 1 == a.ring ? 0 : out + 1;
+        if (F::BS == 32 && span + 1 == n_spans && tail_len != (uint32_t)MF_SPAN) moe_cut<F>(rows, (uint32_t)row_bytes, span, tail_len / (uint32_t)F::BS * (uint32_t)F::TS, slot);
+        const uint32_t skew = G::SKEW ? moe_offset(rows, r, (uint32_t)row_bytes, span * G::SPAN_BYTES) & 15u : 0u;
+        moe_span<F, OUT, MB>(slot + r * G::ROW_STRIDE + skew, x, acc);
+        for (uint32_t q = MB; q < blocks; q++) {                                   // more tokens on one expert than the kernel was picked for
+            const GGQ_GLOBAL uint8_t* const late[1] = {column(q * 16u + r)};
+            u32x4 lx[1][8];
+            f32x4 sum[1] = {spare[(q - MB) * 64u + lane]};
+            moe_columns<F, 1>(late, span, a.ff, lx);
+            moe_span<F, OUT, 1>(slot + r * G::ROW_STRIDE + skew, lx, sum);
+            spare[(q - MB) * 64u + lane] = sum[0];
         }
         wave_sync();
-        const gcptr rows = (gcptr)a.down + ((uint64_t)(uint32_t)expert * a.dim + row0) * row_bytes;
-        for (uint32_t c0 = 0; c0 < n_cols; c0 += MB * 16) {
-            const GGQ_GLOBAL uint8_t* col[MB];
+        item++;
+        span++;
+    };
+    // D[row = 4c + i][column = r]: value and rest are neighbouring lanes; the even one adds the token's share to its wave's y
+    auto add = [&](uint32_t q, f32x4 sum) {
+        const uint32_t v = q * 16u + r;
 #pragma unroll
-            for (int mb = 0; mb < MB; mb++) {
-                const uint32_t v0 = c0 + (uint32_t)(mb * 16) + r, v = v0 < n_cols ? v0 : 0u;
-                col[mb] = (GGQ_GLOBAL const uint8_t*)a.hidden + ((uint64_t)(v & 1u) * pairs + slots[wave][v >> 1]) * a.ff * 2 + c * 64u;
-            }
-            f32x4 acc[MB];
-#pragma unroll
-            for (int mb = 0; mb < MB; mb++) acc[mb] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-            u32x4 pf[G::NUW];
-            moe_fetch<F>(rows, row_bytes, span0, n_spans, tail_len, pf);
-            for (uint32_t span = span0; span < span1; span++) {
-                moe_stash<F>(slice, pf);
-                wave_sync();
-                if (span + 1 < span1) moe_fetch<F>(rows, row_bytes, span + 1, n_spans, tail_len, pf);
-                const uint32_t skew = G::SKEW ? (uint32_t)(uintptr_t)(rows + (uint64_t)r * row_bytes + (uint64_t)span * G::SPAN_BYTES) & 15u : 0u;
-                moe_span<F, OUT, MB>(slice + r * G::ROW_STRIDE + skew, col, span, a.ff, acc);
-                wave_sync();
-            }
-            // D[row = 4c + i][column = r]: value and rest are neighbouring lanes; the even one adds the token's share to its wave's y
-#pragma unroll
-            for (int mb = 0; mb < MB; mb++) {
-                const uint32_t v = c0 + (uint32_t)(mb * 16) + r;
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    float rest = dpp_f<0xB1, 0xF>(acc[mb][i]);                     // the neighbour's sum
-                    if constexpr (OUT == OUT_F16) rest *= 1.0f / 2048.0f;
-                    if (v < n_cols && (v & 1u) == 0) part[slots[wave][v >> 1] / a.top_k * 16u + 4u * c + (uint32_t)i] += shares[wave][v >> 1] * (acc[mb][i] + rest);
-                }
-            }
+        for (int i = 0; i < 4; i++) {
+            float rest = dpp_f<0xB1, 0xF>(sum[i]);                                 // the neighbour's sum
+            if constexpr (OUT == OUT_F16) rest *= 1.0f / 2048.0f;
+            if (v < n_cols && (v & 1u) == 0) part[slots[v >> 1] / a.top_k * 16u + 4u * c + (uint32_t)i] += shares[v >> 1] * (sum[i] + rest);
         }
+    };
+    auto finish = [&]() {
+#pragma unroll
+        for (int mb = 0; mb < MB; mb++) add((uint32_t)mb, acc[mb]);
+        for (uint32_t q = MB; q < blocks; q++) add(q, spare[(q - MB) * 64u + lane]);
         wave_sync();
-        item = stop;
+        nth++;
+        span = 0;
+        if (item < last) start();
+    };
+    if (item < last) start();
+    while (item < last) {
+        one();
+        if (span == n_spans || item == last) finish();
     }
     __syncthreads();
-    for (uint32_t i = threadIdx.x; i < a.tokens * 16u; i += MOE_DOWN_WAVES * 64) {
-        const float* all = reinterpret_cast<const float*>(dyn);
-        float v = all[i];
-        for (uint32_t w = 1; w < MOE_DOWN_WAVES; w++) v += all[(uint64_t)w * a.tokens * 16u + i];
+    for (uint32_t i = threadIdx.x; i < a.tokens * 16u; i += MOE_WAVES * 64) {
+        const float* sums = reinterpret_cast<const float*>(dyn);
+        float v = sums[i];
+        for (uint32_t w = 1; w < MOE_WAVES; w++) v += sums[(uint64_t)w * a.tokens * 16u + i];
         const uint64_t at = (uint64_t)(i >> 4) * a.dim + row0 + (i & 15u);
-        if constexpr (OUT == OUT_F16) reinterpret_cast<_Float16*>(a.y)[at] = (_Float16)v;
+        if (a.parts > 1) a.part[(uint64_t)blockIdx.y * a.tokens * a.dim + at] = v;
+        else if constexpr (OUT == OUT_F16) reinterpret_cast<_Float16*>(a.y)[at] = (_Float16)v;
         else reinterpret_cast<uint16_t*>(a.y)[at] = (uint16_t)(pack_bf16(v, 0.0f) & 0xFFFFu);
     }
+}
+
+// y = the parts of moe_down in order, four values per lane
+template <int OUT>
+__global__ __launch_bounds__(256) void moe_combine(const float* __restrict__ part, uint8_t* __restrict__ y, uint32_t parts, uint32_t quads)
+{
+    const uint32_t i = blockIdx.x * 256u + threadIdx.x;
+    if (i >= quads) return;
+    f32x4 v = reinterpret_cast<const f32x4*>(part)[i];
+    for (uint32_t p = 1; p < parts; p++) v += reinterpret_cast<const f32x4*>(part)[(uint64_t)p * quads + i];
+    if constexpr (OUT == OUT_F16) reinterpret_cast<u32x2*>(y)[i] = u32x2{pack_f16(v.x, v.y), pack_f16(v.z, v.w)};
+    else reinterpret_cast<u32x2*>(y)[i] = u32x2{pack_bf16(v.x, v.y), pack_bf16(v.z, v.w)};
 }
 
 }  // namespace ggq

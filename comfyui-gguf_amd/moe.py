@@ -19,13 +19,13 @@ from .norms import _on_gpu, _plain, _refuse_grad
 
 MAX_TOKENS, MAX_TOP_K, MAX_EXPERTS = 64, 16, 512
 ACTIVATIONS = {"silu": 0, "gelu_tanh": 1}
-_route_call = _experts_call = None
+_route_call = _experts_call = _workspace = None
 
 
 def _bind():
-    global _route_call, _experts_call
+    global _route_call, _experts_call, _workspace
     L = _native.lib()
-    _route_call, _experts_call = L.ggq_moe_route, L.ggq_moe_experts
+    _route_call, _experts_call, _workspace = L.ggq_moe_route, L.ggq_moe_experts, L.ggq_moe_workspace
 
 
 def _rows16(x, what, f32=False):
@@ -113,12 +113,12 @@ def _experts(x, ids, weights, gate, up, down, activation):
     if ids.dtype is torch.int64:
         ids = ids.clamp(-1, experts).int()          # what is no expert stays none in 32 bits
     ids, weights = ids.contiguous(), weights.to(torch.float32).contiguous()
-    size = tokens * top_k * ff * 4
+    if _experts_call is None:
+        _bind()
+    size = int(_workspace(tokens, top_k, dim, ff))
     scratch = torch.empty(size, dtype=torch.uint8, device=device)
     d = _native.ggq_moe_desc(x.data_ptr(), ids.data_ptr(), weights.data_ptr(), gate.data_ptr(), up.data_ptr(), down.data_ptr(), y.data_ptr(), scratch.data_ptr(), size,
                              tokens, top_k, experts, dim, ff, up_id, down_id, ACTIVATIONS[activation], _OUT_CODE[x.dtype])
-    if _experts_call is None:
-        _bind()
     _with_device(device, _experts_call, "ggq_moe_experts", ctypes.byref(d))
     return y
 

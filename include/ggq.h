@@ -266,8 +266,9 @@ int ggq_moe_route(const void* x, const void* router, uint32_t tokens, uint32_t d
 /* y[t] = sum_s weights[t, s] * Wd[e] (act(Wg[e] x[t]) * (Wu[e] x[t])), e = ids[t, s], straight from packed expert weights: gate and up are packed stacks of
  * logical shape (experts, ff, dim) in one format, down (experts, dim, ff) in its own; W = the fp16 values of the packed blocks in `dtype`, as
  * dequantize_tensor gives.  1 <= tokens <= 64 (GGQ_ERR_ARG above), top_k <= 16, experts <= 512, dim and ff multiples of 256 (of 64 where the format that
- * contracts over them has 32-element blocks).  An id outside [0, experts) adds nothing; the same id twice counts twice.  act: 0 silu, 1 gelu
- * (tanh form).  x, y: tokens x dim of `dtype` (GGQ_F16 / GGQ_BF16).  workspace: ggq_moe_workspace() bytes, 16-byte aligned, used until the call's
+ * contracts over them has 32-element blocks) up to 2^24.  An id outside [0, experts) adds nothing; the same id twice counts twice.  act: 0 silu, 1 gelu
+ * (tanh form).  x, y: tokens x dim of `dtype` (GGQ_F16 / GGQ_BF16),
+ * y 8-byte aligned.  workspace: ggq_moe_workspace() bytes, 16-byte aligned, used until the call's
  * kernels have run.  Sums in fp32; the hidden vector is kept in two parts of `dtype` (its value and what rounding left), fp16 hidden values above
  * 65504 overflow.  Deterministic.
  * Replaces: one get_weight + F.linear (ops.py:242-244) per expert and projection. */
@@ -285,7 +286,7 @@ typedef struct ggq_moe_desc {
     int32_t up_qtype, down_qtype, act, dtype;
 } ggq_moe_desc;
 int ggq_moe_experts(const ggq_moe_desc* desc, void* hip_stream);
-uint64_t ggq_moe_workspace(uint32_t tokens, uint32_t top_k, uint32_t ff);
+uint64_t ggq_moe_workspace(uint32_t tokens, uint32_t top_k, uint32_t dim, uint32_t ff);
 
 #ifdef __cplusplus
 }

@@ -38,7 +38,7 @@ def test_block_norm_arguments_at_the_c_entry(pkg):
     assert L.ggq_block_norm(None, None) == n.GGQ_ERR_ARG
     assert call(rows=0) == n.GGQ_OK
     for bad in (dict(dtype=3), dict(dtype=-1), dict(norm=3), dict(post_norm=-1), dict(dim=0), dict(rows_per_mod=0), dict(stream=None), dict(branch=A), dict(y=None),
-                dict(y_scale=A, y_stride=63), dict(y_scale=A, y_stride=72), dict(y_scale=A, y=None, branch=A, stream_out=A, y_stride=64), dict(dim=32769), dict(rows=1 << 40)):
+                dict(y_scale=A, y_stride=63), dict(y_scale=A, y_stride=72), dict(y_scale=A, y=None, branch=A, stream_out=A, y_stride=64), dict(dim=32769)):
         assert call(**bad) == n.GGQ_ERR_ARG, bad
     for bad in (dict(stream=A + 1), dict(y=A + 1), dict(y_scale=A, y_stride=64, y=A + 8), dict(weight=A + 1), dict(weight=A + 2, params_f32=4), dict(dtype=n.F32, stream=A + 2)):
         assert call(**bad) == n.GGQ_ERR_ALIGN, bad
@@ -75,9 +75,10 @@ def test_expert_arguments_at_the_c_entry(pkg):
     assert L.ggq_moe_experts(None, None) == n.GGQ_ERR_ARG
     assert call(tokens=0) == n.GGQ_OK
     assert call(up_qtype=16) == n.GGQ_ERR_QTYPE and call(down_qtype=0) == n.GGQ_ERR_QTYPE
-    for bad in (dict(x=None), dict(ids=None), dict(weights=None), dict(gate=None), dict(up=None), dict(down=None), dict(y=None), dict(workspace=None), dict(workspace_bytes=4 * 2 * 512 * 4 - 1),
+    for bad in (dict(x=None), dict(ids=None), dict(weights=None), dict(gate=None), dict(up=None), dict(down=None), dict(y=None), dict(workspace=None), dict(workspace_bytes=L.ggq_moe_workspace(4, 2, 256, 512) - 1),
                 dict(tokens=65), dict(top_k=0), dict(top_k=17), dict(experts=0), dict(experts=513), dict(dim=192), dict(dim=0), dict(ff=320), dict(ff=0), dict(act=2), dict(dtype=n.F32)):
         assert call(**bad) == n.GGQ_ERR_ARG, bad
-    for bad in (dict(x=A + 8), dict(gate=A + 8), dict(workspace=A + 8), dict(ids=A + 2), dict(y=A + 1)):
+    for bad in (dict(x=A + 8), dict(gate=A + 8), dict(workspace=A + 8), dict(ids=A + 2), dict(y=A + 4)):
         assert call(**bad) == n.GGQ_ERR_ALIGN, bad
-    assert L.ggq_moe_workspace(64, 16, 1 << 20) == 64 * 16 * 4 << 20
+    assert L.ggq_moe_workspace(64, 16, 1 << 20, 1 << 20) == 64 * 16 * 4 << 20              # one part: the hidden values alone
+    assert L.ggq_moe_workspace(3, 2, 256, 512) > 3 * 2 * 512 * 4

@@ -137,6 +137,25 @@ def test_ids_that_are_no_experts_and_experts_twice(pkg, kind):
     assert pkg.moe.moe_experts(x[:0], ids[:0], weights[:0], gate.tensor, up.tensor, down.tensor).shape == (0, 512)
 
 
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("tokens,experts", [(64, 64), (40, 33), (64, 5), (17, 64), (9, 3)])
+def test_all_tokens_on_one_expert(pkg, kind, tokens, experts):
+    """Far more tokens on one expert than evenly spread choices give (the kernels are picked for those): every block of 16 columns, in the registers or not; beside it
+    an expert with one token, and many tiles per workgroup."""
+    dtype = DT[kind]
+    g = torch.Generator(device=DEV)
+    g.manual_seed(51)
+    gate, up, down = _model(pkg, kind, experts=experts, dim=256, ff=512, up="Q5_0", down="Q3_K")
+    x = (torch.randn(tokens, 256, device=DEV, generator=g) * 0.5).to(dtype)
+    ids = torch.full((tokens, 2), experts - 1, device=DEV, dtype=torch.int32)
+    ids[:, 1] = -1
+    ids[3, 1] = 1
+    weights = torch.rand(tokens, 2, device=DEV, generator=g)
+    y = pkg.moe.moe_experts(x, ids, weights, gate.tensor, up.tensor, down.tensor)
+    want, bound = _want(x, ids, weights, gate.dense, up.dense, down.dense, "silu", dtype)
+    _close(y, want, bound, dtype)
+
+
 def test_hidden_values_of_all_sizes(pkg):
     """bf16: hidden values from 1e-30 to 1e8 keep their 16 bits (the two parts share no range).  fp16: small hidden values do not fall into the subnormals."""
     g = torch.Generator(device=DEV)
