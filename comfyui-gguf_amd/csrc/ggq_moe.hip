@@ -9,11 +9,11 @@ using namespace ggq;
 
 typedef hipError_t (*moe_fn)(MoeArgs, hipStream_t);
 
-// Slots of a wave's ring, given the rest of a workgroup's LDS: three where two workgroups then still fit a CU (160 KiB) or would not with two slots either.
+// Slots of a wave's ring, given the rest of a workgroup's LDS: three where as many workgroups then still fit a CU (160 KiB) as with two.
 constexpr uint32_t HALF_LDS = 80u * 1024u, ALL_LDS = 160u * 1024u;
-uint32_t ring_slots(uint32_t rest, uint32_t slot_bytes)
+uint32_t ring_slots(uint32_t rest, uint32_t waves, uint32_t slot_bytes)
 {
-    const uint32_t two = rest + MOE_WAVES * 2u * slot_bytes, three = rest + MOE_WAVES * 3u * slot_bytes;
+    const uint32_t two = rest + waves * 2u * slot_bytes, three = rest + waves * 3u * slot_bytes;
     if (three <= HALF_LDS) return 3u;
     if (two <= HALF_LDS) return 2u;
     return three <= ALL_LDS ? 3u : 2u;
@@ -26,7 +26,7 @@ hipError_t launch_up(MoeArgs a, hipStream_t s)
     const uint32_t pairs = a.tokens * a.top_k, most = (pairs < a.experts ? pairs : a.experts) * (a.ff / 16u);      // tiles, if every pair chose another expert
     const uint32_t blocks = (a.tokens + 15u) / 16u;
     a.spare = blocks > (uint32_t)MB ? blocks - MB : 0u;
-    a.ring = ring_slots(fixed + MOE_WAVES * a.spare * 1024u, Mf16Geom<F>::SLICE);
+    a.ring = ring_slots(fixed + MOE_WAVES * a.spare * 1024u, MOE_WAVES, Mf16Geom<F>::SLICE);
     const uint32_t lds = MOE_WAVES * (a.spare * 1024u + a.ring * Mf16Geom<F>::SLICE);
     if (fixed + lds > ALL_LDS) return hipErrorInvalidConfiguration;
     static std::atomic<uint64_t> raised{0};
@@ -38,21 +38,47 @@ hipError_t launch_up(MoeArgs a, hipStream_t s)
     return hipGetLastError();
 }
 
+// Workgroups of `waves` waves that share the (expert, span) list of moe_down's 16 rows: so many that every CU gets 16 waves.
+uint32_t down_parts(uint32_t dim, uint32_t waves)
+{
+    const uint32_t tiles = dim / 16u, want = 256u * (16u / waves);
+    return tiles >= want ? 1u : (want / tiles < 8u ? want / tiles : 8u);
+}
+
+template <class F, int OUT, int MB, int W>
+hipError_t launch_down_w(MoeArgs a, hipStream_t s, bool& fits)
+{
+    constexpr uint32_t fixed = sizeof(MoeTable) + MOE_MAX_TOKENS * MOE_MAX_TOPK * 4 + 2 * W * MOE_MAX_TOKENS * 4 + 64;
+    const uint32_t blocks = (2u * a.tokens + 15u) / 16u;
+    a.spare = blocks > (uint32_t)MB ? blocks - MB : 0u;
+    const uint32_t sums = W * (a.tokens * 64u + a.spare * 1024u);
+    a.ring = ring_slots(fixed + sums, W, Mf16Geom<F>::SLICE);
+    const uint32_t lds = sums + W * a.ring * Mf16Geom<F>::SLICE;
+    fits = fixed + lds <= ALL_LDS;
+    if (!fits) return hipSuccess;
+    static std::atomic<uint64_t> raised{0};
+    hipError_t e = allow_lds(reinterpret_cast<const void*>(&moe_down<F, OUT, MB, W>), (int)(ALL_LDS - fixed), raised);
+    if (e != hipSuccess) return e;
+    a.parts = down_parts(a.dim, W);
+    hipLaunchKernelGGL((moe_down<F, OUT, MB, W>), dim3(a.dim / 16u, a.parts), dim3(W * 64), lds, s, a);
+    e = hipGetLastError();
+    if (e != hipSuccess || a.parts == 1) return e;
+    const uint32_t quads = a.tokens * a.dim / 4u;
+    hipLaunchKernelGGL((moe_combine<OUT>), dim3((quads + 255u) / 256u), dim3(256), 0, s, a.part, a.y, a.parts, quads);
+    return hipGetLastError();
+}
+
+// One block of columns: 16 waves per workgroup, so that from 4096 rows of y on no second pass over parts is needed (it is 4 us); else 8, for the registers.
 template <class F, int OUT, int MB>
 hipError_t launch_down(MoeArgs a, hipStream_t s)
 {
-    constexpr uint32_t fixed = sizeof(MoeTable) + MOE_MAX_TOKENS * MOE_MAX_TOPK * 4 + 2 * MOE_WAVES * MOE_MAX_TOKENS * 4 + 64;
-    const uint32_t blocks = (2u * a.tokens + 15u) / 16u;
-    a.spare = blocks > (uint32_t)MB ? blocks - MB : 0u;
-    const uint32_t sums = MOE_WAVES * (a.tokens * 64u + a.spare * 1024u);
-    a.ring = ring_slots(fixed + sums, Mf16Geom<F>::SLICE);
-    const uint32_t lds = sums + MOE_WAVES * a.ring * Mf16Geom<F>::SLICE;
-    if (fixed + lds > ALL_LDS) return hipErrorInvalidConfiguration;
-    static std::atomic<uint64_t> raised{0};
-    const hipError_t e = allow_lds(reinterpret_cast<const void*>(&moe_down<F, OUT, MB>), (int)(ALL_LDS - fixed), raised);
-    if (e != hipSuccess) return e;
-    hipLaunchKernelGGL((moe_down<F, OUT, MB>), dim3(a.dim / 16u, a.parts), dim3(MOE_WAVES * 64), lds, s, a);
-    return hipGetLastError();
+    bool fits = false;
+    if constexpr (MB == 1) {
+        const hipError_t e = launch_down_w<F, OUT, 1, 16>(a, s, fits);
+        if (e != hipSuccess || fits) return e;
+    }
+    const hipError_t e = launch_down_w<F, OUT, MB, 8>(a, s, fits);
+    return e != hipSuccess || fits ? e : hipErrorInvalidConfiguration;
 }
 
 struct MoeEntry { int qtype, block_size; moe_fn up[2][3], down[2][3]; };                              // [dtype f16 / bf16][blocks of 16 columns 1 / 2 / 4]
@@ -70,13 +96,6 @@ const MoeEntry* entry(int qtype)
     for (const MoeEntry& e : MOE)
         if (e.qtype == qtype) return &e;
     return nullptr;
-}
-
-// Workgroups that share the (expert, span) list of moe_down's 16 rows: so many that the launch has two for every CU.
-uint32_t down_parts(uint32_t dim)
-{
-    const uint32_t tiles = dim / 16u;
-    return tiles >= 512u ? 1u : (512u / (tiles ? tiles : 1u) < 8u ? 512u / (tiles ? tiles : 1u) : 8u);
 }
 
 // Blocks of 16 columns for `per_token` columns of each token of an expert: room for three standard deviations above the mean of evenly spread choices (more
@@ -112,8 +131,8 @@ extern "C" int ggq_moe_route(const void* x, const void* router, uint32_t tokens,
 
 extern "C" uint64_t ggq_moe_workspace(uint32_t tokens, uint32_t top_k, uint32_t dim, uint32_t ff)
 {
-    const uint64_t hidden = ((uint64_t)tokens * top_k * ff * 4u + 15u) & ~15ull, parts = down_parts(dim);
-    return hidden + (parts > 1 ? parts * tokens * dim * 4u : 0u);
+    const uint64_t hidden = ((uint64_t)tokens * top_k * ff * 4u + 15u) & ~15ull;
+    return dim < 16u ? hidden : hidden + (uint64_t)down_parts(dim, 8) * tokens * dim * 4u;              // 8 waves: the most parts
 }
 
 extern "C" int ggq_moe_experts(const ggq_moe_desc* d, void* hip_stream)
@@ -131,16 +150,9 @@ extern "C" int ggq_moe_experts(const ggq_moe_desc* d, void* hip_stream)
         (reinterpret_cast<uintptr_t>(d->y) & 7u)) return GGQ_ERR_ALIGN;
     MoeArgs a{static_cast<const uint8_t*>(d->x), d->ids, d->weights, static_cast<const uint8_t*>(d->gate), static_cast<const uint8_t*>(d->up),
               static_cast<const uint8_t*>(d->down), static_cast<uint8_t*>(d->y), static_cast<uint8_t*>(d->workspace), nullptr, d->tokens, d->top_k, d->experts, d->dim, d->ff, d->act, 1, 0, 2};
-    a.parts = down_parts(a.dim);
     a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(d->workspace) + (((uint64_t)a.tokens * a.top_k * a.ff * 4u + 15u) & ~15ull));
     hipStream_t s = static_cast<hipStream_t>(hip_stream);
     hipError_t e = up->up[d->dtype][column_blocks(a.tokens, a.top_k, a.experts, 1)](a, s);
     if (e == hipSuccess) e = down->down[d->dtype][column_blocks(a.tokens, a.top_k, a.experts, 2)](a, s);
-    if (e == hipSuccess && a.parts > 1) {
-        const uint32_t quads = a.tokens * a.dim / 4u;
-        if (d->dtype == GGQ_F16) hipLaunchKernelGGL((moe_combine<OUT_F16>), dim3((quads + 255u) / 256u), dim3(256), 0, s, a.part, a.y, a.parts, quads);
-        else hipLaunchKernelGGL((moe_combine<OUT_BF16>), dim3((quads + 255u) / 256u), dim3(256), 0, s, a.part, a.y, a.parts, quads);
-        e = hipGetLastError();
-    }
     return e == hipSuccess ? GGQ_OK : hip_fail(e);
 }

@@ -94,6 +94,7 @@ __global__ __launch_bounds__(MOE_ROUTE_THREADS) void moe_route(const uint8_t* __
     if (mine) {
         const double own = score[t];
         rank = 0;
+#pragma unroll 8
         for (uint32_t e = 0; e < experts; e++) {
             const double o = score[e];
             rank += (o > own || (o == own && e < t) || (own != own && (o == o || e < t))) ? 1u : 0u;
@@ -107,8 +108,13 @@ __global__ __launch_bounds__(MOE_ROUTE_THREADS) void moe_route(const uint8_t* __
     if (rank < top_k) {
         const double top = chosen[0];
         float sum = 0.0f;
-        if (renormalize) for (uint32_t s = 0; s < top_k; s++) sum += __expf((float)(chosen[s] - top));
-        else for (uint32_t e = 0; e < experts; e++) sum += __expf((float)(score[e] - top));
+        if (renormalize) {
+#pragma unroll
+            for (uint32_t s = 0; s < MOE_MAX_TOPK; s++) sum += s < top_k ? __expf((float)(chosen[s] - top)) : 0.0f;
+        } else {
+#pragma unroll 8
+            for (uint32_t e = 0; e < experts; e++) sum += __expf((float)(score[e] - top));
+        }
         weights[(uint64_t)blockIdx.x * top_k + rank] = __expf((float)(score[t] - top)) * __builtin_amdgcn_rcpf(sum);
     }
 }
@@ -435,34 +441,34 @@ __global__ __launch_bounds__(MOE_WAVES * 64) MOE_OCC(MB) void moe_up(const MoeAr
     }
 }
 
-// 16 rows of y for every token; of gridDim.y = `parts` workgroups each takes a part of the (expert, span) list, and each of its waves an equal part of
+// 16 rows of y for every token, W waves; of gridDim.y = `parts` workgroups each takes a part of the (expert, span) list, and each of its waves an equal part of
 // that, one wave after the other.  A wave's columns are (token, part of the hidden vector): column 2 i the value, 2 i + 1 the rest of token i of the expert.
-template <class F, int OUT, int MB>
-__global__ __launch_bounds__(MOE_WAVES * 64) MOE_OCC(MB) void moe_down(const MoeArgs a)
+template <class F, int OUT, int MB, int W>
+__global__ __launch_bounds__(W * 64) MOE_OCC(MB) void moe_down(const MoeArgs a)
 {
     using G = Mf16Geom<F>;
     // y of each wave ([wave][token][16] floats), sums of columns beyond MB blocks ([wave][spare][64] f32x4), the rings
     extern __shared__ __attribute__((aligned(16))) uint8_t dyn[];
     __shared__ MoeTable table;
     __shared__ float shares_all[MOE_MAX_TOKENS * MOE_MAX_TOPK];
-    __shared__ uint32_t slots_[MOE_WAVES][MOE_MAX_TOKENS];
-    __shared__ float shares_[MOE_WAVES][MOE_MAX_TOKENS];
+    __shared__ uint32_t slots_[W][MOE_MAX_TOKENS];
+    __shared__ float shares_[W][MOE_MAX_TOKENS];
     const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const uint32_t lane = threadIdx.x & 63u, r = lane & 15u, c = lane >> 4;
     const uint32_t pairs = a.tokens * a.top_k;
     float* part = reinterpret_cast<float*>(dyn) + (uint64_t)wave * a.tokens * 16u;
-    f32x4* spare = reinterpret_cast<f32x4*>(dyn + (uint64_t)MOE_WAVES * a.tokens * 64u) + (uint64_t)wave * a.spare * 64u;
+    f32x4* spare = reinterpret_cast<f32x4*>(dyn + (uint64_t)W * a.tokens * 64u) + (uint64_t)wave * a.spare * 64u;
     for (uint32_t i = lane; i < a.tokens * 16u; i += 64u) part[i] = 0.0f;
-    for (uint32_t p = threadIdx.x; p < pairs; p += MOE_WAVES * 64) shares_all[p] = a.weights[p];
+    for (uint32_t p = threadIdx.x; p < pairs; p += W * 64) shares_all[p] = a.weights[p];
     moe_table(table, a.ids, pairs, a.experts);
 
     const uint32_t row0 = blockIdx.x * 16u;
     const uint64_t row_bytes = (uint64_t)(a.ff / F::BS) * F::TS, expert_bytes = (uint64_t)a.dim * row_bytes;
     const uint32_t n_spans = (a.ff + MF_SPAN - 1) / MF_SPAN, tail_len = a.ff - (n_spans - 1) * (uint32_t)MF_SPAN;
     const gcptr base = (gcptr)a.down + (uint64_t)row0 * row_bytes;
-    const uint64_t items = (uint64_t)table.n * n_spans, share = blockIdx.y * MOE_WAVES + wave, all = (uint64_t)a.parts * MOE_WAVES;
+    const uint64_t items = (uint64_t)table.n * n_spans, share = blockIdx.y * W + wave, all = (uint64_t)a.parts * W;
     const uint32_t first = (uint32_t)(items * share / all), last = (uint32_t)(items * (share + 1) / all);
-    uint8_t* ring = dyn + MOE_WAVES * (a.tokens * 64u + a.spare * 1024u) + wave * a.ring * (uint32_t)G::SLICE;
+    uint8_t* ring = dyn + W * (a.tokens * 64u + a.spare * 1024u) + wave * a.ring * (uint32_t)G::SLICE;
     uint32_t* slots = slots_[wave];
     float* shares = shares_[wave];
 
@@ -546,10 +552,10 @@ __global__ __launch_bounds__(MOE_WAVES * 64) MOE_OCC(MB) void moe_down(const Moe
         if (span == n_spans || item == last) finish();
     }
     __syncthreads();
-    for (uint32_t i = threadIdx.x; i < a.tokens * 16u; i += MOE_WAVES * 64) {
+    for (uint32_t i = threadIdx.x; i < a.tokens * 16u; i += W * 64) {
         const float* sums = reinterpret_cast<const float*>(dyn);
         float v = sums[i];
-        for (uint32_t w = 1; w < MOE_WAVES; w++) v += sums[(uint64_t)w * a.tokens * 16u + i];
+        for (uint32_t w = 1; w < W; w++) v += sums[(uint64_t)w * a.tokens * 16u + i];
         const uint64_t at = (uint64_t)(i >> 4) * a.dim + row0 + (i & 15u);
         if (a.parts > 1) a.part[(uint64_t)blockIdx.y * a.tokens * a.dim + at] = v;
         else if constexpr (OUT == OUT_F16) reinterpret_cast<_Float16*>(a.y)[at] = (_Float16)v;

@@ -80,5 +80,5 @@ def test_expert_arguments_at_the_c_entry(pkg):
         assert call(**bad) == n.GGQ_ERR_ARG, bad
     for bad in (dict(x=A + 8), dict(gate=A + 8), dict(workspace=A + 8), dict(ids=A + 2), dict(y=A + 4)):
         assert call(**bad) == n.GGQ_ERR_ALIGN, bad
-    assert L.ggq_moe_workspace(64, 16, 1 << 20, 1 << 20) == 64 * 16 * 4 << 20              # one part: the hidden values alone
-    assert L.ggq_moe_workspace(3, 2, 256, 512) > 3 * 2 * 512 * 4
+    assert L.ggq_moe_workspace(64, 16, 1 << 20, 1 << 20) == (64 * 16 * 4 << 20) + (64 * 4 << 20)       # hidden values, and one part of y
+    assert L.ggq_moe_workspace(3, 2, 256, 512) == 3 * 2 * 512 * 4 + 8 * 3 * 256 * 4
