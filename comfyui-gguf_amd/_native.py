@@ -30,8 +30,8 @@ HIPCC_FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-ffp-contract=off"
 
 # packed fp32 instructions stay out of the row, integer-product and expert kernels: some of their forms have returned wrong values on this part
 EXTRA_FLAGS = {f: ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"] for f in ("ggq_rows.hip", "ggq_int8.hip", "ggq_moe.hip")}
-# the one unit that unpacks no weights: its fp32 arithmetic has no operation sequence of the reference to keep
-FMA_ALLOWED = ("ggq_rows.hip",)
+# the units that unpack no weights: their fp32 arithmetic has no operation sequence of the reference to keep
+FMA_ALLOWED = ("ggq_rows.hip", "ggq_int8.hip")
 
 # fused multiply-add mnemonics that must not appear in the dequant kernels
 _FMA_RE = re.compile(r"\b(v_(?:pk_)?(?:fma|fmac)_\w+|v_mad_(?:f16|f32|legacy_f\w+|mix\w*|mixlo\w*|mixhi\w*)\w*)")
@@ -107,7 +107,9 @@ SYMBOLS = {
     "ggq_block_norm": (_int, [ctypes.POINTER(ggq_norm_desc), _vp]),
     "ggq_quantize_rows": (_int, [_vp, _u64, _u32, _vp, _u64, _vp, _int, _vp]),
     "ggq_linear_int8": (_int, [_vp, _u64, _vp, _u32, _vp, _u64, _vp, _u32, _u32, _vp, _vp, _int, _vp]),
-    "ggq_moe_route": (_int, [_vp, _vp, _u32, _u32, _u32, _u32, _int, _vp, _vp, _int, _int, _vp]),
+    "ggq_moe_route": (_int, [_vp, _vp, _u32, _u32, _u32, _u32, _int, _vp, _vp, _int, _int, _vp, _u64, _vp]),
+    "ggq_moe_route_workspace": (_u64, [_u32, _u32]),
+    "ggq_linear_int8_few": (_int, [_vp, _u32, _vp, _u64, _vp, _u32, _u32, _vp, _vp, _int, _vp]),
     "ggq_moe_experts": (_int, [ctypes.POINTER(ggq_moe_desc), _vp]),
     "ggq_moe_workspace": (_u64, [_u32, _u32, _u32, _u32]),
     "ggq_dequant_rows": (_int, [_int, _vp, _u64, _u32, _vp, _u64, _vp, _int, _int, _vp]),

@@ -23,17 +23,18 @@ hipError_t launch_tile(I8Args a, hipStream_t s)
     return hipGetLastError();
 }
 
-template <int DT>
+template <int DT, bool FEW>
 hipError_t launch_rows16(const I8Args& a, hipStream_t s)
 {
-    hipLaunchKernelGGL((linear_i8_rows<DT>), dim3((a.n + 15u) / 16u, (a.m + 15u) / 16u), dim3(I8_ROW_WAVES * 64), 0, s, a);
+    const uint32_t lds = FEW ? a.m * ((a.k + 63u) / 64u * 64u + 16u) : 0u;                  // <= 16384 + 16 x 79 bytes
+    hipLaunchKernelGGL((linear_i8_rows<DT, FEW>), dim3((a.n + 15u) / 16u), dim3(I8_ROW_WAVES * 64), lds, s, a);
     return hipGetLastError();
 }
 
 template <int DT>
 hipError_t launch(const I8Args& a, hipStream_t s)
 {
-    if (a.m <= 16) return launch_rows16<DT>(a, s);
+    if (a.m <= 16) return launch_rows16<DT, false>(a, s);
     // The tile that finishes first: rounds of workgroups over the chip times what a step of 128 k takes, in ns.  Measured at 256 x 4096 x 4096 (a part of
     // the chip), 512 x 10240 x 4096 and 4608 x 10240 x 4096 (all of it, at the clock it holds then): 256 x 256 (128 KiB of LDS: one workgroup per CU) 1330 ...
     // 1450 in one round, 1850 in several; 128 x 128 670 alone on a CU, 1050 for two; 64 x 64 350 alone, 420 for two.
@@ -61,5 +62,18 @@ extern "C" int ggq_linear_int8(const void* xq, uint64_t x_stride, const float* x
                    x_stride, w_stride, m, n, k, 0, 0};
     hipStream_t s = static_cast<hipStream_t>(hip_stream);
     const hipError_t e = dtype == GGQ_F16 ? launch<OUT_F16>(a, s) : (dtype == GGQ_BF16 ? launch<OUT_BF16>(a, s) : launch<OUT_F32>(a, s));
+    return e == hipSuccess ? GGQ_OK : hip_fail(e);
+}
+
+extern "C" int ggq_linear_int8_few(const void* x, uint32_t m, const void* wq, uint64_t w_stride, const float* w_scale, uint32_t n, uint32_t k, const void* bias, void* y,
+                                   int dtype, void* hip_stream)
+{
+    if (dtype < 0 || dtype > 2 || m > 16 || k == 0 || k % 8u != 0 || (uint64_t)m * k > (uint64_t)I8_FEW) return GGQ_ERR_ARG;
+    if (m == 0 || n == 0) return GGQ_OK;
+    if (!x || !wq || !w_scale || !y || w_stride % 16 != 0 || w_stride < ((k + 15u) & ~15u)) return GGQ_ERR_ARG;
+    if (!aligned16(x) || !aligned16(wq) || (reinterpret_cast<uintptr_t>(y) & (dtype == GGQ_F32 ? 3u : 1u))) return GGQ_ERR_ALIGN;
+    const I8Args a{static_cast<const uint8_t*>(x), static_cast<const uint8_t*>(wq), nullptr, w_scale, static_cast<const uint8_t*>(bias), static_cast<uint8_t*>(y), 0, w_stride, m, n, k, 0, 0};
+    hipStream_t s = static_cast<hipStream_t>(hip_stream);
+    const hipError_t e = dtype == GGQ_F16 ? launch_rows16<OUT_F16, true>(a, s) : (dtype == GGQ_BF16 ? launch_rows16<OUT_BF16, true>(a, s) : launch_rows16<OUT_F32, true>(a, s));
     return e == hipSuccess ? GGQ_OK : hip_fail(e);
 }

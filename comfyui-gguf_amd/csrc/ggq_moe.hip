@@ -113,18 +113,32 @@ bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0
 
 }  // namespace
 
+extern "C" uint64_t ggq_moe_route_workspace(uint32_t tokens, uint32_t experts) { return experts > (uint32_t)MOE_ROUTE_WAVES ? (uint64_t)tokens * experts * 8u : 0u; }
+
 extern "C" int ggq_moe_route(const void* x, const void* router, uint32_t tokens, uint32_t dim, uint32_t experts, uint32_t top_k, int renormalize, int32_t* ids,
-                             float* weights, int dtype, int router_dtype, void* hip_stream)
+                             float* weights, int dtype, int router_dtype, void* workspace, uint64_t workspace_bytes, void* hip_stream)
 {
-    if ((dtype != GGQ_F16 && dtype != GGQ_BF16) || (router_dtype != dtype && router_dtype != GGQ_F32) || dim == 0 || dim % 8u != 0 || experts == 0 || experts > (uint32_t)MOE_MAX_EXPERTS || top_k == 0 ||
-        top_k > (uint32_t)MOE_MAX_TOPK || top_k > experts || tokens > 0x7FFFFFFFu / MOE_MAX_TOPK) return GGQ_ERR_ARG;
+    if ((dtype != GGQ_F16 && dtype != GGQ_BF16) || (router_dtype != dtype && router_dtype != GGQ_F32) || dim == 0 || dim % 8u != 0 || experts == 0 ||
+        experts > (uint32_t)MOE_MAX_EXPERTS || top_k == 0 || top_k > (uint32_t)MOE_MAX_TOPK || top_k > experts || tokens > 65535u) return GGQ_ERR_ARG;
     if (tokens == 0) return GGQ_OK;
-    if (!x || !router || !ids || !weights) return GGQ_ERR_ARG;
-    if (!aligned16(x) || !aligned16(router) || !aligned4(ids) || !aligned4(weights)) return GGQ_ERR_ALIGN;
-    typedef void (*route_fn)(const uint8_t*, const uint8_t*, uint32_t, uint32_t, uint32_t, int, int32_t*, float*);
-    static const route_fn ROUTE[2][2] = {{moe_route<OUT_F16, OUT_F16>, moe_route<OUT_F16, OUT_F32>}, {moe_route<OUT_BF16, OUT_BF16>, moe_route<OUT_BF16, OUT_F32>}};
-    hipLaunchKernelGGL(ROUTE[dtype][router_dtype == GGQ_F32 ? 1 : 0], dim3(tokens), dim3(MOE_ROUTE_THREADS), 0, static_cast<hipStream_t>(hip_stream),
-                       static_cast<const uint8_t*>(x), static_cast<const uint8_t*>(router), dim, experts, top_k, renormalize, ids, weights);
+    const uint64_t need = ggq_moe_route_workspace(tokens, experts);
+    if (!x || !router || !ids || !weights || (need && !workspace) || workspace_bytes < need) return GGQ_ERR_ARG;
+    if (!aligned16(x) || !aligned16(router) || !aligned4(ids) || !aligned4(weights) || (reinterpret_cast<uintptr_t>(workspace) & 7u)) return GGQ_ERR_ALIGN;
+    const uint8_t *xb = static_cast<const uint8_t*>(x), *rb = static_cast<const uint8_t*>(router);
+    hipStream_t s = static_cast<hipStream_t>(hip_stream);
+    const int wide = router_dtype == GGQ_F32 ? 1 : 0;
+    if (need == 0) {
+        typedef void (*route_fn)(const uint8_t*, const uint8_t*, uint32_t, uint32_t, uint32_t, int, int32_t*, float*);
+        static const route_fn ROUTE[2][2] = {{moe_route<OUT_F16, OUT_F16>, moe_route<OUT_F16, OUT_F32>}, {moe_route<OUT_BF16, OUT_BF16>, moe_route<OUT_BF16, OUT_F32>}};
+        hipLaunchKernelGGL(ROUTE[dtype][wide], dim3(tokens), dim3(MOE_ROUTE_WAVES * 64), 0, s, xb, rb, dim, experts, top_k, renormalize, ids, weights);
+    } else {
+        typedef void (*scores_fn)(const uint8_t*, const uint8_t*, uint32_t, uint32_t, double*);
+        static const scores_fn SCORES[2][2] = {{moe_scores<OUT_F16, OUT_F16>, moe_scores<OUT_F16, OUT_F32>}, {moe_scores<OUT_BF16, OUT_BF16>, moe_scores<OUT_BF16, OUT_F32>}};
+        hipLaunchKernelGGL(SCORES[dtype][wide], dim3((experts + 3u) / 4u, tokens), dim3(256), 0, s, xb, rb, dim, experts, static_cast<double*>(workspace));
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return hip_fail(e);
+        hipLaunchKernelGGL(moe_pick, dim3(tokens), dim3(MOE_MAX_EXPERTS), 0, s, static_cast<const double*>(workspace), experts, top_k, renormalize, ids, weights);
+    }
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? GGQ_OK : hip_fail(e);
 }

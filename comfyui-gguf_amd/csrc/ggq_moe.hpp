@@ -3,7 +3,7 @@
 // Mathematics, per token x:  l = Wr x;  p = softmax(l);  the top_k largest p (equal ones to the lower index), divided by their sum if asked;
 //     y = sum_s p_s Wd[e_s] (act(Wg[e_s] x) * (Wu[e_s] x)).
 //
-// Kernels: the router (moe_route, a workgroup per token), the gate and up projections with the activation (moe_up), the down projection with the weighted sum
+// Kernels: the router (moe_route, or moe_scores and moe_pick), the gate and up projections with the activation (moe_up), the down projection with the weighted sum
 // over experts (moe_down), and where the output has too few rows for the chip, a sum of its parts (moe_combine).  What bounds them is reading the
 // packed bytes of the chosen experts, each ONCE for all tokens that chose it -- and, as closely, unpacking them (1100 cycles of vector instructions per 16
 // rows x 256 columns of Q4_K for bf16: at the full rate that is 18 us where reading takes 19, for two experts of 2 x 10240 x 4096):
@@ -23,14 +23,12 @@
 #include "ggq_mfma16.hpp"
 #include "ggq_rows.hpp"
 
-#include <type_traits>
-
 namespace ggq {
 
 constexpr int MOE_MAX_TOKENS = 64, MOE_MAX_TOPK = 16, MOE_MAX_EXPERTS = 512;
 constexpr int MOE_WORDS = MOE_MAX_EXPERTS / 32;
 
-// ---- the router: a workgroup per token, four experts per wave at a time
+// ---- the router
 
 // Eight products, four at a time in fp32 (a product of two 16-bit values is exact there), what follows in fp64: which of two close scores is larger decides
 // which experts run.  (All of it in fp64: 17 us for 64 experts x 2048, most of it conversions.)  RT: the router's type, fp32 in GGUF files.
@@ -43,66 +41,50 @@ template <int OUT, int RT> GGQ_DEV double moe_dot8(const float (&u)[8], const ui
     return (double)((s[0] + s[1]) + (s[2] + s[3])) + (double)((s[4] + s[5]) + (s[6] + s[7]));
 }
 
-constexpr int MOE_ROUTE_THREADS = 1024;
-
-template <int OUT, int RT>
-__global__ __launch_bounds__(MOE_ROUTE_THREADS) void moe_route(const uint8_t* __restrict__ x_, const uint8_t* __restrict__ router_, uint32_t dim, uint32_t experts,
-                                                              uint32_t top_k, int renormalize, int32_t* __restrict__ ids, float* __restrict__ weights)
+// the score of one expert, by one wave, in every lane: pieces of 4 x 512 elements on their way at once
+template <int OUT, int RT> GGQ_DEV double moe_score(const uint8_t* x, const uint8_t* w, uint32_t dim)
 {
-    constexpr uint32_t RB = RT == OUT_F32 ? 4 : 2;
-    __shared__ double score[MOE_MAX_EXPERTS];
-    __shared__ double chosen[MOE_MAX_TOPK];
-    const uint32_t t = threadIdx.x, lane = t & 63u, wave = t >> 6;
-    const uint8_t* x = x_ + (uint64_t)blockIdx.x * dim * 2;
-    constexpr uint32_t WAVES = MOE_ROUTE_THREADS / 64;
-    // Q experts e0, e0 + 16, ... of a wave, U pieces of 512 elements of their rows on their way at once; absent experts repeat the last one
-    auto scores = [&](auto q_, auto u_, uint32_t e0) {
-        constexpr uint32_t Q = decltype(q_)::value, U = decltype(u_)::value;
-        double acc[Q] = {};
-        for (uint32_t i0 = lane * 8u; i0 < dim; i0 += 512u * U) {
-            float u[U][8];
+    constexpr uint32_t RB = RT == OUT_F32 ? 4 : 2, U = 4;
+    double acc = 0.0;
+    for (uint32_t i0 = (threadIdx.x & 63u) * 8u; i0 < dim; i0 += 512u * U) {
+        double d[U];
 #pragma unroll
-            for (uint32_t p = 0; p < U; p++) row_load8<OUT>(x + (uint64_t)(i0 + 512u * p < dim ? i0 + 512u * p : 0u) * 2, 0, 8, u[p]);
-#pragma unroll
-            for (uint32_t q = 0; q < Q; q++) {
-                const uint32_t e = e0 + q * WAVES < experts ? e0 + q * WAVES : experts - 1u;
-                double d[U];
-#pragma unroll
-                for (uint32_t p = 0; p < U; p++) d[p] = moe_dot8<OUT, RT>(u[p], router_ + ((uint64_t)e * dim + (i0 + 512u * p < dim ? i0 + 512u * p : 0u)) * RB);
-#pragma unroll
-                for (uint32_t p = 0; p < U; p++) acc[q] += i0 + 512u * p < dim ? d[p] : 0.0;
-            }
+        for (uint32_t p = 0; p < U; p++) {
+            const uint32_t i = i0 + 512u * p < dim ? i0 + 512u * p : 0u;
+            float u[8];
+            row_load8<OUT>(x + (uint64_t)i * 2, 0, 8, u);
+            d[p] = moe_dot8<OUT, RT>(u, w + (uint64_t)i * RB);
         }
 #pragma unroll
-        for (int off = 32; off > 0; off >>= 1)
+        for (uint32_t p = 0; p < U; p++) acc += i0 + 512u * p < dim ? d[p] : 0.0;
+    }
 #pragma unroll
-            for (uint32_t q = 0; q < Q; q++) acc[q] += __shfl_xor(acc[q], off, 64);
-        if (lane == 0)
-#pragma unroll
-            for (uint32_t q = 0; q < Q; q++)
-                if (e0 + q * WAVES < experts) score[e0 + q * WAVES] = acc[q];
-    };
-    if (experts <= WAVES) {
-        if (wave < experts) scores(std::integral_constant<uint32_t, 1>{}, std::integral_constant<uint32_t, 4>{}, wave);
-    } else {
-        for (uint32_t e0 = wave; e0 < experts; e0 += 4 * WAVES) scores(std::integral_constant<uint32_t, 4>{}, std::integral_constant<uint32_t, 2>{}, e0);
+    for (int off = 32; off > 0; off >>= 1) acc += __shfl_xor(acc, off, 64);
+    return acc;
+}
+
+// The top_k experts of one token and their weights, from the scores in LDS; by the whole workgroup, which has a thread for every expert.  rank_[e] = how many
+// experts come before e; a NaN comes last (its weight is NaN all the same).  The comparisons of an expert are split over the threads there are.
+GGQ_DEV void moe_choose(const double* score, uint32_t* rank_, double* chosen, uint32_t experts, uint32_t top_k, int renormalize, int32_t* ids, float* weights)
+{
+    const uint32_t padded = (experts + 63u) & ~63u, parts = blockDim.x / padded, t = threadIdx.x % padded, part = threadIdx.x / padded;
+    if (threadIdx.x < experts) rank_[threadIdx.x] = 0;
+    __syncthreads();
+    if (t < experts && part < parts) {
+        const double own = score[t];
+        uint32_t before = 0;
+#pragma unroll 4
+        for (uint32_t e = part; e < experts; e += parts) {
+            const double o = score[e];
+            before += (o > own || (o == own && e < t) || (own != own && (o == o || e < t))) ? 1u : 0u;
+        }
+        atomicAdd(&rank_[t], before);
     }
     __syncthreads();
-    // rank of an expert = how many come before it; a NaN comes last (its weight is NaN all the same)
-    const bool mine = t < experts;
-    uint32_t rank = ~0u;
-    if (mine) {
-        const double own = score[t];
-        rank = 0;
-#pragma unroll 8
-        for (uint32_t e = 0; e < experts; e++) {
-            const double o = score[e];
-            rank += (o > own || (o == own && e < t) || (own != own && (o == o || e < t))) ? 1u : 0u;
-        }
-        if (rank < top_k) {
-            chosen[rank] = own;
-            ids[(uint64_t)blockIdx.x * top_k + rank] = (int32_t)t;
-        }
+    const uint32_t rank = threadIdx.x < experts ? rank_[threadIdx.x] : ~0u;
+    if (rank < top_k) {
+        chosen[rank] = score[threadIdx.x];
+        ids[rank] = (int32_t)threadIdx.x;
     }
     __syncthreads();
     if (rank < top_k) {
@@ -115,8 +97,48 @@ __global__ __launch_bounds__(MOE_ROUTE_THREADS) void moe_route(const uint8_t* __
 #pragma unroll 8
             for (uint32_t e = 0; e < experts; e++) sum += __expf((float)(score[e] - top));
         }
-        weights[(uint64_t)blockIdx.x * top_k + rank] = __expf((float)(score[t] - top)) * __builtin_amdgcn_rcpf(sum);
+        weights[rank] = __expf((float)(score[threadIdx.x] - top)) * __builtin_amdgcn_rcpf(sum);
     }
+}
+
+// up to 16 experts: one workgroup per token, one wave per expert
+constexpr int MOE_ROUTE_WAVES = 16;
+template <int OUT, int RT>
+__global__ __launch_bounds__(MOE_ROUTE_WAVES * 64) void moe_route(const uint8_t* __restrict__ x, const uint8_t* __restrict__ router, uint32_t dim, uint32_t experts,
+                                                                 uint32_t top_k, int renormalize, int32_t* __restrict__ ids, float* __restrict__ weights)
+{
+    __shared__ double score[MOE_ROUTE_WAVES];
+    __shared__ uint32_t rank[MOE_ROUTE_WAVES];
+    __shared__ double chosen[MOE_MAX_TOPK];
+    const uint32_t wave = threadIdx.x >> 6;
+    if (wave < experts) {
+        const double v = moe_score<OUT, RT>(x + (uint64_t)blockIdx.x * dim * 2, router + (uint64_t)wave * dim * (RT == OUT_F32 ? 4 : 2), dim);
+        if ((threadIdx.x & 63u) == 0) score[wave] = v;
+    }
+    __syncthreads();
+    moe_choose(score, rank, chosen, experts, top_k, renormalize, ids + (uint64_t)blockIdx.x * top_k, weights + (uint64_t)blockIdx.x * top_k);
+}
+
+// more experts: a wave per (expert, token) for the scores, then a workgroup per token for the choice.  (64 experts x 2048, 7 tokens: 18 us with one workgroup per
+// token for both, most of it one CU's latency.)
+template <int OUT, int RT>
+__global__ __launch_bounds__(256) void moe_scores(const uint8_t* __restrict__ x, const uint8_t* __restrict__ router, uint32_t dim, uint32_t experts, double* __restrict__ scores)
+{
+    const uint32_t e = blockIdx.x * 4u + (threadIdx.x >> 6), t = blockIdx.y;
+    if (e >= experts) return;
+    const double v = moe_score<OUT, RT>(x + (uint64_t)t * dim * 2, router + (uint64_t)e * dim * (RT == OUT_F32 ? 4 : 2), dim);
+    if ((threadIdx.x & 63u) == 0) scores[(uint64_t)t * experts + e] = v;
+}
+
+__global__ __launch_bounds__(MOE_MAX_EXPERTS) void moe_pick(const double* __restrict__ scores, uint32_t experts, uint32_t top_k, int renormalize, int32_t* __restrict__ ids,
+                                                           float* __restrict__ weights)
+{
+    __shared__ double score[MOE_MAX_EXPERTS];
+    __shared__ uint32_t rank[MOE_MAX_EXPERTS];
+    __shared__ double chosen[MOE_MAX_TOPK];
+    if (threadIdx.x < experts) score[threadIdx.x] = scores[(uint64_t)blockIdx.x * experts + threadIdx.x];
+    __syncthreads();
+    moe_choose(score, rank, chosen, experts, top_k, renormalize, ids + (uint64_t)blockIdx.x * top_k, weights + (uint64_t)blockIdx.x * top_k);
 }
 
 // ---- which experts were chosen, and by whom

@@ -15,13 +15,14 @@ from .dequant import GGQUnsupported, _OUT_CODE, _cur_device, _is_compiling, _raw
 from .norms import MAX_DIM, _on_gpu, _plain, _refuse_grad
 
 MAX_K = 131071                     # |sum| <= 128 * 128 * k stays below 2^31
-_quantize_call = _linear_call = None
+FEW = 16384                        # elements of x up to which (and 16 rows) one launch does both: the kernels' I8_FEW
+_quantize_call = _linear_call = _few_call = None
 
 
 def _bind():
-    global _quantize_call, _linear_call
+    global _quantize_call, _linear_call, _few_call
     L = _native.lib()
-    _quantize_call, _linear_call = L.ggq_quantize_rows, L.ggq_linear_int8
+    _quantize_call, _linear_call, _few_call = L.ggq_quantize_rows, L.ggq_linear_int8, L.ggq_linear_int8_few
 
 
 def _launch(call, name, device, *args):
@@ -131,6 +132,12 @@ def _linear_int8(x, weight, weight_scale, bias, x_scale, out_dtype):
     x = _plain(x)
     if x.dtype is torch.int8:
         xq, x_scale = _rows8(x.reshape(m, k) if x.dim() != 2 else x, "x", True), x_scale.reshape(m).contiguous()
+    elif m <= 16 and m * k <= FEW and k % 8 == 0 and out_dtype is x.dtype:
+        if not x.is_contiguous() or x.data_ptr() & 15:
+            x = x.contiguous().clone()
+        _launch(_few_call, "ggq_linear_int8_few", device, x.data_ptr(), m, weight.data_ptr(), weight.stride(0), weight_scale.data_ptr(), n, k,
+                None if bias is None else bias.data_ptr(), y.data_ptr(), _OUT_CODE[out_dtype])
+        return y
     else:
         xq, x_scale = _quantize(x.reshape(m, k))
     _launch(_linear_call, "ggq_linear_int8", device, xq.data_ptr(), xq.stride(0), x_scale.data_ptr(), m, weight.data_ptr(), weight.stride(0), weight_scale.data_ptr(), n, k,

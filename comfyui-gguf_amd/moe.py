@@ -58,15 +58,17 @@ def _route(x, router, top_k, renormalize):
     experts = router.shape[0]
     if router.shape[1] != dim or router.dtype not in (x.dtype, torch.float32) or router.device != x.device:
         raise GGQUnsupported(f"moe.route: a router (experts x {dim}) of {x.dtype} or fp32 on {x.device}")
-    if dim % 8 or dim == 0 or not 1 <= experts <= MAX_EXPERTS or not 1 <= top_k <= min(MAX_TOP_K, experts):
-        raise GGQUnsupported(f"moe.route: rows of a multiple of 8 elements, 1 ... {MAX_EXPERTS} experts, 1 ... {MAX_TOP_K} of them per token")
+    if dim % 8 or dim == 0 or not 1 <= experts <= MAX_EXPERTS or not 1 <= top_k <= min(MAX_TOP_K, experts) or tokens > 65535:
+        raise GGQUnsupported(f"moe.route: at most 65535 rows of a multiple of 8 elements, 1 ... {MAX_EXPERTS} experts, 1 ... {MAX_TOP_K} of them per token")
     ids = torch.empty((tokens, top_k), dtype=torch.int32, device=x.device)
     weights = torch.empty((tokens, top_k), dtype=torch.float32, device=x.device)
     if tokens:
         if _route_call is None:
             _bind()
+        size = tokens * experts * 8 if experts > 16 else 0           # ggq_moe_route_workspace()
+        scratch = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
         _with_device(x.device, _route_call, "ggq_moe_route", x.data_ptr(), router.data_ptr(), tokens, dim, experts, top_k, int(bool(renormalize)), ids.data_ptr(),
-                     weights.data_ptr(), _OUT_CODE[x.dtype], _OUT_CODE[router.dtype])
+                     weights.data_ptr(), _OUT_CODE[x.dtype], _OUT_CODE[router.dtype], scratch.data_ptr() if size else None, size)
     return ids, weights
 
 

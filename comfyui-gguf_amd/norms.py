@@ -63,11 +63,14 @@ def _per_sample(v, lead, dim, dtype, device, what):
     """A modulation vector per sample as (2-D tensor, stride between vectors, vectors, is fp32).  v's leading dimensions are the stream's, or the
     first of them followed by ones."""
     v = _plain(v)
-    if v.device != device or v.dim() == 0 or v.shape[-1] != dim:
-        raise GGQUnsupported(f"block_norm: {what} of shape {tuple(v.shape)} on {v.device} for rows of {dim} on {device}")
+    shape = v.shape
+    if v.device != device or not shape or shape[-1] != dim:
+        raise GGQUnsupported(f"block_norm: {what} of shape {tuple(shape)} on {v.device} for rows of {dim} on {device}")
     if v.dtype is not dtype and v.dtype is not torch.float32:
         v = v.float()
-    own = list(v.shape[:-1])
+    if len(lead) == 2 and len(shape) == 3 and shape[1] == 1 and shape[0] == lead[0] and v.stride(2) == 1:          # the usual (batch, 1, dim): no view to make
+        return v, v.stride(0) if shape[0] > 1 else 0, shape[0], v.dtype is torch.float32
+    own = list(shape[:-1])
     while own and own[-1] == 1:
         own.pop()
     if own != list(lead[:len(own)]):

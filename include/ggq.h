@@ -254,14 +254,21 @@ int ggq_quantize_rows(const void* x, uint64_t rows, uint32_t cols, void* q, uint
 int ggq_linear_int8(const void* xq, uint64_t x_stride, const float* x_scale, uint32_t m, const void* wq, uint64_t w_stride, const float* w_scale, uint32_t n,
                     uint32_t k, const void* bias, void* y, int dtype, void* hip_stream);
 
+/* The same for a few rows of x as they are: m <= 16 rows of `dtype`, m * k <= 16384 (GGQ_ERR_ARG above), contiguous, 16-byte aligned, k % 8 == 0; they are put into
+ * 8 bits on the way, as ggq_quantize_rows does, and the result is that of the two calls. */
+int ggq_linear_int8_few(const void* x, uint32_t m, const void* wq, uint64_t w_stride, const float* w_scale, uint32_t n, uint32_t k, const void* bias, void* y,
+                        int dtype, void* hip_stream);
+
 /* ---- mixture of experts for a few tokens ---------------------------------------------------------------------------------------------- */
 
 /* The experts of each token: p = softmax(x Wr^T) over `experts` (<= 512), the top_k (<= 16, <= experts) largest in descending order, equal ones to the
  * lower index.  x: tokens x dim, router: experts x dim, of `dtype`
  * (GGQ_F16 / GGQ_BF16) and router_dtype (`dtype` or GGQ_F32), contiguous, 16-byte aligned, dim % 8 == 0.  ids: int32
- * tokens x top_k; weights: fp32, p of the chosen ones, divided by their sum if `renormalize`. */
+ * tokens x top_k; weights: fp32, p of the chosen ones, divided by their sum if `renormalize`.  At
+ * most 65535 tokens.  Scores are fp64; a NaN score comes last.  workspace: ggq_moe_route_workspace() bytes (0 for up to 16 experts), 8-byte aligned. */
 int ggq_moe_route(const void* x, const void* router, uint32_t tokens, uint32_t dim, uint32_t experts, uint32_t top_k, int renormalize, int32_t* ids,
-                  float* weights, int dtype, int router_dtype, void* hip_stream);
+                  float* weights, int dtype, int router_dtype, void* workspace, uint64_t workspace_bytes, void* hip_stream);
+uint64_t ggq_moe_route_workspace(uint32_t tokens, uint32_t experts);
 
 /* y[t] = sum_s weights[t, s] * Wd[e] (act(Wg[e] x[t]) * (Wu[e] x[t])), e = ids[t, s], straight from packed expert weights: gate and up are packed stacks of
  * logical shape (experts, ff, dim) in one format, down (experts, dim, ff) in its own; W = the fp16 values of the packed blocks in `dtype`, as

@@ -59,13 +59,24 @@ def test_quantize_and_product_arguments_at_the_c_entry(pkg):
         assert rc == n.GGQ_ERR_ALIGN
 
 
+def test_few_rows_arguments_at_the_c_entry(pkg):
+    n, L = pkg._native, _lib(pkg)
+    p = lambda x=A, m=2, w=A, ws=64, sw=A, rows=4, k=64, b=None, y=A, dt=n.F16: L.ggq_linear_int8_few(x, m, w, ws, sw, rows, k, b, y, dt, None)  # noqa: E731
+    assert p(m=0) == n.GGQ_OK and p(rows=0) == n.GGQ_OK
+    for rc in (p(x=None), p(w=None), p(sw=None), p(y=None), p(m=17), p(k=0), p(k=60), p(m=2, k=8200, ws=8208), p(ws=48), p(ws=72), p(dt=3)):
+        assert rc == n.GGQ_ERR_ARG
+    for rc in (p(x=A + 8), p(w=A + 8), p(y=A + 1)):
+        assert rc == n.GGQ_ERR_ALIGN
+
+
 def test_expert_arguments_at_the_c_entry(pkg):
     n, L = pkg._native, _lib(pkg)
-    r = lambda x=A, w=A, t=4, d=64, e=8, k=2, ids=A, out=A, dt=n.F16, rt=n.F16: L.ggq_moe_route(x, w, t, d, e, k, 1, ids, out, dt, rt, None)  # noqa: E731
+    r = lambda x=A, w=A, t=4, d=64, e=8, k=2, ids=A, out=A, dt=n.F16, rt=n.F16, ws=A, size=1 << 20: L.ggq_moe_route(x, w, t, d, e, k, 1, ids, out, dt, rt, ws, size, None)  # noqa: E731
     assert r(t=0) == n.GGQ_OK
-    for rc in (r(x=None), r(w=None), r(ids=None), r(out=None), r(d=0), r(d=60), r(e=0), r(e=513, k=2), r(k=0), r(k=9), r(k=17, e=64), r(dt=n.F32), r(rt=n.BF16)):
+    for rc in (r(x=None), r(w=None), r(ids=None), r(out=None), r(d=0), r(d=60), r(e=0), r(e=513, k=2), r(k=0), r(k=9), r(k=17, e=64), r(dt=n.F32), r(rt=n.BF16), r(t=65536), r(e=17, ws=None), r(e=17, size=4 * 17 * 8 - 1)):
         assert rc == n.GGQ_ERR_ARG
-    assert r(x=A + 2) == n.GGQ_ERR_ALIGN and r(ids=A + 2) == n.GGQ_ERR_ALIGN
+    assert r(x=A + 2) == n.GGQ_ERR_ALIGN and r(ids=A + 2) == n.GGQ_ERR_ALIGN and r(e=17, ws=A + 4) == n.GGQ_ERR_ALIGN
+    assert L.ggq_moe_route_workspace(4, 16) == 0 and L.ggq_moe_route_workspace(4, 17) == 4 * 17 * 8
 
     def call(**kw):
         base = dict(x=A, ids=A, weights=A, gate=A, up=A, down=A, y=A, workspace=A, workspace_bytes=1 << 30, tokens=4, top_k=2, experts=8, dim=256, ff=512, up_qtype=12, down_qtype=14,

@@ -68,6 +68,8 @@ def test_quantization_of_fp32_rows_and_rows_without_a_form(pkg):
     x[1, 5], x[2, 6], x[3] = float("nan"), float("-inf"), 0.0
     q, scale = pkg.int8.quantize_rows(x)
     assert bool(scale[1:3].isnan().all()) and float(scale[3]) == 0 and not bool(q[1:4].any())
+    y = pkg.int8.linear_int8(x[:4, :776], q[:50, :776], torch.ones(50, device=DEV))          # few rows: quantized in the product itself
+    assert bool(y[1:3].isnan().all()) and not bool(y[3].any()) and bool(y[0].isfinite().all())
     y = pkg.int8.linear_int8(x, q[:50], torch.ones(50, device=DEV))
     assert bool(y[1:3].isnan().all()) and not bool(y[3].any()) and bool(y[0].isfinite().all())
 
@@ -87,7 +89,7 @@ def _check(y, q, sx, w, sw, bias, dtype):
 
 
 SIZES = [(1, 1, 1), (1, 17, 64), (3, 100, 1001), (16, 48, 4096), (17, 33, 129), (64, 65, 127), (65, 130, 2432), (128, 128, 128), (129, 257, 384), (333, 1501, 1001), (300, 70, 16),
-         (1, 10240, 4096), (2, 5, 20000), (1100, 1030, 640), (4100, 4099, 160), (31, 16384, 48), (700, 5000, 200)]
+         (1, 10240, 4096), (2, 5, 20000), (1100, 1030, 640), (4100, 4099, 160), (31, 16384, 48), (700, 5000, 200), (1, 100, 16384), (2, 33, 8192), (16, 40, 1024), (5, 20, 8), (4, 64, 4104), (13, 50, 72)]
 
 
 @pytest.mark.parametrize("kind", ["f16", "bf16", "f32"])
