@@ -26,10 +26,9 @@ ABI_VERSION = 11
 
 # -ffp-contract=off is REQUIRED for parity: hipcc otherwise fuses the reference's separately
 # rounded fp16 multiply and subtract into v_pk_fma_f16 (SURVEY.md section 0 finding 3).
-HIPCC_FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-ffp-contract=off", "-fPIC", "-shared"]
+# Packed fp32 instructions (v_pk_add_f32 and the like) stay out of all device code: some of their forms have returned wrong values on this part.
+HIPCC_FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-ffp-contract=off", "-fPIC", "-shared", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
-# packed fp32 instructions stay out of the row, integer-product and expert kernels: some of their forms have returned wrong values on this part
-EXTRA_FLAGS = {f: ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"] for f in ("ggq_rows.hip", "ggq_int8.hip", "ggq_moe.hip")}
 # the units that unpack no weights: their fp32 arithmetic has no operation sequence of the reference to keep
 FMA_ALLOWED = ("ggq_rows.hip", "ggq_int8.hip")
 
@@ -171,6 +170,15 @@ _SPILL_RE = re.compile(r"\.name:\s+(\S+)\n(?:.*\n)*?\s+\.private_segment_fixed_s
 MAX_SCRATCH_BYTES = 16
 
 
+_PACKED_F32_RE = re.compile(r"\bv_pk_(?:add|mul|fma)_f32\b")
+
+
+def check_no_packed_f32(asm_text):
+    """Raise if a packed fp32 instruction made it into the device code (HIPCC_FLAGS keeps the compiler from making them)."""
+    if _PACKED_F32_RE.search(asm_text):
+        raise GGQNativeError("packed fp32 instructions in the device code: build with -Xclang -target-feature -Xclang -packed-fp32-ops")
+
+
 def check_no_spills(asm_text, limit=MAX_SCRATCH_BYTES):
     """Raise if a kernel keeps more than ``limit`` bytes per lane in scratch memory (build-time guard, round 6): a register spill is a vector-memory access in front of the
     in-order weight stream -- the 16-row fused kernel ran Q8_0 at half speed for most of round 6 with 72-108 bytes of it and nothing said so (EXPERIMENTS.md R6-9)."""
@@ -196,7 +204,7 @@ def build(force=False, verbose=False):
             stem = os.path.splitext(os.path.basename(src))[0]
             d = os.path.join(tmp, stem)
             os.makedirs(d)
-            cmd = [hipcc_path()] + compile_flags + EXTRA_FLAGS.get(os.path.basename(src), []) + [f'-DGGQ_BUILD_ID="{source_id()}"', "-save-temps=obj", "-c", "-o", os.path.join(d, stem + ".o"), src]
+            cmd = [hipcc_path()] + compile_flags + [f'-DGGQ_BUILD_ID="{source_id()}"', "-save-temps=obj", "-c", "-o", os.path.join(d, stem + ".o"), src]
             jobs.append((cmd, d, subprocess.Popen(cmd, cwd=d, stdout=subprocess.PIPE, stderr=subprocess.PIPE, text=True)))
         failed = None
         for cmd, d, proc in jobs:
@@ -217,7 +225,8 @@ def build(force=False, verbose=False):
             if not os.path.basename(f).startswith(tuple(os.path.splitext(u)[0] + "-" for u in FMA_ALLOWED)):
                 check_no_fma(text)
             check_no_spills(text)
-        link = [hipcc_path()] + HIPCC_FLAGS + ["-o", out] + [os.path.join(d, os.path.basename(d) + ".o") for _, d, _ in jobs]
+            check_no_packed_f32(text)
+        link = [hipcc_path(), "--offload-arch=gfx950", "-O3", "-fPIC", "-shared", "-o", out] + [os.path.join(d, os.path.basename(d) + ".o") for _, d, _ in jobs]
         proc = subprocess.run(link, cwd=tmp, capture_output=True, text=True)
         if verbose or proc.returncode:
             print(" ".join(link))
