@@ -443,7 +443,7 @@ def reference_gpu_leg(pkg, plan, qtypes, device):
             "parity_vs_hip_path": "bit-exact" if parity else "MISMATCH"}
 
 
-def cpu_baseline_port(pkg, plan, qtype, budget_s):
+def cpu_baseline_port(pkg, plan, qtypes, budget_s):
     """kind 'port': the oracle's throughput leg (oracle/ggq_oracle_simd.c: the same op sequence with AVX2+F16C and OpenMP) on the
     first tensors of the pool -- the fastest CPU implementation of this path the repo has, reported BESIDE the reference's own
     torch-CPU figure so that the GPU/CPU ratio is not flattered by a slow baseline; hosts without AVX2/F16C time the soft-float
@@ -455,16 +455,16 @@ def cpu_baseline_port(pkg, plan, qtype, budget_s):
     outs = [np.empty(plan.outputs[i].numel(), dtype=np.uint16) for i in range(n_sample)]
     max_threads = int(oracle.lib().ggq_oracle_max_threads())
     simd = oracle.simd_available()
-    want = oracle.dequant_f16(qtype, packed[0])                # soft-float checker: parity of the GPU and of the timed leg
+    want = oracle.dequant_f16(qtypes[0], packed[0])            # soft-float checker: parity of the GPU and of the timed leg
     got = plan.outputs[0].cpu().numpy().reshape(-1)
     parity = bool(np.array_equal(got.view(np.uint16), want.view(np.uint16)))
     if simd:
-        parity = parity and bool(np.array_equal(oracle.dequant_f16(qtype, packed[0], simd=True).view(np.uint16), want.view(np.uint16)))
-    nbytes = sum(pkg.qtypes.algorithmic_bytes(qtype, o.size) for o in outs)
+        parity = parity and bool(np.array_equal(oracle.dequant_f16(qtypes[0], packed[0], simd=True).view(np.uint16), want.view(np.uint16)))
+    nbytes = sum(pkg.qtypes.algorithmic_bytes(q, o.size) for q, o in zip(qtypes, outs))
 
     def one_pass(c):
-        for p, o in zip(packed, outs):
-            oracle.dequant_f16(qtype, p, threads=c, simd=simd, out=o)
+        for q, p, o in zip(qtypes, packed, outs):
+            oracle.dequant_f16(q, p, threads=c, simd=simd, out=o)
 
     # OpenMP on every hardware thread of a shared box is not always the fastest setting: try a few team
     # sizes, report the best median and ITS thread count.
@@ -477,7 +477,7 @@ def cpu_baseline_port(pkg, plan, qtype, budget_s):
     med, threads, reps, tmin = best
     leg = "oracle/ggq_oracle_simd.c (AVX2+F16C)" if simd else "oracle/ggq_oracle.c (soft-float; host lacks AVX2/F16C)"
     return {"value": round(nbytes / med / 1e9, 3), "unit": "GB/s", "cores": threads, "threads": threads, "host_cpus": os.cpu_count(), "kind": "port",
-            "sample": (f"{qtype.name}: first {n_sample} pool tensors ({sum(o.size for o in outs)} elements, same packed bytes), "
+            "sample": (f"{' + '.join(sorted({q.name for q in qtypes[:n_sample]}))}: first {n_sample} pool tensors ({sum(o.size for o in outs)} elements, same packed bytes), "
                        f"{reps} passes of {leg} with OpenMP on {threads} threads (best of team sizes {counts}; "
                        f"{os.cpu_count()} host CPUs visible), median; fastest pass {nbytes / tmin / 1e9:.3f} GB/s"),
             "parity_vs_gpu": "bit-exact" if parity else "MISMATCH"}
@@ -523,11 +523,8 @@ def cpu_baselines(pkg, plan, qtypes, budget_s, W):
         W.wait_host()                                           # sleep on the control group while rank 0 times the CPU legs
         return None, None
     ref = cpu_baseline_reference(pkg, plan, qtypes, budget_s * 0.5)
-    port = cpu_baseline_port(pkg, plan, qtypes[0], budget_s * 0.5) if len(set(qtypes[:8])) == 1 else None
+    port = cpu_baseline_port(pkg, plan, qtypes, budget_s * 0.5) if ref is None or len(set(qtypes[:8])) == 1 else None
     head = ref if ref is not None else port
-    if head is None:                                            # mixed-format set without the reference's sources: parity only
-        head = {"value": None, "unit": "GB/s", "cores": 0, "kind": "port", "sample": "no CPU leg (mixed formats, reference sources absent): parity only"}
-        ref = head
     head["parity_vs_gpu"] = parity_statement(rows, head.get("parity_vs_gpu"), with_reference=head.get("kind") == "reference")
     head["parity_check_s"] = max(r["seconds"] for r in rows)
     head["parity_by_rank"] = [{k: r[k] for k in ("rank", "tensors", "differ", "seconds")} for r in rows]
