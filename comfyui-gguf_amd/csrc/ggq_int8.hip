@@ -18,7 +18,6 @@ hipError_t launch_tile(I8Args a, hipStream_t s)
     if (e != hipSuccess) return e;
     a.tiles_m = (a.m + TM - 1) / TM;
     a.tiles_n = (a.n + TN - 1) / TN;
-    if ((uint64_t)a.tiles_m * a.tiles_n > 0x7FFFFFFFull) return hipErrorInvalidValue;
     hipLaunchKernelGGL((linear_i8_tile<DT, TM, TN, WM, WN, KS, NB>), dim3(a.tiles_m * a.tiles_n), dim3(WM * WN * KS * 64), lds, s, a);
     return hipGetLastError();
 }
@@ -47,6 +46,7 @@ hipError_t launch(const I8Args& a, hipStream_t s)
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+bool unaligned(const void* p, int dtype) { return (reinterpret_cast<uintptr_t>(p) & (dtype == GGQ_F32 ? 3u : 1u)) != 0; }
 
 }  // namespace
 
@@ -55,9 +55,10 @@ extern "C" int ggq_linear_int8(const void* xq, uint64_t x_stride, const float* x
 {
     if (dtype < 0 || dtype > 2 || k == 0 || k > MAX_K) return GGQ_ERR_ARG;
     if (m == 0 || n == 0) return GGQ_OK;
+    if (((uint64_t)m + 63) / 64 * (((uint64_t)n + 63) / 64) > 0x7FFFFFFFull) return GGQ_ERR_ARG;      // workgroups of the smallest tile
     const uint64_t k16 = (k + 15u) & ~15u;
     if (!xq || !x_scale || !wq || !w_scale || !y || x_stride % 16 != 0 || w_stride % 16 != 0 || x_stride < k16 || w_stride < k16) return GGQ_ERR_ARG;
-    if (!aligned16(xq) || !aligned16(wq) || (reinterpret_cast<uintptr_t>(y) & (dtype == GGQ_F32 ? 3u : 1u))) return GGQ_ERR_ALIGN;
+    if (!aligned16(xq) || !aligned16(wq) || unaligned(y, dtype) || unaligned(bias, dtype) || unaligned(x_scale, GGQ_F32) || unaligned(w_scale, GGQ_F32)) return GGQ_ERR_ALIGN;
     const I8Args a{static_cast<const uint8_t*>(xq), static_cast<const uint8_t*>(wq), x_scale, w_scale, static_cast<const uint8_t*>(bias), static_cast<uint8_t*>(y),
                    x_stride, w_stride, m, n, k, 0, 0};
     hipStream_t s = static_cast<hipStream_t>(hip_stream);
@@ -71,7 +72,7 @@ extern "C" int ggq_linear_int8_few(const void* x, uint32_t m, const void* wq, ui
     if (dtype < 0 || dtype > 2 || m > 16 || k == 0 || k % 8u != 0 || (uint64_t)m * k > (uint64_t)I8_FEW) return GGQ_ERR_ARG;
     if (m == 0 || n == 0) return GGQ_OK;
     if (!x || !wq || !w_scale || !y || w_stride % 16 != 0 || w_stride < ((k + 15u) & ~15u)) return GGQ_ERR_ARG;
-    if (!aligned16(x) || !aligned16(wq) || (reinterpret_cast<uintptr_t>(y) & (dtype == GGQ_F32 ? 3u : 1u))) return GGQ_ERR_ALIGN;
+    if (!aligned16(x) || !aligned16(wq) || unaligned(y, dtype) || unaligned(bias, dtype) || unaligned(w_scale, GGQ_F32)) return GGQ_ERR_ALIGN;
     const I8Args a{static_cast<const uint8_t*>(x), static_cast<const uint8_t*>(wq), nullptr, w_scale, static_cast<const uint8_t*>(bias), static_cast<uint8_t*>(y), 0, w_stride, m, n, k, 0, 0};
     hipStream_t s = static_cast<hipStream_t>(hip_stream);
     const hipError_t e = dtype == GGQ_F16 ? launch_rows16<OUT_F16, true>(a, s) : (dtype == GGQ_BF16 ? launch_rows16<OUT_BF16, true>(a, s) : launch_rows16<OUT_F32, true>(a, s));

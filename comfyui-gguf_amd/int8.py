@@ -11,7 +11,7 @@ result.  ``ops.GGMLInt8Linear`` is the layer.
 import torch
 
 from . import _native
-from .dequant import GGQUnsupported, _OUT_CODE, _cur_device, _is_compiling, _raw_stream
+from .dequant import GGQUnsupported, _DEVICE_OK, _OUT_CODE, _cur_device, _device_served, _is_compiling, _raw_stream
 from .norms import MAX_DIM, _on_gpu, _plain, _refuse_grad
 
 MAX_K = 131071                     # |sum| <= 128 * 128 * k stays below 2^31
@@ -95,7 +95,9 @@ def _linear_int8(x, weight, weight_scale, bias, x_scale, out_dtype):
     device = weight.device
     if not 1 <= k <= MAX_K:
         raise GGQUnsupported(f"linear_int8: 1 ... {MAX_K} columns")
-    if weight_scale.dtype is not torch.float32 or weight_scale.numel() != n or weight_scale.device != device:
+    if not (_DEVICE_OK.get(device.index) or _device_served(device.index)):
+        raise GGQUnsupported(f"{device} is not a gfx950 device")
+    if not isinstance(weight_scale, torch.Tensor) or weight_scale.dtype is not torch.float32 or weight_scale.numel() != n or weight_scale.device != device:
         raise GGQUnsupported(f"linear_int8: weight_scale is {n} fp32 values on {device}")
     if x.dtype is torch.int8:
         if x_scale is None or out_dtype not in _OUT_CODE:
@@ -111,7 +113,7 @@ def _linear_int8(x, weight, weight_scale, bias, x_scale, out_dtype):
             raise GGQUnsupported("linear_int8: results in fp16 / bf16 / fp32")
         if x.device != device or k > MAX_DIM:
             raise GGQUnsupported(f"linear_int8: x on {x.device}, the weight on {device}; rows of at most {MAX_DIM} elements are quantized")
-    _refuse_grad("linear_int8", x, weight_scale, bias)
+    _refuse_grad("linear_int8", x, x_scale, weight_scale, bias)
     if x.dim() == 0 or x.shape[-1] != k:
         raise GGQUnsupported(f"linear_int8: rows of {k} elements for this weight")
     lead = x.shape[:-1]
@@ -122,6 +124,8 @@ def _linear_int8(x, weight, weight_scale, bias, x_scale, out_dtype):
         if bias.dtype is not out_dtype or bias.device != device or not bias.is_contiguous():
             bias = bias.to(device=device, dtype=out_dtype).contiguous()
     m = x.numel() // k
+    if m >= 1 << 31 or n >= 1 << 31:
+        raise GGQUnsupported("linear_int8: fewer than 2^31 rows of x and of the weight")
     y = torch.empty((*lead, n), dtype=out_dtype, device=device)
     if not m or not n:
         return y
@@ -134,7 +138,7 @@ def _linear_int8(x, weight, weight_scale, bias, x_scale, out_dtype):
         xq, x_scale = _rows8(x.reshape(m, k) if x.dim() != 2 else x, "x", True), x_scale.reshape(m).contiguous()
     elif m <= 16 and m * k <= FEW and k % 8 == 0 and out_dtype is x.dtype:
         if not x.is_contiguous() or x.data_ptr() & 15:
-            x = x.contiguous().clone()
+            x = x.clone(memory_format=torch.contiguous_format)
         _launch(_few_call, "ggq_linear_int8_few", device, x.data_ptr(), m, weight.data_ptr(), weight.stride(0), weight_scale.data_ptr(), n, k,
                 None if bias is None else bias.data_ptr(), y.data_ptr(), _OUT_CODE[out_dtype])
         return y

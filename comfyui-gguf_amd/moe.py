@@ -34,7 +34,7 @@ def _rows16(x, what, f32=False):
     if x.dim() != 2 or (x.dtype is torch.float32 and not f32):
         raise GGQUnsupported(f"{what}: fp16 / bf16 matrices")
     if not x.is_contiguous() or x.data_ptr() & 15:
-        x = x.contiguous().clone()
+        x = x.clone(memory_format=torch.contiguous_format)
     return x
 
 
@@ -127,6 +127,8 @@ def _experts(x, ids, weights, gate, up, down, activation):
 
 def _layer(x, router, gate, up, down, top_k, renormalize, activation):
     lead = x.shape
+    if not lead or not lead[-1]:
+        raise GGQUnsupported(f"moe_layer: rows of a tensor, got shape {tuple(lead)}")
     x = x.reshape(-1, lead[-1]) if x.dim() != 2 else x
     if x.shape[0] > MAX_TOKENS:
         raise GGQUnsupported(f"moe_layer: at most {MAX_TOKENS} tokens, got {x.shape[0]}")

@@ -100,6 +100,7 @@ def _block_norm(stream, branch, gate, post_norm, post_weight, norm, weight, bias
     if not 1 <= dim <= MAX_DIM:
         raise GGQUnsupported(f"block_norm: rows of 1 ... {MAX_DIM} elements")
     rows = stream.numel() // dim
+    out = stream
     stream = stream if stream.is_contiguous() else stream.contiguous()
     d = _native.ggq_norm_desc(stream=stream.data_ptr(), rows=rows, dim=dim, rows_per_mod=max(rows, 1), dtype=_OUT_CODE[dtype], norm=kind, post_norm=post_kind, eps=eps)
     keep = []
@@ -131,7 +132,6 @@ def _block_norm(stream, branch, gate, post_norm, post_weight, norm, weight, bias
     if counts:
         d.rows_per_mod = max(1, rows // counts.pop())
     d.params_f32 = flags
-    out = stream
     if branch is not None:
         out = torch.empty_like(stream)
         d.stream_out = out.data_ptr()

@@ -192,6 +192,8 @@ class GGMLInt8Linear(torch.nn.Module):
     def __init__(self, weight, bias=None):
         super().__init__()
         from .int8 import quantize_rows
+        if getattr(weight, "patches", None):
+            raise ValueError("GGMLInt8Linear: the weight is LoRA-patched; apply the patches first")
         dense = dequantize_tensor(weight, torch.float16) if is_quantized(weight) else weight
         dense = dense if type(dense) is torch.Tensor else dense.as_subclass(torch.Tensor)
         q, scale = quantize_rows(dense.detach())
@@ -220,7 +222,7 @@ class GGMLMoE(torch.nn.Module):
     def __init__(self, router, gate, up, down, top_k, renormalize=True, activation="silu"):
         super().__init__()
         router = dequantize_tensor(router, torch.float32) if is_quantized(router) else router
-        self.router = router if type(router) is torch.Tensor else router.as_subclass(torch.Tensor)
+        self.router = (router if type(router) is torch.Tensor else router.as_subclass(torch.Tensor)).float()      # one type for activations of any
         self.gate, self.up, self.down = gate, up, down
         self.top_k, self.renormalize, self.activation = top_k, renormalize, activation
 
@@ -251,7 +253,11 @@ class GGMLMoE(torch.nn.Module):
 
     @staticmethod
     def _expert(stack, expert, dtype):
+        if getattr(stack, "patches", None):
+            raise ValueError("GGMLMoE: the experts are LoRA-patched; patches are not applied to a stack")
         plain = stack if type(stack) is torch.Tensor else stack.as_subclass(torch.Tensor)
+        if not is_quantized(stack):
+            return plain.reshape(stack.shape)[expert].to(dtype)
         experts, rows, cols = stack.tensor_shape
         per = plain.numel() // experts
         one = GGMLTensor(plain.reshape(-1)[expert * per:(expert + 1) * per].clone(), tensor_type=stack.tensor_type, tensor_shape=(rows, cols))

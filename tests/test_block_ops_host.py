@@ -20,6 +20,30 @@ def test_cpu_tensors_are_refused(pkg):
         pkg.moe.moe_experts(x, torch.zeros(2, 1, dtype=torch.int32), torch.zeros(2, 1), x, x, x)
 
 
+def test_layers_do_not_drop_patches(pkg):
+    Q, ops = pkg.qtypes.Q, pkg.ops
+    packed = torch.from_numpy(pkg.synth.make_tensor_bytes(Q.Q8_0, (2 * 64, 64), seed=1))
+    stack = ops.GGMLTensor(packed, tensor_type=Q.Q8_0, tensor_shape=(2, 64, 64), patches=[("lora", "key")])
+    x = torch.ones(3, 64)
+    with pytest.raises(ValueError, match="patch"):
+        ops.GGMLMoE(torch.zeros(2, 64), stack, stack, stack, 1)(x)
+    with pytest.raises(ValueError, match="patch"):
+        ops.GGMLInt8Linear(ops.GGMLTensor(packed, tensor_type=Q.Q8_0, tensor_shape=(128, 64), patches=[("lora", "key")]))
+    with pytest.raises(pkg.dequant.GGQUnsupported):
+        pkg.moe.moe_layer(torch.tensor(1.0), torch.zeros(2, 64), stack, stack, stack, top_k=1)
+
+
+def test_layer_with_stacks_that_are_not_packed(pkg):
+    """Equal experts, equal scores: each token's result is one expert's, every value a small integer or a half (exact in fp32)."""
+    g = torch.Generator().manual_seed(2)
+    one = [torch.randint(-1, 2, s, generator=g).float() for s in ((32, 16), (32, 16), (16, 32))]
+    stacks = [w[None].expand(2, *w.shape) for w in one]
+    x = torch.randint(-2, 3, (5, 16), generator=g).float()
+    layer = pkg.ops.GGMLMoE(torch.zeros(2, 16), *stacks, 2, activation="silu")
+    want = (torch.nn.functional.silu(x @ one[0].t()) * (x @ one[1].t())) @ one[2].t()
+    torch.testing.assert_close(layer(x), want, rtol=2.0 ** -20, atol=2.0 ** -12)
+
+
 def _lib(pkg):
     return pkg._native.lib()
 
@@ -53,9 +77,9 @@ def test_quantize_and_product_arguments_at_the_c_entry(pkg):
     assert q(to=A + 8) == n.GGQ_ERR_ALIGN and q(x=A + 1) == n.GGQ_ERR_ALIGN
     p = lambda x=A, xs=64, sx=A, m=4, w=A, ws=64, sw=A, rows=4, k=64, b=None, y=A, dt=n.F16: L.ggq_linear_int8(x, xs, sx, m, w, ws, sw, rows, k, b, y, dt, None)  # noqa: E731
     assert p(m=0) == n.GGQ_OK and p(rows=0) == n.GGQ_OK
-    for rc in (p(x=None), p(sx=None), p(w=None), p(sw=None), p(y=None), p(xs=48), p(xs=72), p(ws=48), p(k=65), p(k=0), p(k=131072, xs=1 << 20, ws=1 << 20), p(dt=3)):
+    for rc in (p(x=None), p(sx=None), p(w=None), p(sw=None), p(y=None), p(xs=48), p(xs=72), p(ws=48), p(k=65), p(k=0), p(k=131072, xs=1 << 20, ws=1 << 20), p(dt=3), p(m=(1 << 32) - 1, rows=(1 << 32) - 1)):
         assert rc == n.GGQ_ERR_ARG
-    for rc in (p(x=A + 8), p(w=A + 8), p(y=A + 1), p(dt=n.F32, y=A + 2)):
+    for rc in (p(x=A + 8), p(w=A + 8), p(y=A + 1), p(dt=n.F32, y=A + 2), p(b=A + 1), p(sx=A + 2), p(sw=A + 2)):
         assert rc == n.GGQ_ERR_ALIGN
 
 

@@ -104,3 +104,31 @@ def test_the_block_on_another_stream(pkg):
         got = block(*args)
     side.synchronize()
     assert torch.equal(got, want)
+
+
+def test_two_streams_at_once(pkg):
+    """Calls that overlap on two streams do not share scratch memory: each gives what it gives alone."""
+    block = Block(pkg)
+    args = [_inputs(2, 9, 512, torch.float16, 3), _inputs(1, 30, 512, torch.float16, 4)]
+    want = [block(*a) for a in args]
+    sides = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[], []]
+    for side in sides:
+        side.wait_stream(torch.cuda.current_stream())
+    for _ in range(10):
+        for i, side in enumerate(sides):
+            with torch.cuda.stream(side):
+                got[i].append(block(*args[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(g, want[i]) for g in got[i])
+
+
+def test_under_torch_compile(pkg):
+    """A compiled caller runs the same kernels (the calls are graph breaks) and gets the same bits."""
+    block = Block(pkg)
+    args = _inputs(2, 9, 512, torch.bfloat16, 3)
+    want = block(*args)
+    torch._dynamo.reset()
+    got = torch.compile(lambda *a: block(*a), backend="eager")(*args)
+    assert torch.equal(got, want)
