@@ -11,6 +11,7 @@ As the fused linears do, the call raises GGQUnsupported for what the kernel does
 keeps its torch operations then.
 """
 import ctypes
+import struct
 
 import torch
 
@@ -19,12 +20,15 @@ from .dequant import GGQUnsupported, _DEVICE_OK, _OUT_CODE, _cur_device, _device
 
 NORMS = {None: 0, "none": 0, "rms": 1, "layer": 2}
 MAX_DIM = 32768                    # elements of a row: they live in the registers or the LDS of one workgroup
+_PACK = struct.Struct("@16Q3I3if4x").pack         # ggq_norm_desc in one step: a ctypes structure costs 3 us more per call to fill
 _call = None
 
 
 def _bind():
     global _call
-    _call = _native.lib().ggq_block_norm
+    fn = _native.lib()["ggq_block_norm"]            # a function object of its own: the argument is the descriptor's bytes
+    fn.argtypes, fn.restype = [ctypes.c_char_p, ctypes.c_void_p], ctypes.c_int
+    _call = fn
     return _call
 
 
@@ -43,8 +47,10 @@ def _on_gpu(x, what):
 
 
 def _refuse_grad(what, *tensors):
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise GGQUnsupported(f"{what}: autograd is recording -- torch's operations build the graph")
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise GGQUnsupported(f"{what}: autograd is recording -- torch's operations build the graph")
 
 
 def _vector(v, dim, dtype, device, what):
@@ -59,8 +65,8 @@ def _vector(v, dim, dtype, device, what):
     return v.contiguous(), v.dtype is torch.float32
 
 
-def _per_sample(v, lead, dim, dtype, device, what):
-    """A modulation vector per sample as (2-D tensor, stride between vectors, vectors, is fp32).  v's leading dimensions are the stream's, or the
+def _per_sample(v, lead, dim, dtype, device, what, vectors):
+    """A modulation vector per sample as (tensor, stride between vectors, vectors so far or its own, is fp32).  v's leading dimensions are the stream's, or the
     first of them followed by ones."""
     v = _plain(v)
     shape = v.shape
@@ -68,18 +74,21 @@ def _per_sample(v, lead, dim, dtype, device, what):
         raise GGQUnsupported(f"block_norm: {what} of shape {tuple(shape)} on {v.device} for rows of {dim} on {device}")
     if v.dtype is not dtype and v.dtype is not torch.float32:
         v = v.float()
-    if len(lead) == 2 and len(shape) == 3 and shape[1] == 1 and shape[0] == lead[0] and v.stride(2) == 1:          # the usual (batch, 1, dim): no view to make
-        return v, v.stride(0) if shape[0] > 1 else 0, shape[0], v.dtype is torch.float32
-    own = list(shape[:-1])
-    while own and own[-1] == 1:
-        own.pop()
-    if own != list(lead[:len(own)]):
-        raise GGQUnsupported(f"block_norm: {what} of shape {tuple(v.shape)} does not follow the stream's leading dimensions {tuple(lead)}")
-    v = v.reshape(-1, dim)                          # a view where the vectors are one stride apart (a chunk of a modulation linear's output)
-    if v.stride(1) != 1:
-        v = v.contiguous()
+    if not (len(lead) == 2 and len(shape) == 3 and shape[1] == 1 and shape[0] == lead[0] and v.stride(2) == 1):      # the usual (batch, 1, dim): no view to make
+        own = list(shape[:-1])
+        while own and own[-1] == 1:
+            own.pop()
+        if own != list(lead[:len(own)]):
+            raise GGQUnsupported(f"block_norm: {what} of shape {tuple(shape)} does not follow the stream's leading dimensions {tuple(lead)}")
+        v = v.reshape(-1, dim)                      # a view where the vectors are one stride apart (a chunk of a modulation linear's output)
+        if v.stride(1) != 1:
+            v = v.contiguous()
     n = v.shape[0]
-    return v, v.stride(0) if n > 1 else 0, n, v.dtype is torch.float32
+    if n <= 1:
+        return v, 0, vectors, v.dtype is torch.float32
+    if vectors not in (1, n):
+        raise GGQUnsupported(f"block_norm: gate, scale and shift of {vectors} and {n} vectors: give them for the same rows")
+    return v, v.stride(0), n, v.dtype is torch.float32
 
 
 def _block_norm(stream, branch, gate, post_norm, post_weight, norm, weight, bias, scale, shift, eps, quantize):
@@ -102,57 +111,55 @@ def _block_norm(stream, branch, gate, post_norm, post_weight, norm, weight, bias
     rows = stream.numel() // dim
     out = stream
     stream = stream if stream.is_contiguous() else stream.contiguous()
-    d = _native.ggq_norm_desc(stream=stream.data_ptr(), rows=rows, dim=dim, rows_per_mod=max(rows, 1), dtype=_OUT_CODE[dtype], norm=kind, post_norm=post_kind, eps=eps)
-    keep = []
+    flags = at_branch = at_out = at_post = at_weight = at_bias = at_gate = at_scale = at_shift = at_y = at_y_scale = gate_stride = scale_stride = shift_stride = y_stride = 0
     if branch is not None:
         branch = _plain(branch)
         if branch.shape != stream.shape or branch.dtype is not dtype or branch.device != device:
             raise GGQUnsupported(f"block_norm: branch {tuple(branch.shape)} {branch.dtype} is not like the stream {tuple(stream.shape)} {dtype}")
         branch = branch if branch.is_contiguous() else branch.contiguous()
-        d.branch = branch.data_ptr()
-    flags = 0
-    for bit, name, v in ((1, "post_weight", post_weight), (4, "weight", weight), (8, "bias", bias)):
-        if v is not None:
-            v, is32 = _vector(v, dim, dtype, device, name)
-            keep.append(v)
-            setattr(d, name, v.data_ptr())
-            flags |= bit if is32 else 0
-    counts = set()
-    for bit, name, v in ((2, "gate", gate), (16, "scale", scale), (32, "shift", shift)):
-        if v is not None:
-            v, stride, n, is32 = _per_sample(v, lead, dim, dtype, device, name)
-            keep.append(v)
-            setattr(d, name, v.data_ptr())
-            setattr(d, name + "_stride", stride)
-            flags |= bit if is32 else 0
-            if n > 1:
-                counts.add(n)
-    if len(counts) > 1:
-        raise GGQUnsupported(f"block_norm: gate, scale and shift of {sorted(counts)} vectors: give them for the same rows")
-    if counts:
-        d.rows_per_mod = max(1, rows // counts.pop())
-    d.params_f32 = flags
+        at_branch = branch.data_ptr()
+    if post_weight is not None:
+        post_weight, is32 = _vector(post_weight, dim, dtype, device, "post_weight")
+        at_post, flags = post_weight.data_ptr(), 1 if is32 else 0
+    if weight is not None:
+        weight, is32 = _vector(weight, dim, dtype, device, "weight")
+        at_weight, flags = weight.data_ptr(), flags | (4 if is32 else 0)
+    if bias is not None:
+        bias, is32 = _vector(bias, dim, dtype, device, "bias")
+        at_bias, flags = bias.data_ptr(), flags | (8 if is32 else 0)
+    vectors = 1                                     # vectors per parameter, where one of them has more than one
+    if gate is not None:
+        gate, gate_stride, vectors, is32 = _per_sample(gate, lead, dim, dtype, device, "gate", vectors)
+        at_gate, flags = gate.data_ptr(), flags | (2 if is32 else 0)
+    if scale is not None:
+        scale, scale_stride, vectors, is32 = _per_sample(scale, lead, dim, dtype, device, "scale", vectors)
+        at_scale, flags = scale.data_ptr(), flags | (16 if is32 else 0)
+    if shift is not None:
+        shift, shift_stride, vectors, is32 = _per_sample(shift, lead, dim, dtype, device, "shift", vectors)
+        at_shift, flags = shift.data_ptr(), flags | (32 if is32 else 0)
     if branch is not None:
         out = torch.empty_like(stream)
-        d.stream_out = out.data_ptr()
+        at_out = out.data_ptr()
     y = y_scale = None
     if quantize:
-        pad = (dim + 15) // 16 * 16
-        y = torch.empty((*lead, pad), dtype=torch.int8, device=device)
+        y_stride = (dim + 15) // 16 * 16
+        y = torch.empty((*lead, y_stride), dtype=torch.int8, device=device)
         y_scale = torch.empty(lead, dtype=torch.float32, device=device)
-        d.y, d.y_scale, d.y_stride = y.data_ptr(), y_scale.data_ptr(), pad
-        y = y[..., :dim] if pad != dim else y
+        at_y, at_y_scale = y.data_ptr(), y_scale.data_ptr()
+        y = y[..., :dim] if y_stride != dim else y
     elif kind:
         y = torch.empty_like(stream)
-        d.y = y.data_ptr()
+        at_y = y.data_ptr()
     if rows:
         index = device.index
         call = _call or _bind()
+        desc = _PACK(stream.data_ptr(), at_branch, at_out, at_y, at_y_scale, at_post, at_gate, at_weight, at_bias, at_scale, at_shift,
+                     rows, gate_stride, scale_stride, shift_stride, y_stride, dim, max(rows // vectors, 1), flags, _OUT_CODE[dtype], kind, post_kind, eps)
         if _cur_device() != index:
             with torch.cuda.device(index):
-                rc = call(ctypes.byref(d), _raw_stream(index))
+                rc = call(desc, _raw_stream(index))
         else:
-            rc = call(ctypes.byref(d), _raw_stream(index))
+            rc = call(desc, _raw_stream(index))
         if rc:
             _native.check(rc, "ggq_block_norm")
     return out, ((y, y_scale) if quantize else y)
