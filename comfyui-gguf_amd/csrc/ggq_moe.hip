@@ -22,12 +22,12 @@ uint32_t ring_slots(uint32_t rest, uint32_t waves, uint32_t slot_bytes)
 template <class F, int OUT, int MB>
 hipError_t launch_up(MoeArgs a, hipStream_t s)
 {
-    constexpr uint32_t fixed = sizeof(MoeTable) + MOE_WAVES * MOE_MAX_TOKENS * 4 + (MB == 1 ? 2 : MB) * MOE_WAVES * 1024 + 64;
+    constexpr uint32_t fixed = sizeof(MoeTable) + MOE_WAVES * MOE_MAX_TOKENS * 4 + 2 * MB * MOE_WAVES * 1024 + 64, mats = MB == 1 ? 1 : 2;
     const uint32_t pairs = a.tokens * a.top_k, most = (pairs < a.experts ? pairs : a.experts) * (a.ff / 16u);      // tiles, if every pair chose another expert
     const uint32_t blocks = (a.tokens + 15u) / 16u;
     a.spare = blocks > (uint32_t)MB ? blocks - MB : 0u;
-    a.ring = ring_slots(fixed + MOE_WAVES * a.spare * 1024u, MOE_WAVES, Mf16Geom<F>::SLICE);
-    const uint32_t lds = MOE_WAVES * (a.spare * 1024u + a.ring * Mf16Geom<F>::SLICE);
+    a.ring = ring_slots(fixed + MOE_WAVES * mats * a.spare * 1024u, MOE_WAVES, Mf16Geom<F>::SLICE);
+    const uint32_t lds = MOE_WAVES * (mats * a.spare * 1024u + a.ring * Mf16Geom<F>::SLICE);
     if (fixed + lds > ALL_LDS) return hipErrorInvalidConfiguration;
     static std::atomic<uint64_t> raised{0};
     const hipError_t e = allow_lds(reinterpret_cast<const void*>(&moe_up<F, OUT, MB>), (int)(ALL_LDS - fixed), raised);

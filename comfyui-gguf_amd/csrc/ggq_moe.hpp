@@ -264,27 +264,33 @@ template <int KEEP> GGQ_DEV void moe_wait() { asm volatile("s_waitcnt vmcnt(%0)"
 // keep what they hold: a column of the product depends on that column alone.  (One token, 2 x 10240 x 4096: with every lane loading, the columns were 8 KiB
 // per span against 2.3 of weights, and cost 8 of 38 us in the vector cache.)
 template <class F, int MB>
-GGQ_DEV void moe_columns(const GGQ_GLOBAL uint8_t* const (&col)[MB], uint32_t span, uint32_t k_len, u32x4 (&x)[MB][8])
+GGQ_DEV void moe_half(const GGQ_GLOBAL uint8_t* const (&col)[MB], uint32_t span, uint32_t k_len, int g, u32x4 (&x)[MB][8])
 {
     const int c = (int)(threadIdx.x & 63u) >> 4;
 #pragma unroll
-    for (int g = 0; g < 2; g++)
-#pragma unroll
-        for (int mb = 0; mb < MB; mb++) {
-            const GGQ_GLOBAL uint8_t* src = col[mb] + (uint64_t)span * (MF_SPAN * 2) + (uint32_t)(g * 256);
-            if constexpr (F::BS == 32) {                                                                   // past the end of k: zeros
-                if (span * (uint32_t)MF_SPAN + (uint32_t)(128 * g + 32 * c) >= k_len) src = (GGQ_GLOBAL const uint8_t*)MF16_ZEROS;
-            }
-            if (col[mb] != nullptr) {
-#pragma unroll
-                for (int t = 0; t < 4; t++) x[mb][4 * g + t] = *(GGQ_GLOBAL const u32x4*)(src + t * 16);
-            }
+    for (int mb = 0; mb < MB; mb++) {
+        const GGQ_GLOBAL uint8_t* src = col[mb] + (uint64_t)span * (MF_SPAN * 2) + (uint32_t)(g * 256);
+        if constexpr (F::BS == 32) {                                                                       // past the end of k: zeros
+            if (span * (uint32_t)MF_SPAN + (uint32_t)(128 * g + 32 * c) >= k_len) src = (GGQ_GLOBAL const uint8_t*)MF16_ZEROS;
         }
+        if (col[mb] != nullptr) {
+#pragma unroll
+            for (int t = 0; t < 4; t++) x[mb][4 * g + t] = *(GGQ_GLOBAL const u32x4*)(src + t * 16);
+        }
+    }
 }
 
-// acc += 16 rows of weights, decoded from one span of packed bytes (`wspan`: this lane's row in LDS), times MB blocks of 16 columns
-template <class F, int OUT, int MB>
-GGQ_DEV void moe_span(const uint8_t* wspan, const u32x4 (&x)[MB][8], f32x4 (&acc)[MB])
+template <class F, int MB>
+GGQ_DEV void moe_columns(const GGQ_GLOBAL uint8_t* const (&col)[MB], uint32_t span, uint32_t k_len, u32x4 (&x)[MB][8])
+{
+#pragma unroll
+    for (int g = 0; g < 2; g++) moe_half<F, MB>(col, span, k_len, g, x);
+}
+
+// acc += 16 rows of weights, decoded from one span of packed bytes (`wspan`: this lane's row in LDS), times MB blocks of 16 columns.  after(g): half g of the columns
+// has been multiplied
+template <class F, int OUT, int MB, class After>
+GGQ_DEV void moe_span(const uint8_t* wspan, const u32x4 (&x)[MB][8], f32x4 (&acc)[MB], After after)
 {
     constexpr int CPB = F::BS / 8;
     const int c = (int)(threadIdx.x & 63u) >> 4;
@@ -301,6 +307,7 @@ GGQ_DEV void moe_span(const uint8_t* wspan, const u32x4 (&x)[MB][8], f32x4 (&acc
 #pragma unroll
             for (int mb = 0; mb < MB; mb++) acc[mb] = mfma16<OUT>(wa, x[mb][4 * g + t], acc[mb]);
         }
+        after(g);
     }
 }
 
@@ -338,7 +345,10 @@ GGQ_DEV uint32_t moe_list(const MoeTable& s, const float* weights, const MoeArgs
 }
 
 // hidden = act(Wg x) * (Wu x), 16 hidden rows of a chosen expert at a time.  The (expert, tile of 16 rows) list is dealt out evenly: the first workgroups take
-// one tile more.  Waves 0, 2, 4, 6 contract gate rows, waves 1, 3, 5, 7 up rows, every fourth span each.
+// one tile more.  With one block of columns, waves 0, 2, 4, 6 contract gate rows, waves 1, 3, 5, 7 up rows, every fourth span each.  With more, the columns are several
+// times the weights' bytes, and a wave takes an equal, contiguous part of the list (span 0 of gate, span 0 of up, span 1 of gate, ...), with sums for both and the columns of
+// a span loaded once for the two, ahead: as soon as the last span's have been used.  (33 tokens, two of four experts of 2 x 6848 x 2432 in Q8_0: 71 us as with one block, 76 with
+// the columns shared but not ahead, 64 so; 64 tokens, two of eight of 2 x 10240 x 4096 in Q4_K: the layer 532 -> 415.)
 template <class F, int OUT, int MB>
 __global__ __launch_bounds__(MOE_WAVES * 64) MOE_OCC(MB) void moe_up(const MoeArgs a)
 {
@@ -348,7 +358,8 @@ __global__ __launch_bounds__(MOE_WAVES * 64) MOE_OCC(MB) void moe_up(const MoeAr
     __shared__ MoeTable table;
     __shared__ uint32_t slots_[MOE_WAVES][MOE_MAX_TOKENS];                         // per column: where its hidden row goes (= token * top_k + place)
     constexpr int TURNS = MB == 1 ? 2 : 1;                                         // two tiles' partial sums: the next tile's are written while one is added up
-    __shared__ f32x4 red[TURNS][MOE_WAVES][MB][64];
+    constexpr int MATS = MB == 1 ? 1 : 2;                                          // matrices that a wave has sums of
+    __shared__ f32x4 red[TURNS][MOE_WAVES][MATS][MB][64];
     const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const uint32_t lane = threadIdx.x & 63u, r = lane & 15u, c = lane >> 4;
     const uint32_t pairs = a.tokens * a.top_k;
@@ -357,76 +368,109 @@ __global__ __launch_bounds__(MOE_WAVES * 64) MOE_OCC(MB) void moe_up(const MoeAr
     const uint32_t tiles = a.ff / 16u, total = table.n * tiles, each = total / gridDim.x, more = total - each * gridDim.x;
     const uint32_t t0 = blockIdx.x * each + (blockIdx.x < more ? blockIdx.x : more), t1 = t0 + each + (blockIdx.x < more ? 1u : 0u);
     const uint64_t row_bytes = (uint64_t)(a.dim / F::BS) * F::TS;
-    const uint32_t n_spans = (a.dim + MF_SPAN - 1) / MF_SPAN, tail_len = a.dim - (n_spans - 1) * (uint32_t)MF_SPAN, span0 = wave >> 1;
-    const gcptr weights = (gcptr)((wave & 1u) ? a.up : a.gate);
-    uint8_t* ring = dyn + MOE_WAVES * a.spare * 1024u + wave * a.ring * (uint32_t)G::SLICE;
+    const uint32_t n_spans = (a.dim + MF_SPAN - 1) / MF_SPAN, tail_len = a.dim - (n_spans - 1) * (uint32_t)MF_SPAN;
+    // this wave's units of a tile: [u0, u1) in steps of `by`, unit u = span u / MATS of matrix u % 2 (or of the wave's own)
+    const uint32_t u0 = MATS == 1 ? wave >> 1 : 2u * n_spans * wave / MOE_WAVES, u1 = MATS == 1 ? n_spans : 2u * n_spans * (wave + 1u) / MOE_WAVES, by = MATS == 1 ? MOE_WAVES / 2 : 1;
+    auto is_up = [&](uint32_t u) { return MATS == 1 ? wave & 1u : u & 1u; };
+    uint8_t* ring = dyn + MOE_WAVES * MATS * a.spare * 1024u + wave * a.ring * (uint32_t)G::SLICE;
     uint32_t* slots = slots_[wave];
-    f32x4* spare = reinterpret_cast<f32x4*>(dyn) + (uint64_t)wave * a.spare * 64u;
+    f32x4* spare = reinterpret_cast<f32x4*>(dyn) + (uint64_t)wave * MATS * a.spare * 64u;
     uint32_t turn = 0;
     for (uint32_t t = t0; t < t1;) {                                               // one expert at a time: tiles [t, stop) of the list
         const uint32_t nth = t / tiles, stop = (nth + 1) * tiles < t1 ? (nth + 1) * tiles : t1;
         const uint32_t n_cols = moe_list(table, nullptr, a, table.list[nth], slots, nullptr);
-        const gcptr base = weights + (uint64_t)table.list[nth] * a.ff * row_bytes;
-        auto weights_at = [&](uint32_t i) { return base + (uint64_t)(i - nth * tiles) * 16u * row_bytes; };        // tile i of the list
+        const uint64_t base = (uint64_t)table.list[nth] * a.ff * row_bytes;
+        auto weights_at = [&](uint32_t i, uint32_t u) { return (gcptr)(is_up(u) ? a.up : a.gate) + base + (uint64_t)(i - nth * tiles) * 16u * row_bytes; };      // tile i of the list
         auto column = [&](uint32_t v) { return v < n_cols ? (GGQ_GLOBAL const uint8_t*)a.x + (uint64_t)(slots[v] / a.top_k) * a.dim * 2 + c * 64u : nullptr; };
         const GGQ_GLOBAL uint8_t* col[MB];
 #pragma unroll
         for (int mb = 0; mb < MB; mb++) col[mb] = column((uint32_t)(mb * 16) + r);
         const uint32_t blocks = (n_cols + 15u) / 16u;
+        u32x4 both[MATS == 1 ? 1 : MB][8];                                         // the columns of a span, for its two units
+        if constexpr (MATS == 2) {
+            if (u0 < u1) moe_columns<F, MB>(col, u0 / MATS, a.dim, both);
+        }
 
-        uint32_t ft = t, fs = span0, in = 0, out = 0;                              // the next span to request; ring slots
+        uint32_t ft = t, fu = u0, in = 0, out = 0;                                 // the next unit to request; ring slots
         auto request = [&]() {                                                     // -> 2: a whole span, 1: a short one, 0: nothing left
-            if (ft >= stop || fs >= n_spans) return 0;
+            if (ft >= stop || fu >= u1) return 0;
+            const uint32_t fs = fu / MATS;
             const bool tail = F::BS == 32 && fs + 1 == n_spans && tail_len != (uint32_t)MF_SPAN;
-            moe_request<F>(weights_at(ft), (uint32_t)row_bytes, fs, (tail ? tail_len : (uint32_t)MF_SPAN) / (uint32_t)F::BS * (uint32_t)F::TS, ring + in * G::SLICE);
+            moe_request<F>(weights_at(ft, fu), (uint32_t)row_bytes, fs, (tail ? tail_len : (uint32_t)MF_SPAN) / (uint32_t)F::BS * (uint32_t)F::TS, ring + in * G::SLICE);
             in = in + 1 == a.ring ? 0 : in + 1;
-            fs += MOE_WAVES / 2;
-            if (fs >= n_spans) { fs = span0; ft++; }
+            fu += by;
+            if (fu >= u1) { fu = u0; ft++; }
             return tail ? 1 : 2;
         };
         request();
         if (a.ring > 2) request();
-        f32x4 acc[MB];
+        f32x4 acc[MATS][MB];                                                       // acc[0]: of the matrix of this unit, acc[1] of the other
         auto clear = [&]() {
 #pragma unroll
-            for (int mb = 0; mb < MB; mb++) acc[mb] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-            for (uint32_t q = MB; q < blocks; q++) spare[(q - MB) * 64u + lane] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            for (int mb = 0; mb < MB; mb++)
+#pragma unroll
+                for (int i = 0; i < MATS; i++) acc[i][mb] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            for (uint32_t q = 0; q < (blocks > (uint32_t)MB ? MATS * a.spare : 0u); q++) spare[q * 64u + lane] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         };
-        uint32_t tile = t - nth * tiles, span = span0;
+        uint32_t tile = t - nth * tiles, unit = u0;
         const uint32_t tile_end = stop - nth * tiles;
         auto one = [&]() {
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");                     // the slot that is filled next has been read
-            u32x4 x[MB][8];
-            moe_columns<F, MB>(col, span, a.dim, x);
+            const uint32_t span = unit / MATS, mat = is_up(unit);
+            u32x4 own[MB][8];
+            auto& x = [&]() -> u32x4 (&)[MB][8] { if constexpr (MATS == 1) return own; else return both; }();
+            if constexpr (MATS == 1) moe_columns<F, MB>(col, span, a.dim, x);
             asm volatile("" ::: "memory");
             if (request() == 2) moe_wait<(int)MoeGeom<F>::LOADS>();                // all but the span just requested
             else moe_wait<0>();
             uint8_t* slot = ring + out * G::SLICE;
             out = out + 1 == a.ring ? 0 : out + 1;
-            const gcptr rows = weights_at(nth * tiles + tile);
+            const gcptr rows = weights_at(nth * tiles + tile, unit);
             if (F::BS == 32 && span + 1 == n_spans && tail_len != (uint32_t)MF_SPAN) moe_cut<F>(rows, (uint32_t)row_bytes, span, tail_len / (uint32_t)F::BS * (uint32_t)F::TS, slot);
             const uint32_t skew = G::SKEW ? moe_offset(rows, r, (uint32_t)row_bytes, span * G::SPAN_BYTES) & 15u : 0u;
-            moe_span<F, OUT, MB>(slot + r * G::ROW_STRIDE + skew, x, acc);
+            // MATS 2: the columns of the next span, if the next unit has another, are on their way as soon as this one's have been used
+            const uint32_t next = unit + by < u1 ? unit + by : u0;
+            const bool other = MATS == 2 && (next > unit ? (next & 1u) == 0 : tile + 1 < tile_end);
+            moe_span<F, OUT, MB>(slot + r * G::ROW_STRIDE + skew, x, acc[0], [&](int g) {
+                if constexpr (MATS == 2) {
+                    if (other) moe_half<F, MB>(col, next / MATS, a.dim, g, both);
+                }
+            });
             for (uint32_t q = MB; q < blocks; q++) {                               // more tokens on one expert than the kernel was picked for
                 const GGQ_GLOBAL uint8_t* const late[1] = {column(q * 16u + r)};
                 u32x4 lx[1][8];
-                f32x4 sum[1] = {spare[(q - MB) * 64u + lane]};
+                f32x4& kept = spare[((MATS == 1 ? 0u : mat * a.spare) + q - MB) * 64u + lane];
+                f32x4 sum[1] = {kept};
                 moe_columns<F, 1>(late, span, a.dim, lx);
-                moe_span<F, OUT, 1>(slot + r * G::ROW_STRIDE + skew, lx, sum);
-                spare[(q - MB) * 64u + lane] = sum[0];
+                moe_span<F, OUT, 1>(slot + r * G::ROW_STRIDE + skew, lx, sum, [](int) {});
+                kept = sum[0];
             }
             wave_sync();
-            span += MOE_WAVES / 2;
+            if constexpr (MATS == 2) {                                             // units take turns between the matrices
+#pragma unroll
+                for (int mb = 0; mb < MB; mb++) {
+                    const f32x4 o = acc[0][mb];
+                    acc[0][mb] = acc[1][mb];
+                    acc[1][mb] = o;
+                }
+            }
+            unit += by;
         };
         // the sums of a tile over the waves, the activation, the two parts of the hidden value; the waves take turns at it
         auto finish = [&]() {
+            if (TURNS == 1) moe_barrier();                                         // the last tile's sums have been added up: by waves that were a tile's time behind at most
 #pragma unroll
-            for (int mb = 0; mb < MB; mb++) red[turn][wave][mb][lane] = acc[mb];
+            for (int mb = 0; mb < MB; mb++)
+#pragma unroll
+                for (int i = 0; i < MATS; i++) red[turn][wave][MATS == 1 ? 0u : (unit + (uint32_t)i) & 1u][mb][lane] = acc[i][mb];
             moe_barrier();
             for (uint32_t q = (wave - tile * MB) % MOE_WAVES; q < blocks; q += MOE_WAVES) {
-                auto sum = [&](uint32_t w) { return q < (uint32_t)MB ? red[turn][w][q][lane] : reinterpret_cast<const f32x4*>(dyn)[(uint64_t)(w * a.spare + q - MB) * 64u + lane]; };
-                f32x4 g = sum(0), u = sum(1);
-                for (uint32_t w = 2; w < MOE_WAVES; w += 2) { g += sum(w); u += sum(w + 1); }
+                auto sum = [&](uint32_t w, uint32_t i) {
+                    return q < (uint32_t)MB ? red[turn][w][i][q][lane] : reinterpret_cast<const f32x4*>(dyn)[(uint64_t)((w * MATS + i) * a.spare + q - MB) * 64u + lane];
+                };
+                constexpr uint32_t EACH = 3 - MATS, UP = MATS == 1 ? 0 : 1;
+                f32x4 g = sum(0, 0), u = sum(EACH - 1, UP);
+                for (uint32_t w = EACH; w < MOE_WAVES; w += EACH) { g += sum(w, 0); u += sum(w + EACH - 1, UP); }
                 const uint32_t v = q * 16u + r;                                    // D[row = 4c + i][column = r]
                 if (v < n_cols) {
                     uint32_t hi[2], lo[2];
@@ -448,16 +492,16 @@ __global__ __launch_bounds__(MOE_WAVES * 64) MOE_OCC(MB) void moe_up(const MoeAr
                     *reinterpret_cast<u32x2*>(dst + (uint64_t)pairs * a.ff * 2) = u32x2{lo[0], lo[1]};
                 }
             }
-            if (TURNS == 1 || blocks > (uint32_t)MB) moe_barrier();                // the same sums' place is written next
-            else turn ^= 1u;
+            if (blocks > (uint32_t)MB) moe_barrier();                              // the same sums' place is written next
+            else if (TURNS == 2) turn ^= 1u;
             tile++;
-            span = span0;
+            unit = u0;
             clear();
         };
         clear();
         while (tile < tile_end) {
-            if (span < n_spans) one();
-            if (span >= n_spans) finish();
+            if (unit < u1) one();
+            if (unit >= u1) finish();
         }
         t = stop;
     }
@@ -536,13 +580,13 @@ __global__ __launch_bounds__(W * 64) MOE_OCC(MB) void moe_down(const MoeArgs a)
         out = out + 1 == a.ring ? 0 : out + 1;
         if (F::BS == 32 && span + 1 == n_spans && tail_len != (uint32_t)MF_SPAN) moe_cut<F>(rows, (uint32_t)row_bytes, span, tail_len / (uint32_t)F::BS * (uint32_t)F::TS, slot);
         const uint32_t skew = G::SKEW ? moe_offset(rows, r, (uint32_t)row_bytes, span * G::SPAN_BYTES) & 15u : 0u;
-        moe_span<F, OUT, MB>(slot + r * G::ROW_STRIDE + skew, x, acc);
+        moe_span<F, OUT, MB>(slot + r * G::ROW_STRIDE + skew, x, acc, [](int) {});
         for (uint32_t q = MB; q < blocks; q++) {                                   // more tokens on one expert than the kernel was picked for
             const GGQ_GLOBAL uint8_t* const late[1] = {column(q * 16u + r)};
             u32x4 lx[1][8];
             f32x4 sum[1] = {spare[(q - MB) * 64u + lane]};
             moe_columns<F, 1>(late, span, a.ff, lx);
-            moe_span<F, OUT, 1>(slot + r * G::ROW_STRIDE + skew, lx, sum);
+            moe_span<F, OUT, 1>(slot + r * G::ROW_STRIDE + skew, lx, sum, [](int) {});
             spare[(q - MB) * 64u + lane] = sum[0];
         }
         wave_sync();
