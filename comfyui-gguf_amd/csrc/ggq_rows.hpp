@@ -283,6 +283,7 @@ GGQ_DEV void team_clear(float* red, uint32_t n)
 // is one wave, four teams to a workgroup, no barrier; else a team is a workgroup of up to 16 waves.  The next row's loads are under way while a row is
 // computed, and a sample's factors stay in registers from row to row (read for every row, they would be up to 14 bytes per element from the caches
 // beside the 8 from memory that the row itself moves).
+// Measured: 9216 x 4096 bf16, rms on either side, gate and modulation: 55 us, 5.5 TB/s (a large copy: 4.9); 666 x 2432 fp16, layer norm: 9.0 us; one row of 4096: 3.2 us.
 template <int DT, bool SOLO, bool TAIL>
 __global__ __launch_bounds__(SOLO ? 256 : TAIL ? 512 : 1024) void block_norm(const RowArgs a, uint32_t rows_per_team)
 {
@@ -370,7 +371,7 @@ __global__ __launch_bounds__(SOLO ? 256 : TAIL ? 512 : 1024) void block_norm(con
 }
 
 // 8-bit form of rows as they are: as block_norm without its norms, and without its registers -- a row per team, so many more rows are under way at once
-// (4608 x 2432 bf16: 22 us with block_norm's kernel).
+// (4608 x 2432 bf16: 11 us, 22 with block_norm's kernel).
 template <int DT, bool SOLO, bool TAIL>
 __global__ __launch_bounds__(SOLO ? 256 : 1024) void quantize_rows(const uint8_t* __restrict__ x, uint64_t rows, uint32_t dim, uint8_t* __restrict__ q, uint64_t q_stride,
                                                                   float* __restrict__ q_scale)
