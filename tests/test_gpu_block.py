@@ -132,3 +132,16 @@ def test_under_torch_compile(pkg):
     torch._dynamo.reset()
     got = torch.compile(lambda *a: block(*a), backend="eager")(*args)
     assert torch.equal(got, want)
+
+
+def test_no_rows_and_rows_that_had_to_be_copied(pkg):
+    norm = pkg.norms.block_norm
+    none = torch.empty(0, 5, 64, device=DEV, dtype=torch.bfloat16)
+    r, y = norm(none, none, scale=torch.empty(0, 1, 64, device=DEV), shift=torch.empty(0, 64, device=DEV))
+    assert r.shape == y.shape == none.shape
+    r, (q, s) = norm(torch.empty(2, 0, 64, device=DEV, dtype=torch.float16), gate=None, scale=torch.ones(2, 1, 64, device=DEV), quantize=True)
+    assert q.shape == (2, 0, 64) and s.shape == (2, 0)
+    x = torch.randn(64, 6, device=DEV, dtype=torch.bfloat16).t()
+    r, y = norm(x)
+    assert r is x and torch.equal(y, norm(x.contiguous())[1])
+    assert pkg.int8.linear_int8(torch.empty(0, 64, device=DEV, dtype=torch.float16), *pkg.int8.quantize_rows(torch.ones(8, 64, device=DEV))).shape == (0, 8)
