@@ -66,11 +66,12 @@ template <int OUT, int RT> GGQ_DEV double moe_score(const uint8_t* x, const uint
 }
 
 // The top_k experts of one token and their weights, from the scores in LDS; by the whole workgroup, which has a thread for every expert.  rank_[e] = how many
-// experts come before e; a NaN comes last (its weight is NaN all the same).  The comparisons of an expert are split over the threads there are.
+// experts come before e.  A NaN comes last and makes all of the token's weights NaN, chosen or not: it is in the softmax's sum (rank_[experts]: whether there
+// is one).  The comparisons of an expert are split over the threads there are.
 GGQ_DEV void moe_choose(const double* score, uint32_t* rank_, double* chosen, uint32_t experts, uint32_t top_k, int renormalize, int32_t* ids, float* weights)
 {
     const uint32_t padded = (experts + 63u) & ~63u, parts = blockDim.x / padded, t = threadIdx.x % padded, part = threadIdx.x / padded;
-    if (threadIdx.x < experts) rank_[threadIdx.x] = 0;
+    for (uint32_t i = threadIdx.x; i <= experts; i += blockDim.x) rank_[i] = 0;
     __syncthreads();
     if (t < experts && part < parts) {
         const double own = score[t];
@@ -81,6 +82,7 @@ GGQ_DEV void moe_choose(const double* score, uint32_t* rank_, double* chosen, ui
             before += (o > own || (o == own && e < t) || (own != own && (o == o || e < t))) ? 1u : 0u;
         }
         atomicAdd(&rank_[t], before);
+        if (own != own) rank_[experts] = 1;                                 // whoever writes, the same value
     }
     __syncthreads();
     const uint32_t rank = threadIdx.x < experts ? rank_[threadIdx.x] : ~0u;
@@ -91,7 +93,7 @@ GGQ_DEV void moe_choose(const double* score, uint32_t* rank_, double* chosen, ui
     __syncthreads();
     if (rank < top_k) {
         const double top = chosen[0];
-        float sum = 0.0f;
+        float sum = rank_[experts] ? __builtin_nanf("") : 0.0f;
         if (renormalize) {
 #pragma unroll
             for (uint32_t s = 0; s < MOE_MAX_TOPK; s++) sum += s < top_k ? __expf((float)(chosen[s] - top)) : 0.0f;
@@ -110,7 +112,7 @@ __global__ __launch_bounds__(MOE_ROUTE_WAVES * 64) void moe_route(const uint8_t*
                                                                  uint32_t top_k, int renormalize, int32_t* __restrict__ ids, float* __restrict__ weights)
 {
     __shared__ double score[MOE_ROUTE_WAVES];
-    __shared__ uint32_t rank[MOE_ROUTE_WAVES];
+    __shared__ uint32_t rank[MOE_ROUTE_WAVES + 1];
     __shared__ double chosen[MOE_MAX_TOPK];
     const uint32_t wave = threadIdx.x >> 6;
     if (wave < experts) {
@@ -136,7 +138,7 @@ __global__ __launch_bounds__(MOE_MAX_EXPERTS) void moe_pick(const double* __rest
                                                            float* __restrict__ weights)
 {
     __shared__ double score[MOE_MAX_EXPERTS];
-    __shared__ uint32_t rank[MOE_MAX_EXPERTS];
+    __shared__ uint32_t rank[MOE_MAX_EXPERTS + 1];
     __shared__ double chosen[MOE_MAX_TOPK];
     if (threadIdx.x < experts) score[threadIdx.x] = scores[(uint64_t)blockIdx.x * experts + threadIdx.x];
     __syncthreads();

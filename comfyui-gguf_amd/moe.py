@@ -142,7 +142,7 @@ _eager_route, _eager_experts, _eager_layer = (torch.compiler.disable(f) for f in
 
 def route(x, router, top_k, *, renormalize=True):
     """-> (ids int32, weights fp32), both (tokens, top_k), the largest probability first.  x: (tokens, dim) fp16 / bf16 on the GPU, router: (experts, dim) of x's type or
-    fp32 (as GGUF files keep it), dim % 8 == 0.  Scores are fp64; a NaN score comes last, and its token's weights are NaN."""
+    fp32 (as GGUF files keep it), dim % 8 == 0.  Scores are fp64; a NaN score comes last, and all of its token's weights are NaN."""
     return (_eager_route if _is_compiling() else _route)(x, router, top_k, renormalize)
 
 

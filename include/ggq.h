@@ -265,7 +265,8 @@ int ggq_linear_int8_few(const void* x, uint32_t m, const void* wq, uint64_t w_st
  * lower index.  x: tokens x dim, router: experts x dim, of `dtype`
  * (GGQ_F16 / GGQ_BF16) and router_dtype (`dtype` or GGQ_F32), contiguous, 16-byte aligned, dim % 8 == 0.  ids: int32
  * tokens x top_k; weights: fp32, p of the chosen ones, divided by their sum if `renormalize`.  At
- * most 65535 tokens.  Scores are fp64; a NaN score comes last.  workspace: ggq_moe_route_workspace() bytes (0 for up to 16 experts), 8-byte aligned. */
+ * most 65535 tokens.  Scores are fp64; a NaN score comes last and makes
+ * all weights of its token NaN, as the softmax does.  workspace: ggq_moe_route_workspace() bytes (0 for up to 16 experts), 8-byte aligned. */
 int ggq_moe_route(const void* x, const void* router, uint32_t tokens, uint32_t dim, uint32_t experts, uint32_t top_k, int renormalize, int32_t* ids,
                   float* weights, int dtype, int router_dtype, void* workspace, uint64_t workspace_bytes, void* hip_stream);
 uint64_t ggq_moe_route_workspace(uint32_t tokens, uint32_t experts);
