@@ -1,8 +1,9 @@
 """The block operators (norms, int8, moe and their layers) at the edges of what their documentation allows."""
+import numpy as np
 import pytest
 import torch
 
-from test_gpu_moe import Stack, U
+from test_gpu_moe import DT, Stack, U
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -50,3 +51,44 @@ def test_a_layer_whose_router_holds_a_nan(pkg):
     x = torch.randn(65, 64, device=DEV, generator=g).bfloat16()
     layer = pkg.ops.GGMLMoE(router, gate, up, down, top_k=2)
     assert bool(layer(x[:64]).isnan().all()) and bool(layer(x).isnan().all())
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("experts", [8, 48])
+@pytest.mark.parametrize("wide", [False, True])
+def test_scores_that_cancel(pkg, kind, experts, wide):
+    """Each expert's score is a small number beside terms of 2^24 that cancel exactly: every sum of these terms is exact in 64 bits in any order (31 bits), and in
+    32 bits the small numbers are lost.  Equal scores from different columns tie to the lower expert."""
+    g = np.random.default_rng(17)
+    dim = 1024
+    small = g.permutation(experts) // 2                         # each value twice: ties
+    w = np.zeros((experts, dim // 4, 4))
+    for e in range(experts):
+        fours = g.permutation(dim // 4)[:8]
+        w[e, fours[:4], 0], w[e, fours[4:], 0] = 4096.0, -4096.0
+        w[e, fours[g.integers(8)], 1 + e % 3] = small[e] * 2.0 ** -17                        # in the same four as a large one
+    x = torch.full((2, dim), 4096.0, dtype=DT[kind], device=DEV)
+    x[1] = -4096.0
+    router = torch.from_numpy(w.reshape(experts, dim)).to(torch.float32 if wide else DT[kind]).to(DEV)
+    exact = (x.double() @ router.double().T).cpu().numpy()
+    top = 8
+    ids, weights = pkg.moe.route(x, router, top)
+    for t in range(2):
+        order = np.argsort(-exact[t], kind="stable")[:top]
+        assert ids[t].tolist() == order.tolist()
+        p = np.exp(exact[t][order] - exact[t][order[0]])
+        assert np.abs(weights[t].cpu().numpy() / (p / p.sum()) - 1).max() <= 640 * U
+
+
+def test_scores_of_products_that_32_bits_do_not_hold(pkg):
+    """An fp32 router: products of 24 x 8 bits whose neighbours are equal once rounded to fp32."""
+    for experts in (8, 48):
+        order = np.random.default_rng(5).permutation(experts)
+        w = torch.zeros(experts, 16, device=DEV)
+        # 1.99 ... + e 2^-23 times 1.0078125: neighbours are 2^-23 apart, fp32 has steps of 2^-22 there
+        w[:, 0] = torch.from_numpy((np.float32(1.9921875) + order.astype(np.float32) * np.float32(2.0 ** -23)).astype(np.float32)).to(DEV)
+        w[:, 8] = -2.0
+        x = torch.zeros(1, 16, device=DEV, dtype=torch.bfloat16)
+        x[0, 0], x[0, 8] = 1.0078125, 1.0
+        ids, _ = pkg.moe.route(x, w, 8)
+        assert ids[0].tolist() == np.argsort(-order, kind="stable")[:8].tolist()
