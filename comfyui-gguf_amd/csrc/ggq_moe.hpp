@@ -16,7 +16,8 @@
 //     requested behind weights would wait for those weights.
 // A weight is the reference's value bit for bit (ggq_device.hpp: same decode, same fp16 operations, then the rounding to the activations' type).
 // The hidden vector act(g) * u is kept in two parts of the activations' type -- its rounded value and the rounded rest -- which ride as two columns of
-// the down product: about 16 (bf16) or 22 (fp16) bits, for no more weight traffic.  The fp16 rest is kept times 2^11, out of the subnormals.
+// the down product: about 16 (bf16) or 22 (fp16) bits, for no more weight traffic.  The fp16 rest is kept times 2^11, out of the subnormals; a value that fp16
+// does not hold is kept as a NaN that says what it is, and the columns that have one are added up again in fp32 (moe_big).
 // Measured, bf16: one token, two of 8 x 10240 x 4096 (Q4_K, down Q6_K): moe_up 36 us (2.6 TB/s of packed bytes), moe_down 28 (2.5); 33 tokens, fp16, two of 4 x 6848 x
 // 2432 (Q8_0, down Q5_0): 62 and 58 us.
 // Sums: fp32 in the MFMA's order, k-parts in wave order, experts in ascending order within a wave: the result does not depend on timing.
@@ -334,6 +335,60 @@ constexpr int MOE_WAVES = 8;
 // waves per SIMD that the registers are asked to leave room for: with one block of columns 4, two workgroups per CU
 #define MOE_OCC(MB) __attribute__((amdgpu_waves_per_eu((MB) == 1 ? 4 : 2, 8)))
 
+// Hidden values beyond fp16.  One of magnitude 65520 or more would round to infinity, and infinity and minus infinity as its two parts add up to NaN whatever the down
+// projection makes of it.  Such a value h is kept as
+//     first part   sign | 0x7E00 (a quiet NaN) | (exponent field of h - 142) << 2 | bits 21 and 22 of h        second part   bits 5 ... 20 of h
+// of h in fp32, rounded to 18 bits behind its point (2^-19 of it).  The matrix product of its column is a NaN then, which moe_down finds when it adds the column
+// up, at no cost to the others.  Infinities stay infinities, with a second part of 0; NaN is 0x7FFF.
+constexpr uint32_t MOE_FP16_TOP = 0x477FF000u;                                 // 65520 in fp32
+GGQ_DEV bool moe_is_big(float h) { return (__builtin_bit_cast(uint32_t, h) & 0x7FFFFFFFu) >= MOE_FP16_TOP; }
+GGQ_DEV void moe_keep_big(float h, uint32_t& hi, uint32_t& lo)
+{
+    const uint32_t bits = __builtin_bit_cast(uint32_t, h), sign = (bits >> 16) & 0x8000u;
+    uint32_t b = bits & 0x7FFFFFFFu;
+    if (b >= 0x7F800000u) {
+        hi = b > 0x7F800000u ? 0x7FFFu : sign | 0x7C00u;
+        lo = 0;
+        return;
+    }
+    b += 15u + ((b >> 5) & 1u);                                                // half to even
+    hi = sign | 0x7E00u | ((b >> 23) - 142u) << 2 | ((b >> 21) & 3u);
+    lo = (b >> 5) & 0xFFFFu;
+}
+GGQ_DEV float moe_hidden_f16(uint32_t hi, uint32_t lo)                         // the value of two parts
+{
+    if ((hi & 0x7E00u) != 0x7E00u) return (float)h_of(hi) + (float)h_of(lo) * (1.0f / 2048.0f);
+    const uint32_t exponent = (hi >> 2) & 127u;
+    return exponent == 127u ? __builtin_nanf("") : bits_f32((hi & 0x8000u) << 16 | (exponent + 142u) << 23 | (hi & 3u) << 21 | lo << 5);
+}
+
+// One hidden vector times 16 rows of packed weights, spans [s0, s1), in fp32: lane r, r + 16, r + 32, r + 48 share row r; the sum comes back in all of them.  For the few
+// columns that need it: straight from memory, element by element.  (33 tokens, two of four experts of 2 x 6848 x 2432 in fp16: the layer 123 us, 261 with such values in every token.)
+// `lane` is hidden from the compiler, so that nothing of this is computed ahead in registers of the loop that it stands in.
+template <class F>
+GGQ_DEV float moe_big(gcptr rows, uint64_t row_bytes, const GGQ_GLOBAL uint8_t* value, const GGQ_GLOBAL uint8_t* rest, uint32_t s0, uint32_t s1, uint32_t k_len, uint32_t lane)
+{
+    constexpr uint32_t CPB = F::BS / 8;
+    const uint32_t r = lane & 15u, c = lane >> 4;
+    const uint8_t* row = (const uint8_t*)(rows + r * row_bytes);
+    float sum = 0.0f;
+#pragma unroll 1
+    for (uint32_t j = s0 * 32u + c; j < s1 * 32u && j * 8u < k_len; j += 4u) {                             // chunks of 8 elements
+        const Fields f = F::template fields<false>(row + (uint64_t)(j / CPB) * F::TS, (int)(j % CPB));
+        uint32_t w[4];
+        weights8<F, OUT_F16>(f, w);
+        const u32x4 hi = *(GGQ_GLOBAL const u32x4*)(value + (uint64_t)j * 16u), lo = *(GGQ_GLOBAL const u32x4*)(rest + (uint64_t)j * 16u);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const h2 v = as_h2(w[i]);
+            sum += (float)v.x * moe_hidden_f16(hi[i] & 0xFFFFu, lo[i] & 0xFFFFu);
+            sum += (float)v.y * moe_hidden_f16(hi[i] >> 16, lo[i] >> 16);
+        }
+    }
+    sum += __builtin_bit_cast(float, __builtin_amdgcn_ds_bpermute((int)((lane ^ 16u) << 2), __builtin_bit_cast(int, sum)));
+    return sum + __builtin_bit_cast(float, __builtin_amdgcn_ds_bpermute((int)((lane ^ 32u) << 2), __builtin_bit_cast(int, sum)));
+}
+
 // this wave's list of the columns' places: `per` columns for each token of the expert; returns how many columns
 GGQ_DEV uint32_t moe_list(const MoeTable& s, const float* weights, const MoeArgs& a, int expert, uint32_t* slots, float* shares)
 {
@@ -488,6 +543,19 @@ __global__ __launch_bounds__(MOE_WAVES * 64) MOE_OCC(MB) void moe_up(const MoeAr
                             const h2 n{(_Float16)h0, (_Float16)h1};
                             hi[p] = as_u32(n);
                             lo[p] = as_u32(h2{(_Float16)__builtin_ldexpf(h0 - (float)n.x, 11), (_Float16)__builtin_ldexpf(h1 - (float)n.y, 11)});
+                            if (moe_is_big(h0) || moe_is_big(h1)) {
+                                uint32_t top, rest;
+                                if (moe_is_big(h0)) {
+                                    moe_keep_big(h0, top, rest);
+                                    hi[p] = (hi[p] & 0xFFFF0000u) | top;
+                                    lo[p] = (lo[p] & 0xFFFF0000u) | rest;
+                                }
+                                if (moe_is_big(h1)) {
+                                    moe_keep_big(h1, top, rest);
+                                    hi[p] = (hi[p] & 0xFFFFu) | top << 16;
+                                    lo[p] = (lo[p] & 0xFFFFu) | rest << 16;
+                                }
+                            }
                         } else {
                             hi[p] = pack_bf16(h0, h1);
                             lo[p] = pack_bf16(h0 - bits_f32(hi[p] << 16), h1 - bits_f32(hi[p] & 0xFFFF0000u));
@@ -539,7 +607,7 @@ __global__ __launch_bounds__(W * 64) MOE_OCC(MB) void moe_down(const MoeArgs a)
     const uint32_t n_spans = (a.ff + MF_SPAN - 1) / MF_SPAN, tail_len = a.ff - (n_spans - 1) * (uint32_t)MF_SPAN;
     const gcptr base = (gcptr)a.down + (uint64_t)row0 * row_bytes;
     const uint64_t items = (uint64_t)table.n * n_spans, share = blockIdx.y * W + wave, all = (uint64_t)a.parts * W;
-    const uint32_t first = (uint32_t)(items * share / all), last = (uint32_t)(items * (share + 1) / all);
+    const uint32_t first = (uint32_t)__builtin_amdgcn_readfirstlane((int)(items * share / all)), last = (uint32_t)__builtin_amdgcn_readfirstlane((int)(items * (share + 1) / all));
     uint8_t* ring = dyn + W * (a.tokens * 64u + a.spare * 1024u) + wave * a.ring * (uint32_t)G::SLICE;
     uint32_t* slots = slots_[wave];
     float* shares = shares_[wave];
@@ -557,7 +625,7 @@ __global__ __launch_bounds__(W * 64) MOE_OCC(MB) void moe_down(const MoeArgs a)
     request();
     if (a.ring > 2) request();
 
-    uint32_t item = first, nth = first / n_spans, span = first % n_spans, n_cols = 0, blocks = 0;
+    uint32_t item = first, nth = first / n_spans, span = first % n_spans, from = 0, n_cols = 0, blocks = 0;
     gcptr rows = base;
     const GGQ_GLOBAL uint8_t* col[MB];
     f32x4 acc[MB];
@@ -567,7 +635,8 @@ __global__ __launch_bounds__(W * 64) MOE_OCC(MB) void moe_down(const MoeArgs a)
     auto start = [&]() {                                                           // the columns of the next expert
         n_cols = 2u * moe_list(table, shares_all, a, table.list[nth], slots, shares);
         blocks = (n_cols + 15u) / 16u;
-        rows = base + (uint64_t)table.list[nth] * expert_bytes;
+        from = span;
+        rows = base + (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)table.list[nth]) * expert_bytes;
 #pragma unroll
         for (int mb = 0; mb < MB; mb++) {
             col[mb] = column((uint32_t)(mb * 16) + r);
@@ -600,19 +669,43 @@ __global__ __launch_bounds__(W * 64) MOE_OCC(MB) void moe_down(const MoeArgs a)
         span++;
     };
     // D[row = 4c + i][column = r]: value and rest are neighbouring lanes; the even one adds the token's share to its wave's y
-    auto add = [&](uint32_t q, f32x4 sum) {
+    // (anew: bit i: token i of the expert is to be added up anew, from its hidden values)
+    auto add = [&](uint32_t q, f32x4 sum, uint64_t& anew) {
         const uint32_t v = q * 16u + r;
+        bool fine = v < n_cols && (v & 1u) == 0;
+        if constexpr (OUT == OUT_F16) {
+            const float all = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            const uint64_t lanes = __ballot(v < n_cols && all != all);
+            if (lanes != 0) {
+                uint32_t bad = (uint32_t)lanes | (uint32_t)(lanes >> 32);
+                bad |= bad >> 16;
+                bad = (bad | bad >> 1) & 0x5555u;                                  // column 2 i, its own or its rest's
+                fine = fine && !((bad >> r) & 1u);
+                for (; bad != 0; bad &= bad - 1u) anew |= 1ull << (q * 8u + (uint32_t)__builtin_ctz(bad) / 2u);
+            }
+        }
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             float rest = dpp_f<0xB1, 0xF>(sum[i]);                                 // the neighbour's sum
             if constexpr (OUT == OUT_F16) rest *= 1.0f / 2048.0f;
-            if (v < n_cols && (v & 1u) == 0) part[slots[v >> 1] / a.top_k * 16u + 4u * c + (uint32_t)i] += shares[v >> 1] * (sum[i] + rest);
+            if (fine) part[slots[v >> 1] / a.top_k * 16u + 4u * c + (uint32_t)i] += shares[v >> 1] * (sum[i] + rest);
         }
     };
     auto finish = [&]() {
+        uint64_t anew = 0;
 #pragma unroll
-        for (int mb = 0; mb < MB; mb++) add((uint32_t)mb, acc[mb]);
-        for (uint32_t q = MB; q < blocks; q++) add(q, spare[(q - MB) * 64u + lane]);
+        for (int mb = 0; mb < MB; mb++) add((uint32_t)mb, acc[mb], anew);
+        for (uint32_t q = MB; q < blocks; q++) add(q, spare[(q - MB) * 64u + lane], anew);
+        if constexpr (OUT == OUT_F16) {
+            for (; anew != 0; anew &= anew - 1u) {
+                const uint32_t i = (uint32_t)__builtin_ctzll(anew), slot = slots[i];
+                const GGQ_GLOBAL uint8_t* value = (GGQ_GLOBAL const uint8_t*)a.hidden + (uint64_t)slot * a.ff * 2;
+                uint32_t at = lane;
+                asm volatile("" : "+v"(at));
+                const float y = moe_big<F>(rows, row_bytes, value, value + (uint64_t)pairs * a.ff * 2, from, span, a.ff, at);
+                if (at < 16u) part[slot / a.top_k * 16u + at] += shares[i] * y;
+            }
+        }
         wave_sync();
         nth++;
         span = 0;

@@ -277,8 +277,8 @@ uint64_t ggq_moe_route_workspace(uint32_t tokens, uint32_t experts);
  * contracts over them has 32-element blocks) up to 2^24.  An id outside [0, experts) adds nothing; the same id twice counts twice.  act: 0 silu, 1 gelu
  * (tanh form).  x, y: tokens x dim of `dtype` (GGQ_F16 / GGQ_BF16),
  * y 8-byte aligned.  workspace: ggq_moe_workspace() bytes, 16-byte aligned, used until the call's
- * kernels have run.  Sums in fp32; the hidden vector is kept in two parts of `dtype` (its value and what rounding left), fp16 hidden values above
- * 65504 overflow.  Deterministic.
+ * kernels have run.  Sums in fp32; the hidden vector is kept in two parts of `dtype` (its value and what rounding left: 16 bits
+ * of bf16, 22 of fp16), fp16 hidden values beyond 65504 with 19 bits; the columns that have one take longer.  Deterministic.
  * Replaces: one get_weight + F.linear (ops.py:242-244) per expert and projection. */
 typedef struct ggq_moe_desc {
     const void* x;

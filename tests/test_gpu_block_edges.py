@@ -3,7 +3,8 @@ import numpy as np
 import pytest
 import torch
 
-from test_gpu_moe import DT, Stack, U
+from test_gpu_linear import ALL
+from test_gpu_moe import DT, Stack, U, _act, _close, _want
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -92,3 +93,65 @@ def test_scores_of_products_that_32_bits_do_not_hold(pkg):
         x[0, 0], x[0, 8] = 1.0078125, 1.0
         ids, _ = pkg.moe.route(x, w, 8)
         assert ids[0].tolist() == np.argsort(-order, kind="stable")[:8].tolist()
+
+
+# ---- hidden values
+
+@pytest.mark.parametrize("tokens,experts,top_k", [(1, 3, 2), (20, 4, 2), (64, 3, 2)])
+@pytest.mark.parametrize("names", [("Q8_0", "Q8_0"), ("Q4_K", "Q6_K"), ("Q5_0", "IQ4_NL")])
+def test_fp16_hidden_values_beyond_fp16(pkg, tokens, experts, top_k, names):
+    """Hidden values up to 1e7 and beyond, where every result is far inside fp16; beside them tokens whose values are small, unchanged by the others.
+    A hidden value above 65504 is kept to 19 bits: 2^-19 of it, weighted, joins the bound."""
+    g = torch.Generator(device=DEV)
+    g.manual_seed(95)
+    dtype, dim, ff = torch.float16, 256, 512
+    gate, up = (Stack(pkg, names[0], (experts, ff, dim), "f16", 60 + i, shrink=0.25) for i in range(2))
+    down = Stack(pkg, names[1], (experts, dim, ff), "f16", 62, shrink=2.0 ** -9)
+    x = torch.randn(tokens, dim, device=DEV, generator=g) * 0.5
+    scale = 4000.0 / float((gate.dense[0] @ x[0].double()).abs().max())          # gate and up values of thousands
+    x[::2] *= scale
+    x = x.to(dtype)
+    ids = torch.stack([torch.randperm(experts, device=DEV, generator=g)[:top_k] for _ in range(tokens)]).int()
+    weights = torch.rand(tokens, top_k, device=DEV, generator=g)
+    weights[::2] *= 2.0 ** -6
+    want, bound = _want(x, ids, weights, gate.dense, up.dense, down.dense, "silu", dtype)
+    most = 0.0
+    for t in range(tokens):
+        for s in range(top_k):
+            i = int(ids[t, s])
+            h = _act(gate.dense[i] @ x[t].double(), "silu") * (up.dense[i] @ x[t].double())
+            most = max(most, float(h.abs().max()))
+            bound[t] += 2.0 ** -19 * float(weights[t, s]) * (down.dense[i].abs() @ (h.abs() * (h.abs() > 65000)))
+    assert most > 1e6 and float(want.abs().max()) < 30000
+    y = pkg.moe.moe_experts(x, ids, weights, gate.tensor, up.tensor, down.tensor)
+    _close(y, want, bound, dtype)
+    if tokens > 1:                                              # the tokens between: bit for bit what they are without the large ones
+        calm = x.clone()
+        calm[::2] = 0
+        assert torch.equal(pkg.moe.moe_experts(calm, ids, weights, gate.tensor, up.tensor, down.tensor)[1::2], y[1::2])
+
+
+@pytest.mark.parametrize("name", ALL)
+def test_fp16_hidden_values_beyond_fp16_in_every_format(pkg, name):
+    """The same for the down projection's formats, with short last spans in the 32-element ones; the shares bring the results back into fp16."""
+    g = torch.Generator(device=DEV)
+    g.manual_seed(96)
+    dtype = torch.float16
+    dim, ff = (192, 320) if pkg.qtypes.block_geometry(pkg.qtypes.Q[name])[0] == 32 else (256, 768)
+    gate, up = (Stack(pkg, "Q8_0", (3, ff, dim), "f16", 70 + i, shrink=0.25) for i in range(2))
+    down = Stack(pkg, name, (3, dim, ff), "f16", 72, shrink=0.25)
+    x = (torch.randn(5, dim, device=DEV, generator=g) * (3000.0 / (gate.dense.abs().mean() * dim ** 0.5).float())).to(dtype)
+    ids = torch.tensor([[0, 1], [1, 1], [2, 0], [-1, 2], [0, 2]], device=DEV, dtype=torch.int32)
+    most, bound, reach = 0.0, torch.zeros(5, dim, dtype=torch.float64, device=DEV), 0.0
+    for t in range(5):
+        for i in ids[t].tolist():
+            if i >= 0:
+                h = _act(gate.dense[i] @ x[t].double(), "silu") * (up.dense[i] @ x[t].double())
+                most, reach = max(most, float(h.abs().max())), max(reach, float((down.dense[i] @ h).abs().max()))
+                bound[t] += 2.0 ** -19 * (down.dense[i].abs() @ (h.abs() * (h.abs() > 65000)))
+    share = 2.0 ** float(np.floor(np.log2(10000.0 / reach)))
+    assert most > 1e6
+    weights = torch.full((5, 2), share, device=DEV)
+    want, base = _want(x, ids, weights, gate.dense, up.dense, down.dense, "silu", dtype)
+    y = pkg.moe.moe_experts(x, ids, weights, gate.tensor, up.tensor, down.tensor)
+    _close(y, want, base + share * bound, dtype)
