@@ -247,8 +247,14 @@ class GGMLMoE(torch.nn.Module):
             token, place = torch.nonzero(ids == expert, as_tuple=True)
             gate, up, down = (self._expert(w, expert, x.dtype) for w in (self.gate, self.up, self.down))
             rows = x[token]
-            out = torch.nn.functional.linear(act(torch.nn.functional.linear(rows, gate)) * torch.nn.functional.linear(rows, up), down)
-            y = y.index_add(0, token, out.float() * share[token, place][:, None])
+            left, right = torch.nn.functional.linear(rows, gate), torch.nn.functional.linear(rows, up)
+            part = share[token, place][:, None]
+            if x.dtype is torch.float16:                 # hidden values beyond 65504: |act(left)| <= |left|, so a power of two per row keeps them in range (1 for the others)
+                reach = left.detach().abs().amax(-1, keepdim=True).float() * right.detach().abs().amax(-1, keepdim=True).float()
+                down_by = torch.exp2(torch.ceil(torch.log2(reach / 32768)).clamp_min(0))
+                right, part = (right.float() / down_by).to(x.dtype), part * down_by
+            out = torch.nn.functional.linear(act(left) * right, down)
+            y = y.index_add(0, token, out.float() * part)
         return y.to(input.dtype).reshape(input.shape)
 
     @staticmethod

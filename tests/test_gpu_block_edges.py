@@ -155,3 +155,34 @@ def test_fp16_hidden_values_beyond_fp16_in_every_format(pkg, name):
     want, base = _want(x, ids, weights, gate.dense, up.dense, down.dense, "silu", dtype)
     y = pkg.moe.moe_experts(x, ids, weights, gate.tensor, up.tensor, down.tensor)
     _close(y, want, base + share * bound, dtype)
+
+
+def test_fp16_hidden_values_beyond_fp16_one_by_one(pkg):
+    """More than 64 tokens take the experts one by one: the same hidden values, in fp16 products.  Gate, up, activation, hidden and output are rounded to fp16: a few steps
+    of the largest magnitudes, as where nothing overflows.  Tokens that are in range get the bits that they get without the others."""
+    g = torch.Generator(device=DEV)
+    g.manual_seed(97)
+    gate, up = (Stack(pkg, "Q8_0", (3, 512, 256), "f16", 60 + i, shrink=0.25) for i in range(2))
+    down = Stack(pkg, "Q8_0", (3, 256, 512), "f16", 62, shrink=2.0 ** -13)
+    router = torch.randn(3, 256, device=DEV, generator=g) * 0.01
+    x = torch.randn(70, 256, device=DEV, generator=g)
+    x = x * (3000.0 / float((gate.dense[0] @ x[0].double()).abs().max()))
+    x[1::2] *= 2.0 ** -6
+    x = x.half()
+    layer = pkg.ops.GGMLMoE(router, gate.tensor, up.tensor, down.tensor, top_k=2)
+    hidden = _act(gate.dense[0] @ x[0].double(), "silu") * (up.dense[0] @ x[0].double())
+    assert float(hidden.abs().max()) > 1e6
+    slow, fast = layer(x), layer(x[:64])
+    assert bool(slow.isfinite().all()) and bool(fast.isfinite().all())
+    assert float((slow[:64].double() - fast.double()).norm() / fast.double().norm()) < 8 * torch.finfo(torch.float16).eps
+    calm = x.clone()
+    calm[::2] *= 2.0 ** -6
+    f = torch.nn.functional
+    want, same = torch.zeros(70, 256, device=DEV), layer(calm)
+    p, ids = torch.sort(torch.softmax(calm.float() @ router.t(), -1), dim=-1, descending=True, stable=True)
+    p, ids = p[:, :2] / p[:, :2].sum(-1, keepdim=True), ids[:, :2]
+    for e in range(3):
+        token, place = torch.nonzero(ids == e, as_tuple=True)
+        w = [s.dense[e].half() for s in (gate, up, down)]
+        want = want.index_add(0, token, f.linear(f.silu(f.linear(calm[token], w[0])) * f.linear(calm[token], w[1]), w[2]).float() * p[token, place][:, None])
+    assert torch.equal(same, want.half())
