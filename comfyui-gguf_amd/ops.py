@@ -221,7 +221,12 @@ class GGMLMoE(torch.nn.Module):
 
     def __init__(self, router, gate, up, down, top_k, renormalize=True, activation="silu"):
         super().__init__()
+        from .moe import ACTIVATIONS
+        if activation not in ACTIVATIONS:
+            raise ValueError(f"GGMLMoE: activations {sorted(ACTIVATIONS)}, got {activation!r}")
         router = dequantize_tensor(router, torch.float32) if is_quantized(router) else router
+        if not 1 <= top_k <= router.shape[0]:
+            raise ValueError(f"GGMLMoE: {top_k} of {router.shape[0]} experts")
         self.router = (router if type(router) is torch.Tensor else router.as_subclass(torch.Tensor)).float()      # one type for activations of any
         self.gate, self.up, self.down = gate, up, down
         self.top_k, self.renormalize, self.activation = top_k, renormalize, activation
