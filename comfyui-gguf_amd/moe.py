@@ -17,7 +17,7 @@ from . import _native
 from .dequant import GGQUnsupported, _HIP_TABLE, _OUT_CODE, _cur_device, _is_compiling, _qtype_key, _raw_stream
 from .norms import _on_gpu, _plain, _refuse_grad
 
-MAX_TOKENS, MAX_TOP_K, MAX_EXPERTS = 64, 16, 512
+MAX_TOKENS, MAX_TOP_K, MAX_EXPERTS, MAX_WIDTH = 64, 16, 512, 1 << 24
 ACTIVATIONS = {"silu": 0, "gelu_tanh": 1}
 _route_call = _experts_call = _workspace = None
 
@@ -91,24 +91,36 @@ def _stack(w, what, device):
     return qid, shape, w
 
 
-def _experts(x, ids, weights, gate, up, down, activation):
-    x = _rows16(x, "moe_experts")
-    _refuse_grad("moe_experts", x, weights)
+def _stacks(x, gate, up, down, activation):
+    """What is refused of x (rows as _rows16 gives them) and of the stacks, whatever the routes -> (experts, ff, their type ids, their bytes)."""
     if activation not in ACTIVATIONS:
         raise GGQUnsupported(f"moe_experts: activations {sorted(ACTIVATIONS)}")
     tokens, dim = x.shape
     if tokens > MAX_TOKENS:
         raise GGQUnsupported(f"moe_experts: at most {MAX_TOKENS} tokens, got {tokens}")
-    device = x.device
-    (gate_id, gate_shape, gate), (up_id, up_shape, up), (down_id, down_shape, down) = (_stack(w, name, device) for w, name in ((gate, "gate"), (up, "up"), (down, "down")))
+    (gate_id, gate_shape, gate), (up_id, up_shape, up), (down_id, down_shape, down) = (_stack(w, name, x.device) for w, name in ((gate, "gate"), (up, "up"), (down, "down")))
     experts, ff = up_shape[0], up_shape[1]
     if gate_id != up_id or gate_shape != up_shape or up_shape[2] != dim or down_shape != (experts, dim, ff):
         raise GGQUnsupported(f"moe_experts: gate and up of one type and shape (experts, ff, {dim}), down (experts, {dim}, ff); got {gate_shape}, {up_shape}, {down_shape}")
+    if not 1 <= experts <= MAX_EXPERTS or not 1 <= ff <= MAX_WIDTH or not 1 <= dim <= MAX_WIDTH:
+        raise GGQUnsupported(f"moe_experts: 1 ... {MAX_EXPERTS} experts, widths of 1 ... {MAX_WIDTH}")
+    return experts, ff, up_id, down_id, gate, up, down
+
+
+def _experts(x, ids, weights, gate, up, down, activation):
+    x = _rows16(x, "moe_experts")
+    _refuse_grad("moe_experts", x, weights)
+    return _run(x, ids, weights, _stacks(x, gate, up, down, activation), activation)
+
+
+def _run(x, ids, weights, stacks, activation):
+    experts, ff, up_id, down_id, gate, up, down = stacks
+    (tokens, dim), device = x.shape, x.device
     if ids.dim() != 2 or ids.shape != weights.shape or ids.shape[0] != tokens or ids.device != device or weights.device != device or ids.dtype not in (torch.int32, torch.int64):
         raise GGQUnsupported("moe_experts: ids (int32 / int64) and weights of shape (tokens, top_k) on x's device")
     top_k = ids.shape[1]
-    if not 1 <= top_k <= MAX_TOP_K or experts > MAX_EXPERTS or experts < 1 or ff < 1:
-        raise GGQUnsupported(f"moe_experts: 1 ... {MAX_TOP_K} experts per token of at most {MAX_EXPERTS}")
+    if not 1 <= top_k <= MAX_TOP_K:
+        raise GGQUnsupported(f"moe_experts: 1 ... {MAX_TOP_K} experts per token")
     y = torch.empty_like(x)
     if not tokens:
         return y
@@ -129,11 +141,12 @@ def _layer(x, router, gate, up, down, top_k, renormalize, activation):
     lead = x.shape
     if not lead or not lead[-1]:
         raise GGQUnsupported(f"moe_layer: rows of a tensor, got shape {tuple(lead)}")
-    x = x.reshape(-1, lead[-1]) if x.dim() != 2 else x
-    if x.shape[0] > MAX_TOKENS:
-        raise GGQUnsupported(f"moe_layer: at most {MAX_TOKENS} tokens, got {x.shape[0]}")
+    if x.numel() // lead[-1] > MAX_TOKENS:
+        raise GGQUnsupported(f"moe_layer: at most {MAX_TOKENS} tokens, got {x.numel() // lead[-1]}")
+    x = _rows16(x.reshape(-1, lead[-1]) if x.dim() != 2 else x, "moe_layer")
+    stacks = _stacks(x, gate, up, down, activation)              # refusals come before the router is launched
     ids, weights = _route(x, router, top_k, renormalize)
-    return _experts(x, ids, weights, gate, up, down, activation).reshape(lead)
+    return _run(x, ids, weights, stacks, activation).reshape(lead)
 
 
 # while torch.compile traces, the launches are a graph break: nothing in them can be traced

@@ -186,3 +186,30 @@ def test_fp16_hidden_values_beyond_fp16_one_by_one(pkg):
         w = [s.dense[e].half() for s in (gate, up, down)]
         want = want.index_add(0, token, f.linear(f.silu(f.linear(calm[token], w[0])) * f.linear(calm[token], w[1]), w[2]).float() * p[token, place][:, None])
     assert torch.equal(same, want.half())
+
+
+# ---- refusals
+
+def _small_mixture(pkg, experts=6):
+    g = torch.Generator(device=DEV)
+    g.manual_seed(98)
+    return (torch.randn(experts, 256, device=DEV, generator=g), *(Stack(pkg, "Q4_K", (experts, 256, 256), "f16", 80 + i, shrink=0.25).tensor for i in range(3)))
+
+
+def test_the_layer_refuses_before_it_launches(pkg, monkeypatch):
+    """What moe_experts refuses of the stacks, moe_layer refuses before the router has run."""
+    router, gate, up, down = _small_mixture(pkg)
+    x = torch.ones(3, 256, device=DEV, dtype=torch.float16)
+    pkg.moe._bind()
+
+    def launched(*args):
+        raise AssertionError("the router was launched")
+    monkeypatch.setattr(pkg.moe, "_route_call", launched)
+    with pytest.raises(AssertionError):
+        pkg.moe.moe_layer(x, router, gate, up, down, top_k=2)
+    G = pkg.ops.GGMLTensor
+    short = G(down.as_subclass(torch.Tensor)[:-144], tensor_type=down.tensor_type, tensor_shape=down.tensor_shape)
+    patched = G(down.as_subclass(torch.Tensor), tensor_type=down.tensor_type, tensor_shape=down.tensor_shape, patches=[1])
+    for stacks, kw in (((gate, up, short), {}), ((gate, up, patched), {}), ((gate, up, down.cpu()), {}), ((gate, up, gate.as_subclass(torch.Tensor)), {}), ((gate, up, down), {"activation": "relu"})):
+        with pytest.raises(pkg.dequant.GGQUnsupported):
+            pkg.moe.moe_layer(x, router, *stacks, top_k=2, **kw)
