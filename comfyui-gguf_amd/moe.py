@@ -145,6 +145,8 @@ def _layer(x, router, gate, up, down, top_k, renormalize, activation):
         raise GGQUnsupported(f"moe_layer: at most {MAX_TOKENS} tokens, got {x.numel() // lead[-1]}")
     x = _rows16(x.reshape(-1, lead[-1]) if x.dim() != 2 else x, "moe_layer")
     stacks = _stacks(x, gate, up, down, activation)              # refusals come before the router is launched
+    if router.shape[0] != stacks[0]:
+        raise GGQUnsupported(f"moe_layer: a router of {router.shape[0]} experts, stacks of {stacks[0]}")
     ids, weights = _route(x, router, top_k, renormalize)
     return _run(x, ids, weights, stacks, activation).reshape(lead)
 

@@ -227,6 +227,8 @@ class GGMLMoE(torch.nn.Module):
         router = dequantize_tensor(router, torch.float32) if is_quantized(router) else router
         if not 1 <= top_k <= router.shape[0]:
             raise ValueError(f"GGMLMoE: {top_k} of {router.shape[0]} experts")
+        if not router.shape[0] == gate.shape[0] == up.shape[0] == down.shape[0]:
+            raise ValueError(f"GGMLMoE: a router of {router.shape[0]} experts, stacks of {gate.shape[0]}, {up.shape[0]} and {down.shape[0]}")
         self.router = (router if type(router) is torch.Tensor else router.as_subclass(torch.Tensor)).float()      # one type for activations of any
         self.gate, self.up, self.down = gate, up, down
         self.top_k, self.renormalize, self.activation = top_k, renormalize, activation

@@ -213,3 +213,14 @@ def test_the_layer_refuses_before_it_launches(pkg, monkeypatch):
     for stacks, kw in (((gate, up, short), {}), ((gate, up, patched), {}), ((gate, up, down.cpu()), {}), ((gate, up, gate.as_subclass(torch.Tensor)), {}), ((gate, up, down), {"activation": "relu"})):
         with pytest.raises(pkg.dequant.GGQUnsupported):
             pkg.moe.moe_layer(x, router, *stacks, top_k=2, **kw)
+
+
+def test_a_router_of_other_experts_than_the_stacks(pkg):
+    """Ids beyond the stacks add nothing in moe_experts; a layer whose router has more (or fewer) experts than its stacks is a mistake."""
+    router, gate, up, down = _small_mixture(pkg)
+    x = torch.ones(3, 256, device=DEV, dtype=torch.float16)
+    for other in (router[:5], torch.cat((router, router))):
+        with pytest.raises(pkg.dequant.GGQUnsupported, match="router"):
+            pkg.moe.moe_layer(x, other, gate, up, down, top_k=2)
+        with pytest.raises(ValueError, match="router"):
+            pkg.ops.GGMLMoE(other, gate, up, down, top_k=2)
