@@ -20,11 +20,14 @@ What runs where
       the reference's own functions, which keep handling those cases.
 """
 import torch
+from torch.autograd import forward_ad as _forward_ad
 
 from . import _native
 from .qtypes import GGMLQuantizationType, GGML_QUANT_SIZES, HIP_QTYPES
 
 Q = GGMLQuantizationType
+
+_functorch = getattr(torch._C, "_functorch", None)
 
 TORCH_COMPATIBLE_QTYPES = (None, Q.F32, Q.F16)
 
@@ -60,6 +63,26 @@ def hip_supported(qtype):
 def _is_compiling():
     c = getattr(torch, "compiler", None)
     return bool(c and hasattr(c, "is_compiling") and c.is_compiling())
+
+
+def _transforms():
+    """(inside torch.func's vmap, inside another of its transforms)."""
+    if _functorch is None or _functorch.peek_interpreter_stack() is None:
+        return False, False
+    keys = [i.key() for i in _functorch.get_interpreter_stack()]
+    batched = [k == _functorch.TransformType.Vmap for k in keys]
+    return any(batched), not all(batched)
+
+
+def _transformed(*tensors):
+    """Whether a raw kernel launch would drop something of these tensors or cannot see their memory: a forward-mode tangent; a batch inside vmap; any tensor inside
+    jvp, grad and the like, where also those that the call makes are wrapped.  Outside of such calls this is two look-ups."""
+    batched, other = _transforms()
+    dual = _forward_ad._current_level >= 0
+    if not (batched or other or dual):
+        return False
+    return other or any(isinstance(t, torch.Tensor) and ((batched and _functorch.is_functorch_wrapped_tensor(t)) or (dual and _forward_ad.unpack_dual(t).tangent is not None))
+                        for t in tensors)
 
 
 def _as_bytes(data, align=True):

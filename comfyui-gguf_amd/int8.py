@@ -113,7 +113,7 @@ def _linear_int8(x, weight, weight_scale, bias, x_scale, out_dtype):
             raise GGQUnsupported("linear_int8: results in fp16 / bf16 / fp32")
         if x.device != device or k > MAX_DIM:
             raise GGQUnsupported(f"linear_int8: x on {x.device}, the weight on {device}; rows of at most {MAX_DIM} elements are quantized")
-    _refuse_grad("linear_int8", x, x_scale, weight_scale, bias)
+    _refuse_grad("linear_int8", x, x_scale, weight, weight_scale, bias)
     if x.dim() == 0 or x.shape[-1] != k:
         raise GGQUnsupported(f"linear_int8: rows of {k} elements for this weight")
     lead = x.shape[:-1]

@@ -83,6 +83,7 @@ def _stack(w, what, device):
     if len(shape) != 3:
         raise GGQUnsupported(f"moe_experts: {what} of shape (experts, rows, columns)")
     qid, block, size = ent
+    _refuse_grad("moe_experts", w)
     w = _plain(w)
     if w.device != device or w.dtype is not torch.uint8 or not w.is_contiguous() or w.data_ptr() & 15:
         raise GGQUnsupported(f"moe_experts: packed {what} must be a contiguous, 16-byte aligned byte tensor on {device}")
@@ -109,7 +110,7 @@ def _stacks(x, gate, up, down, activation):
 
 def _experts(x, ids, weights, gate, up, down, activation):
     x = _rows16(x, "moe_experts")
-    _refuse_grad("moe_experts", x, weights)
+    _refuse_grad("moe_experts", x, ids, weights)
     return _run(x, ids, weights, _stacks(x, gate, up, down, activation), activation)
 
 

@@ -16,7 +16,7 @@ import struct
 import torch
 
 from . import _native
-from .dequant import GGQUnsupported, _DEVICE_OK, _OUT_CODE, _cur_device, _device_served, _is_compiling, _raw_stream, dequantize_tensor, is_quantized
+from .dequant import GGQUnsupported, _DEVICE_OK, _OUT_CODE, _cur_device, _device_served, _is_compiling, _raw_stream, _transformed, dequantize_tensor, is_quantized
 
 NORMS = {None: 0, "none": 0, "rms": 1, "layer": 2}
 MAX_DIM = 32768                    # elements of a row: they live in the registers or the LDS of one workgroup
@@ -37,7 +37,9 @@ def _plain(t):
 
 
 def _on_gpu(x, what):
-    """x as a plain tensor on a served GPU, of a type that the row kernels take."""
+    """x as a plain tensor on a served GPU, of a type that the row kernels take, with memory of its own."""
+    if _transformed(x):
+        raise GGQUnsupported(f"{what}: inside a torch.func transform or forward-mode autograd -- torch's operations carry it on")
     if not isinstance(x, torch.Tensor) or not x.is_cuda or x.dtype not in _OUT_CODE:
         raise GGQUnsupported(f"{what}: fp16 / bf16 / fp32 tensors on the GPU")
     index = x.device.index
@@ -51,6 +53,8 @@ def _refuse_grad(what, *tensors):
         for t in tensors:
             if t is not None and t.requires_grad:
                 raise GGQUnsupported(f"{what}: autograd is recording -- torch's operations build the graph")
+    if _transformed(*tensors):
+        raise GGQUnsupported(f"{what}: inside a torch.func transform or forward-mode autograd -- torch's operations carry it on")
 
 
 def _vector(v, dim, dtype, device, what):

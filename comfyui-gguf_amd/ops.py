@@ -12,7 +12,7 @@ re-implemented here.
 """
 import torch
 
-from .dequant import dequantize_tensor, is_quantized
+from .dequant import _is_compiling, _transforms, dequantize_tensor, is_quantized
 
 
 class GGMLTensor(torch.Tensor):
@@ -249,19 +249,26 @@ class GGMLMoE(torch.nn.Module):
         if self.renormalize:
             share = share / share.sum(-1, keepdim=True)
         act = torch.nn.functional.silu if self.activation == "silu" else (lambda v: torch.nn.functional.gelu(v, approximate="tanh"))
-        y = torch.zeros(x.shape, dtype=torch.float32, device=x.device)
-        for expert in torch.unique(ids).tolist():
-            token, place = torch.nonzero(ids == expert, as_tuple=True)
+
+        def one(expert, rows, part):
+            """part * what one expert makes of rows, in 32 bits."""
             gate, up, down = (self._expert(w, expert, x.dtype) for w in (self.gate, self.up, self.down))
-            rows = x[token]
             left, right = torch.nn.functional.linear(rows, gate), torch.nn.functional.linear(rows, up)
-            part = share[token, place][:, None]
             if x.dtype is torch.float16:                 # hidden values beyond 65504: |act(left)| <= |left|, so a power of two per row keeps them in range (1 for the others)
                 reach = left.detach().abs().amax(-1, keepdim=True).float() * right.detach().abs().amax(-1, keepdim=True).float()
                 down_by = torch.exp2(torch.ceil(torch.log2(reach / 32768)).clamp_min(0))
                 right, part = (right.float() / down_by).to(x.dtype), part * down_by
-            out = torch.nn.functional.linear(act(left) * right, down)
-            y = y.index_add(0, token, out.float() * part)
+            return torch.nn.functional.linear(act(left) * right, down).float() * part
+
+        y = torch.zeros(x.shape, dtype=torch.float32, device=x.device)
+        if not _is_compiling() and any(_transforms()):   # inside torch.func's transforms ids cannot be read, and an expert's tokens not picked out: every expert for all
+            for expert in range(self.gate.shape[0]):
+                mine = ids == expert
+                y = y + torch.where(mine.any(-1, keepdim=True), one(expert, x, torch.where(mine, share, 0.0).sum(-1, keepdim=True)), 0.0)
+            return y.to(input.dtype).reshape(input.shape)
+        for expert in torch.unique(ids).tolist():
+            token, place = torch.nonzero(ids == expert, as_tuple=True)
+            y = y.index_add(0, token, one(expert, x[token], share[token, place][:, None]))
         return y.to(input.dtype).reshape(input.shape)
 
     @staticmethod
@@ -273,5 +280,6 @@ class GGMLMoE(torch.nn.Module):
             return plain.reshape(stack.shape)[expert].to(dtype)
         experts, rows, cols = stack.tensor_shape
         per = plain.numel() // experts
-        one = GGMLTensor(plain.reshape(-1)[expert * per:(expert + 1) * per].clone(), tensor_type=stack.tensor_type, tensor_shape=(rows, cols))
-        return dequantize_tensor(one, dtype)
+        with torch._C._DisableFuncTorch():               # a weight is the same inside torch.func's transforms, and has to have memory there
+            one = GGMLTensor(plain.reshape(-1)[expert * per:(expert + 1) * per].clone(), tensor_type=stack.tensor_type, tensor_shape=(rows, cols))
+            return dequantize_tensor(one, dtype)

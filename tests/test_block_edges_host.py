@@ -15,3 +15,46 @@ def test_a_mixture_that_is_not_one_is_refused_when_it_is_made(pkg, bad):
     layer = pkg.ops.GGMLMoE(torch.zeros(3, 4), *_stacks(), top_k=3, activation="gelu_tanh")
     x = torch.full((2, 4), 0.25)
     torch.testing.assert_close(layer(x), torch.full((2, 4), 8 * float(torch.nn.functional.gelu(torch.tensor(1.0), approximate="tanh"))))
+
+
+def test_tensors_that_a_launch_cannot_see_are_refused(pkg):
+    """A dual tensor's requires_grad is false; inside vmap a tensor has no memory of its own.  Others in the same call are what they were."""
+    from torch.autograd import forward_ad
+    refuse, no = pkg.norms._refuse_grad, pkg.dequant.GGQUnsupported
+    x = torch.ones(3, 4)
+    with torch.no_grad(), forward_ad.dual_level():
+        refuse("call", x, None, x[0])
+        for args in ((forward_ad.make_dual(x, x),), (x, None, forward_ad.make_dual(x, x))):
+            with pytest.raises(no, match="forward"):
+                refuse("call", *args)
+
+    def inside(v, alone=False):
+        if not alone:                                             # inside jvp the results of a call would be wrapped too
+            refuse("call", x)
+        with pytest.raises(no, match="transform"):
+            refuse("call", x, v)
+        with pytest.raises(no, match="transform"):
+            pkg.norms.block_norm(v)
+        return v
+    torch.vmap(inside)(x)
+    torch.func.jvp(lambda v: inside(v, True), (x,), (x,))
+    refuse("call", x)
+
+
+def test_experts_one_by_one_under_transforms(pkg):
+    """Forward-mode gradients against backward ones (in fp32: sums of up to 8 x 4 x 8 terms in another order, 2^-17), vmap against a loop."""
+    from torch.autograd import forward_ad
+    g = torch.Generator().manual_seed(5)
+    stacks = [torch.randn(s, generator=g) * 0.4 for s in ((3, 8, 4), (3, 8, 4), (3, 4, 8))]
+    layer = pkg.ops.GGMLMoE(torch.randn(3, 4, generator=g), *stacks, top_k=2)
+    x, v = torch.randn(5, 4, generator=g), torch.randn(5, 4, generator=g)
+    y, back = torch.autograd.functional.vjp(layer, x, torch.ones(5, 4))
+    with forward_ad.dual_level():
+        dual = forward_ad.unpack_dual(layer(forward_ad.make_dual(x, v)))
+    value, tangent = torch.func.jvp(layer, (x,), (v,))
+    for t in (dual.tangent, tangent):
+        assert abs(float(t.sum()) - float((back * v).sum())) <= 2.0 ** -17 * float((back * v).abs().sum())
+    assert torch.equal(dual.primal, y)
+    torch.testing.assert_close(value, y, rtol=2.0 ** -17, atol=2.0 ** -20)
+    many = torch.randn(6, 5, 4, generator=g)
+    torch.testing.assert_close(torch.vmap(layer)(many), torch.stack([layer(m) for m in many]), rtol=2.0 ** -17, atol=2.0 ** -20)

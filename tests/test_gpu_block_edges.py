@@ -224,3 +224,40 @@ def test_a_router_of_other_experts_than_the_stacks(pkg):
             pkg.moe.moe_layer(x, other, gate, up, down, top_k=2)
         with pytest.raises(ValueError, match="router"):
             pkg.ops.GGMLMoE(other, gate, up, down, top_k=2)
+
+
+def test_the_layers_under_transforms(pkg):
+    """Forward-mode gradients and vmap take the layers' torch operations: the tangent of an 8-bit linear is F.linear of the tangent, bit for bit; the calls themselves refuse."""
+    from torch.autograd import forward_ad
+    g = torch.Generator(device=DEV)
+    g.manual_seed(99)
+    no = pkg.dequant.GGQUnsupported
+    layer = pkg.ops.GGMLInt8Linear(torch.randn(48, 64, device=DEV, generator=g).half(), torch.randn(48, device=DEV, generator=g).half())
+    x, v = (torch.randn(3, 5, 64, device=DEV, generator=g).half() for _ in range(2))
+    dense = (layer.weight.float() * layer.weight_scale[:, None]).half()
+    f = torch.nn.functional
+    with torch.no_grad(), forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, v)
+        y = forward_ad.unpack_dual(layer(dual))
+        assert torch.equal(y.primal, f.linear(x, dense, layer.bias)) and torch.equal(y.tangent, f.linear(v, dense))
+        for call in (lambda: pkg.norms.block_norm(dual), lambda: pkg.norms.block_norm(x, scale=dual[0, 0]), lambda: pkg.int8.quantize_rows(dual), lambda: pkg.int8.linear_int8(x, layer.weight, layer.weight_scale, dual[0, 0, :48]),
+                     lambda: pkg.moe.route(dual[0], x[1, :3], 2)):
+            with pytest.raises(no, match="forward"):
+                call()
+        pkg.norms.block_norm(x)                                 # nothing in this one
+    _, tangent = torch.func.jvp(layer, (x,), (v,))
+    assert torch.equal(tangent, f.linear(v, dense))
+    torch.testing.assert_close(torch.vmap(layer)(x), f.linear(x, dense, layer.bias), rtol=2.0 ** -10, atol=2.0 ** -8)          # a batched product's sums in fp32, and two roundings
+
+    router, gate, up, down = _small_mixture(pkg)
+    mix = pkg.ops.GGMLMoE(router, gate, up, down, top_k=2)
+    x, v = (torch.randn(4, 3, 256, device=DEV, generator=g).half() * 0.5 for _ in range(2))
+    slow = torch.stack([mix._one_by_one(t) for t in x]).double()
+    near = 8 * torch.finfo(torch.float16).eps
+    assert float((torch.vmap(mix)(x).double() - slow).norm() / slow.norm()) < near
+    value, tangent = torch.func.jvp(mix, (x,), (v,))
+    assert float((value.double() - slow).norm() / slow.norm()) < near
+    leaf = x.clone().requires_grad_()
+    back, = torch.autograd.grad(mix(leaf).float().sum(), leaf)
+    pairs = back.double() * v.double()
+    assert abs(float(tangent.double().sum() - pairs.sum())) < 16 * torch.finfo(torch.float16).eps * (float(pairs.norm()) + float(tangent.double().norm()) * 4)
