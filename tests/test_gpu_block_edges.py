@@ -261,3 +261,24 @@ def test_the_layers_under_transforms(pkg):
     back, = torch.autograd.grad(mix(leaf).float().sum(), leaf)
     pairs = back.double() * v.double()
     assert abs(float(tangent.double().sum() - pairs.sum())) < 16 * torch.finfo(torch.float16).eps * (float(pairs.norm()) + float(tangent.double().norm()) * 4)
+
+
+@pytest.mark.parametrize("rows", [1, 20])
+def test_the_fused_linears_under_transforms(pkg, rows):
+    """The same for a packed linear with the fused kernels on: unpack + F.linear carries tangents and batches."""
+    from torch.autograd import forward_ad
+    g = torch.Generator(device=DEV)
+    g.manual_seed(100)
+    ops, q = pkg.ops, pkg.qtypes.Q.Q8_0
+    packed = torch.from_numpy(pkg.synth.make_tensor_bytes(q, (64, 256), seed=3, mode="signed")).to(DEV)
+    layer = ops.GGMLLinear(ops.GGMLTensor(packed, tensor_type=q, tensor_shape=(64, 256)))
+    layer.fuse_small_m, layer.fuse_mfma_max_m = True, 256
+    dense = pkg.dequant.dequantize_tensor(layer.weight, torch.float16)
+    x, v = (torch.randn(rows, 256, device=DEV, generator=g).half() for _ in range(2))
+    with torch.no_grad(), forward_ad.dual_level():
+        y = forward_ad.unpack_dual(layer(forward_ad.make_dual(x, v)))
+    f = torch.nn.functional
+    assert torch.equal(y.primal, f.linear(x, dense)) and torch.equal(y.tangent, f.linear(v, dense))
+    batch = torch.stack((x, v, x - v))
+    got, want = torch.vmap(layer)(batch), f.linear(batch.double(), dense.double())
+    assert float((got.double() - want).norm() / want.norm()) < 2 * torch.finfo(torch.float16).eps
