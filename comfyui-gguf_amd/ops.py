@@ -204,6 +204,13 @@ class GGMLInt8Linear(torch.nn.Module):
         self.register_buffer("weight_scale", scale)
         self.register_buffer("bias", bias)
 
+    def _apply(self, fn, recurse=True):
+        scale = self.weight_scale
+        super()._apply(fn, recurse)
+        if self.weight_scale.dtype is not torch.float32:         # .half() and the like cast the bias only: 16-bit scales are other weights
+            self.weight_scale = scale.to(self.weight_scale.device)
+        return self
+
     def forward(self, input):
         from .dequant import GGQUnsupported
         from .int8 import linear_int8

@@ -1,4 +1,6 @@
 """The block operators (norms, int8, moe and their layers) at the edges of what their documentation allows."""
+import copy
+
 import numpy as np
 import pytest
 import torch
@@ -282,3 +284,25 @@ def test_the_fused_linears_under_transforms(pkg, rows):
     batch = torch.stack((x, v, x - v))
     got, want = torch.vmap(layer)(batch), f.linear(batch.double(), dense.double())
     assert float((got.double() - want).norm() / want.norm()) < 2 * torch.finfo(torch.float16).eps
+
+
+# ---- layers that are cast, moved, copied and saved
+
+def _int8_layer(pkg, k=200):
+    g = torch.Generator(device=DEV)
+    g.manual_seed(101)
+    layer = pkg.ops.GGMLInt8Linear(torch.randn(40, k, device=DEV, generator=g), torch.randn(40, device=DEV, generator=g))
+    x = torch.randn(6, k, device=DEV, generator=g)
+    return layer, x
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_an_8_bit_layer_that_is_cast(pkg, dtype):
+    """Its scales stay in 32 bits and its result that of linear_int8: only the bias is cast."""
+    layer, x = _int8_layer(pkg)
+    want = pkg.int8.linear_int8(x.to(dtype), layer.weight, layer.weight_scale, layer.bias)
+    scale = layer.weight_scale.clone()
+    for cast in (lambda m: m.to(dtype), lambda m: m.half() if dtype is torch.float16 else m.bfloat16(), lambda m: m.to(DEV, dtype), lambda m: torch.nn.Sequential(m).to(dtype)[0]):
+        m = cast(copy.deepcopy(layer))
+        assert m.weight_scale.dtype is torch.float32 and torch.equal(m.weight_scale, scale) and m.bias.dtype is dtype
+        assert torch.equal(m(x.to(dtype)), want)
