@@ -209,6 +209,11 @@ class GGMLInt8Linear(torch.nn.Module):
         super()._apply(fn, recurse)
         if self.weight_scale.dtype is not torch.float32:         # .half() and the like cast the bias only: 16-bit scales are other weights
             self.weight_scale = scale.to(self.weight_scale.device)
+        if not self.weight.is_meta:
+            from .int8 import _rows8
+            laid_out = _rows8(self.weight, "weight", False)      # a move packs rows of odd widths: apart again, so that no call has to copy them
+            if laid_out is not self.weight:
+                self.weight = laid_out[:, :self.weight.shape[1]]
         return self
 
     def forward(self, input):

@@ -306,3 +306,26 @@ def test_an_8_bit_layer_that_is_cast(pkg, dtype):
         m = cast(copy.deepcopy(layer))
         assert m.weight_scale.dtype is torch.float32 and torch.equal(m.weight_scale, scale) and m.bias.dtype is dtype
         assert torch.equal(m(x.to(dtype)), want)
+
+
+def test_an_8_bit_layer_that_is_moved_copied_and_saved(pkg, monkeypatch):
+    """The layout that linear_int8 reads without a copy (rows of 200 bytes, 208 apart) survives; where it cannot, the result does."""
+    layer, x = _int8_layer(pkg)
+    want = layer(x)
+    elsewhere = layer.cpu()
+    assert elsewhere.weight.device.type == "cpu" and torch.equal(elsewhere(x.cpu()), torch.nn.functional.linear(x.cpu(), elsewhere.weight.float() * elsewhere.weight_scale[:, None], elsewhere.bias))
+    back = elsewhere.to(DEV)
+    copies = [back, copy.deepcopy(back), back.float()]
+    loaded, _ = _int8_layer(pkg)
+    loaded.weight.zero_()
+    loaded.load_state_dict(back.state_dict())
+    copies.append(loaded)
+    made = []
+    zeros = torch.zeros
+    monkeypatch.setattr(pkg.int8.torch, "zeros", lambda *a, **k: made.append(a) or zeros(*a, **k))
+    for m in copies:
+        assert m.weight.shape == (40, 200) and m.weight.stride() == (208, 1) and m.weight.dtype is torch.int8
+        assert torch.equal(m(x), want)
+    assert not made                                             # nothing was copied on a call
+    loaded.load_state_dict({k: v.contiguous() for k, v in back.state_dict().items()}, assign=True)
+    assert torch.equal(loaded(x), want)
