@@ -219,17 +219,19 @@ class GGMLInt8Linear(torch.nn.Module):
     def forward(self, input):
         from .dequant import GGQUnsupported
         from .int8 import linear_int8
+        weight, scale, bias = (t if t is None or t.device == input.device else t.to(input.device) for t in (self.weight, self.weight_scale, self.bias))
         try:
-            return linear_int8(input, self.weight, self.weight_scale, self.bias)
+            return linear_int8(input, weight, scale, bias)
         except GGQUnsupported:
-            weight = (self.weight.float() * self.weight_scale.float()[:, None]).to(input.dtype)
-            return torch.nn.functional.linear(input, weight, None if self.bias is None else self.bias.to(input.dtype))
+            weight = (weight.float() * scale[:, None]).to(input.dtype)
+            return torch.nn.functional.linear(input, weight, None if bias is None else bias.to(input.dtype))
 
 
 class GGMLMoE(torch.nn.Module):
     """A mixture-of-experts layer over packed expert stacks (moe.moe_layer): ``router`` (experts, dim); ``gate``, ``up`` (experts, ff, dim) and ``down``
-    (experts, dim, ff) are GGMLTensors of three dimensions.  What the fused kernels do not take -- more than 64 tokens, CPU tensors, a recording
-    autograd -- runs one expert after the other: get_weight + F.linear, the reference's way (ops.py:242-244)."""
+    (experts, dim, ff) are GGMLTensors of three dimensions, on any device: they come to the input's for the call, as a GGMLLayer's weight does.  What the fused
+    kernels do not take -- more than 64 tokens, CPU tensors, a recording autograd, torch.func's transforms -- runs one expert after the other: get_weight + F.linear,
+    the reference's way (ops.py:242-244), rounded to the input's type after each.  (Packed weights are unpacked on the GPU alone.)"""
 
     def __init__(self, router, gate, up, down, top_k, renormalize=True, activation="silu"):
         super().__init__()
@@ -247,15 +249,18 @@ class GGMLMoE(torch.nn.Module):
 
     def forward(self, input):
         from .dequant import GGQUnsupported
-        from .moe import moe_layer
+        from .moe import MAX_TOKENS, moe_layer
+        stacks = self.router, self.gate, self.up, self.down
+        if input.is_cuda and input.numel() <= MAX_TOKENS * input.shape[-1] and any(w.device != input.device for w in stacks):
+            stacks = [w.to(input.device) for w in stacks]        # weights that are kept elsewhere come over for the call, as GGMLLayer's do (ops.py:209)
         try:
-            return moe_layer(input, self.router, self.gate, self.up, self.down, top_k=self.top_k, renormalize=self.renormalize, activation=self.activation)
+            return moe_layer(input, *stacks, top_k=self.top_k, renormalize=self.renormalize, activation=self.activation)
         except GGQUnsupported:
             return self._one_by_one(input)
 
     def _one_by_one(self, input):
         x = input.reshape(-1, input.shape[-1])
-        scores = torch.softmax(x.float() @ self.router.float().t(), -1)
+        scores = torch.softmax(x.float() @ self.router.to(x.device).float().t(), -1)
         share, ids = torch.sort(scores, dim=-1, descending=True, stable=True)
         share, ids = share[:, :self.top_k], ids[:, :self.top_k]
         if self.renormalize:
@@ -264,7 +269,7 @@ class GGMLMoE(torch.nn.Module):
 
         def one(expert, rows, part):
             """part * what one expert makes of rows, in 32 bits."""
-            gate, up, down = (self._expert(w, expert, x.dtype) for w in (self.gate, self.up, self.down))
+            gate, up, down = (self._expert(w, expert, x.dtype, x.device) for w in (self.gate, self.up, self.down))
             left, right = torch.nn.functional.linear(rows, gate), torch.nn.functional.linear(rows, up)
             if x.dtype is torch.float16:                 # hidden values beyond 65504: |act(left)| <= |left|, so a power of two per row keeps them in range (1 for the others)
                 reach = left.detach().abs().amax(-1, keepdim=True).float() * right.detach().abs().amax(-1, keepdim=True).float()
@@ -284,14 +289,15 @@ class GGMLMoE(torch.nn.Module):
         return y.to(input.dtype).reshape(input.shape)
 
     @staticmethod
-    def _expert(stack, expert, dtype):
+    def _expert(stack, expert, dtype, device):
         if getattr(stack, "patches", None):
             raise ValueError("GGMLMoE: the experts are LoRA-patched; patches are not applied to a stack")
         plain = stack if type(stack) is torch.Tensor else stack.as_subclass(torch.Tensor)
         if not is_quantized(stack):
-            return plain.reshape(stack.shape)[expert].to(dtype)
+            return plain.reshape(stack.shape)[expert].to(device, dtype)
         experts, rows, cols = stack.tensor_shape
         per = plain.numel() // experts
         with torch._C._DisableFuncTorch():               # a weight is the same inside torch.func's transforms, and has to have memory there
-            one = GGMLTensor(plain.reshape(-1)[expert * per:(expert + 1) * per].clone(), tensor_type=stack.tensor_type, tensor_shape=(rows, cols))
-            return dequantize_tensor(one, dtype)
+            one = plain.reshape(-1)[expert * per:(expert + 1) * per].clone()
+            one = GGMLTensor(one if one.is_cuda else one.to(device), tensor_type=stack.tensor_type, tensor_shape=(rows, cols))
+            return dequantize_tensor(one, dtype).to(device)

@@ -329,3 +329,23 @@ def test_an_8_bit_layer_that_is_moved_copied_and_saved(pkg, monkeypatch):
     assert not made                                             # nothing was copied on a call
     loaded.load_state_dict({k: v.contiguous() for k, v in back.state_dict().items()}, assign=True)
     assert torch.equal(loaded(x), want)
+
+
+def test_layers_whose_weights_are_on_another_device(pkg):
+    """As with GGMLLayer, weights that are kept elsewhere come to the input: the result is what it is with the weights in place, in the kernels and one by one."""
+    G = pkg.ops.GGMLTensor
+    router, *stacks = _small_mixture(pkg)
+    away = [G(s.as_subclass(torch.Tensor).cpu(), tensor_type=s.tensor_type, tensor_shape=s.tensor_shape) for s in stacks]
+    here, there = pkg.ops.GGMLMoE(router, *stacks, top_k=2), pkg.ops.GGMLMoE(router.cpu(), *away, top_k=2)
+    g = torch.Generator(device=DEV)
+    g.manual_seed(102)
+    for tokens in (1, 64, 70):
+        x = torch.randn(tokens, 256, device=DEV, generator=g).half() * 0.5
+        assert torch.equal(there(x), here(x))
+    leaf = x.clone().requires_grad_()
+    assert torch.equal(torch.autograd.grad(there(leaf).float().sum(), leaf)[0], torch.autograd.grad(here(leaf).float().sum(), leaf)[0])
+    layer, x = _int8_layer(pkg)
+    want = layer(x)
+    assert torch.equal(copy.deepcopy(layer).cpu()(x), want)
+    dense = layer.weight.float() * layer.weight_scale[:, None]
+    assert torch.equal(layer(x.cpu()), torch.nn.functional.linear(x.cpu(), dense.cpu(), layer.bias.cpu()))
