@@ -260,11 +260,10 @@ class GGMLMoE(torch.nn.Module):
 
     def _one_by_one(self, input):
         x = input.reshape(-1, input.shape[-1])
-        scores = torch.softmax(x.float() @ self.router.to(x.device).float().t(), -1)
-        share, ids = torch.sort(scores, dim=-1, descending=True, stable=True)
-        share, ids = share[:, :self.top_k], ids[:, :self.top_k]
-        if self.renormalize:
-            share = share / share.sum(-1, keepdim=True)
+        scores = x.double() @ self.router.to(x.device).double().t()                   # moe.route in torch: which of two close scores is larger decides which experts run
+        ids = torch.sort(scores, dim=-1, descending=True, stable=True)[1][:, :self.top_k]
+        share = torch.softmax(scores, -1).gather(-1, ids)
+        share = (share / share.sum(-1, keepdim=True) if self.renormalize else share).float()
         act = torch.nn.functional.silu if self.activation == "silu" else (lambda v: torch.nn.functional.gelu(v, approximate="tanh"))
 
         def one(expert, rows, part):

@@ -181,8 +181,8 @@ def test_fp16_hidden_values_beyond_fp16_one_by_one(pkg):
     calm[::2] *= 2.0 ** -6
     f = torch.nn.functional
     want, same = torch.zeros(70, 256, device=DEV), layer(calm)
-    p, ids = torch.sort(torch.softmax(calm.float() @ router.t(), -1), dim=-1, descending=True, stable=True)
-    p, ids = p[:, :2] / p[:, :2].sum(-1, keepdim=True), ids[:, :2]
+    p, ids = torch.sort(torch.softmax(calm.double() @ router.double().t(), -1), dim=-1, descending=True, stable=True)
+    p, ids = (p[:, :2] / p[:, :2].sum(-1, keepdim=True)).float(), ids[:, :2]
     for e in range(3):
         token, place = torch.nonzero(ids == e, as_tuple=True)
         w = [s.dense[e].half() for s in (gate, up, down)]
@@ -349,3 +349,23 @@ def test_layers_whose_weights_are_on_another_device(pkg):
     assert torch.equal(copy.deepcopy(layer).cpu()(x), want)
     dense = layer.weight.float() * layer.weight_scale[:, None]
     assert torch.equal(layer(x.cpu()), torch.nn.functional.linear(x.cpu(), dense.cpu(), layer.bias.cpu()))
+
+
+@pytest.mark.parametrize("tokens", [64, 65])
+def test_a_layer_whose_scores_cancel(pkg, tokens, monkeypatch):
+    """The experts one by one are the experts that the kernels choose: scores that 32 bits do not tell apart, as in the router's own test."""
+    router, gate, up, down = _small_mixture(pkg, experts=8)
+    order = np.random.default_rng(6).permutation(8)
+    w = torch.zeros(8, 64, 4, device=DEV)
+    for e in range(8):
+        w[e, e, 0], w[e, 63 - e, 0] = 2.0 ** 18, -2.0 ** 18
+        w[e, e, 1] = float(order[e]) * 2.0 ** -9                 # products of 2^24 beside up to 7 * 2^-3
+    x = torch.full((tokens, 256), 64.0, device=DEV, dtype=torch.float16)
+    chosen = [int(i) for i in np.argsort(-order)[:2]]
+    layer = pkg.ops.GGMLMoE(w.view(8, 256), gate, up, down, top_k=2, renormalize=False)
+    ids, share = pkg.moe.route(x, w.view(8, 256), 2, renormalize=False)
+    assert ids.tolist() == [chosen] * tokens
+    ran, expert = set(), layer._expert
+    monkeypatch.setattr(layer, "_expert", lambda stack, e, *a: ran.add(e) or expert(stack, e, *a))
+    layer._one_by_one(x)
+    assert ran == set(chosen)
