@@ -33,7 +33,12 @@ def _bind():
 
 
 def _plain(t):
-    return t if type(t) is torch.Tensor else t.as_subclass(torch.Tensor)
+    """t without its subclass -- GGMLTensor's attributes go with it, so a patched one is refused."""
+    if type(t) is torch.Tensor:
+        return t
+    if getattr(t, "patches", None):
+        raise GGQUnsupported("LoRA-patched parameter: needs the reference's get_weight")
+    return t.as_subclass(torch.Tensor)
 
 
 def _on_gpu(x, what):
@@ -59,7 +64,7 @@ def _refuse_grad(what, *tensors):
 
 def _vector(v, dim, dtype, device, what):
     """A parameter of `dim` values as (tensor, is fp32)."""
-    if is_quantized(v):
+    if is_quantized(v) and not getattr(v, "patches", None):
         v = dequantize_tensor(v, torch.float32)
     v = _plain(v)
     if v.device != device or v.numel() != dim:

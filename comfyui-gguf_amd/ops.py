@@ -192,8 +192,8 @@ class GGMLInt8Linear(torch.nn.Module):
     def __init__(self, weight, bias=None):
         super().__init__()
         from .int8 import quantize_rows
-        if getattr(weight, "patches", None):
-            raise ValueError("GGMLInt8Linear: the weight is LoRA-patched; apply the patches first")
+        if getattr(weight, "patches", None) or getattr(bias, "patches", None):
+            raise ValueError("GGMLInt8Linear: the weight or bias is LoRA-patched; apply the patches first")
         dense = dequantize_tensor(weight, torch.float16) if is_quantized(weight) else weight
         dense = dense if type(dense) is torch.Tensor else dense.as_subclass(torch.Tensor)
         q, scale = quantize_rows(dense.detach())
@@ -238,6 +238,8 @@ class GGMLMoE(torch.nn.Module):
         from .moe import ACTIVATIONS
         if activation not in ACTIVATIONS:
             raise ValueError(f"GGMLMoE: activations {sorted(ACTIVATIONS)}, got {activation!r}")
+        if getattr(router, "patches", None):
+            raise ValueError("GGMLMoE: the router is LoRA-patched; apply the patches first")
         router = dequantize_tensor(router, torch.float32) if is_quantized(router) else router
         if not 1 <= top_k <= router.shape[0]:
             raise ValueError(f"GGMLMoE: {top_k} of {router.shape[0]} experts")

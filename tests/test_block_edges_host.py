@@ -58,3 +58,28 @@ def test_experts_one_by_one_under_transforms(pkg):
     torch.testing.assert_close(value, y, rtol=2.0 ** -17, atol=2.0 ** -20)
     many = torch.randn(6, 5, 4, generator=g)
     torch.testing.assert_close(torch.vmap(layer)(many), torch.stack([layer(m) for m in many]), rtol=2.0 ** -17, atol=2.0 ** -20)
+
+
+def test_patched_parameters_are_refused_everywhere(pkg):
+    """A LoRA patch on a norm's weight, a router or a bias is not dropped either: get_weight applies those (ops.py:183-190), the kernels do not."""
+    G, no = pkg.ops.GGMLTensor, pkg.dequant.GGQUnsupported
+    f32, q8 = pkg.qtypes.Q.F32, pkg.qtypes.Q.Q8_0
+    plain = G(torch.ones(64), tensor_type=f32, tensor_shape=(64,))
+    patched = G(torch.ones(64), tensor_type=f32, tensor_shape=(64,), patches=[("lora", "key")])
+    packed = torch.from_numpy(pkg.synth.make_tensor_bytes(q8, (1, 64), seed=1))
+    for good in (plain, torch.ones(64)):
+        v, is32 = pkg.norms._vector(good, 64, torch.float16, torch.device("cpu"), "weight")
+        assert type(v) is torch.Tensor and is32
+        assert pkg.norms._per_sample(good, (2, 3), 64, torch.float16, torch.device("cpu"), "gate", 1)[0].shape == (1, 64)
+    for bad in (patched, G(packed, tensor_type=q8, tensor_shape=(1, 64), patches=[("lora", "key")])):
+        with pytest.raises(no, match="patch"):
+            pkg.norms._vector(bad, 64, torch.float16, torch.device("cpu"), "weight")
+    with pytest.raises(no, match="patch"):
+        pkg.norms._per_sample(patched, (2, 3), 64, torch.float16, torch.device("cpu"), "gate", 1)
+    with pytest.raises(no, match="patch"):
+        pkg.norms._plain(patched)
+    router = G(torch.zeros(3, 4), tensor_type=f32, tensor_shape=(3, 4), patches=[("lora", "key")])
+    with pytest.raises(ValueError, match="patch"):
+        pkg.ops.GGMLMoE(router, *_stacks(), top_k=2)
+    with pytest.raises(ValueError, match="patch"):
+        pkg.ops.GGMLInt8Linear(torch.ones(64, 8), patched)
