@@ -33,13 +33,16 @@ hipError_t launch_rows16(const I8Args& a, hipStream_t s)
 template <int DT>
 hipError_t launch(const I8Args& a, hipStream_t s)
 {
-    if (a.m <= 16) return launch_rows16<DT, false>(a, s);
+    if (a.m <= 16 && launchable((a.n + 15u) / 16u, I8_ROW_WAVES * 64)) return launch_rows16<DT, false>(a, s);
     // The tile that finishes first: rounds of workgroups over the chip times what a step of 128 k takes, in ns.  Measured at 256 x 4096 x 4096 (a part of
     // the chip), 512 x 10240 x 4096 and 4608 x 10240 x 4096 (all of it, at the clock it holds then): 256 x 256 (128 KiB of LDS: one workgroup per CU) 1330 ...
-    // 1450 in one round, 1850 in several; 128 x 128 670 alone on a CU, 1050 for two; 64 x 64 350 alone, 420 for two.
+    // 1450 in one round, 1850 in several; 128 x 128 670 alone on a CU, 1050 for two; 64 x 64 350 alone, 420 for two.  A list of tiles that is too long for
+    // one launch does not finish.
     auto tiles = [&](uint64_t t) { return ((a.m + t - 1) / t) * ((a.n + t - 1) / t); };
-    const uint64_t t256 = tiles(256), t128 = tiles(128), t64 = tiles(64);
-    const uint64_t big = t256 <= 256 ? 1450 : (t256 + 255) / 256 * 1850, mid = t128 <= 256 ? 670 : (t128 + 511) / 512 * 1050, small = t64 <= 256 ? 350 : (t64 + 511) / 512 * 420;
+    const uint64_t t256 = tiles(256), t128 = tiles(128), t64 = tiles(64), never = ~0ull;
+    const uint64_t big = !launchable(t256, 512) ? never : t256 <= 256 ? 1450 : (t256 + 255) / 256 * 1850;
+    const uint64_t mid = !launchable(t128, 256) ? never : t128 <= 256 ? 670 : (t128 + 511) / 512 * 1050;
+    const uint64_t small = !launchable(t64, 256) ? never : t64 <= 256 ? 350 : (t64 + 511) / 512 * 420;
     if (small <= mid && small <= big) return launch_tile<DT, 64, 64, 1, 2, 2, 4>(a, s);
     if (mid < big) return launch_tile<DT, 128, 128, 2, 2, 1, 2>(a, s);
     return launch_tile<DT, 256, 256, 2, 4, 1, 2>(a, s);
@@ -55,7 +58,7 @@ extern "C" int ggq_linear_int8(const void* xq, uint64_t x_stride, const float* x
 {
     if (dtype < 0 || dtype > 2 || k == 0 || k > MAX_K) return GGQ_ERR_ARG;
     if (m == 0 || n == 0) return GGQ_OK;
-    if (((uint64_t)m + 63) / 64 * (((uint64_t)n + 63) / 64) > 0x7FFFFFFFull) return GGQ_ERR_ARG;      // workgroups of the smallest tile
+    if (m >= 1u << 31 || n >= 1u << 31 || !launchable(((uint64_t)m + 255) / 256 * (((uint64_t)n + 255) / 256), 512)) return GGQ_ERR_ARG;      // workgroups of the largest tile
     const uint64_t k16 = (k + 15u) & ~15u;
     if (!xq || !x_scale || !wq || !w_scale || !y || x_stride % 16 != 0 || w_stride % 16 != 0 || x_stride < k16 || w_stride < k16) return GGQ_ERR_ARG;
     if (!aligned16(xq) || !aligned16(wq) || unaligned(y, dtype) || unaligned(bias, dtype) || unaligned(x_scale, GGQ_F32) || unaligned(w_scale, GGQ_F32)) return GGQ_ERR_ALIGN;
@@ -69,7 +72,7 @@ extern "C" int ggq_linear_int8(const void* xq, uint64_t x_stride, const float* x
 extern "C" int ggq_linear_int8_few(const void* x, uint32_t m, const void* wq, uint64_t w_stride, const float* w_scale, uint32_t n, uint32_t k, const void* bias, void* y,
                                    int dtype, void* hip_stream)
 {
-    if (dtype < 0 || dtype > 2 || m > 16 || k == 0 || k % 8u != 0 || (uint64_t)m * k > (uint64_t)I8_FEW) return GGQ_ERR_ARG;
+    if (dtype < 0 || dtype > 2 || m > 16 || k == 0 || k % 8u != 0 || (uint64_t)m * k > (uint64_t)I8_FEW || !launchable(n / 16u + 1u, I8_ROW_WAVES * 64)) return GGQ_ERR_ARG;
     if (m == 0 || n == 0) return GGQ_OK;
     if (!x || !wq || !w_scale || !y || w_stride % 16 != 0 || w_stride < ((k + 15u) & ~15u)) return GGQ_ERR_ARG;
     if (!aligned16(x) || !aligned16(wq) || unaligned(y, dtype) || unaligned(bias, dtype) || unaligned(w_scale, GGQ_F32)) return GGQ_ERR_ALIGN;

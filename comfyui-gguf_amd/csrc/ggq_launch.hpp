@@ -8,6 +8,9 @@
 
 namespace ggq {
 
+// HIP takes fewer than 2^32 threads in one dimension of a launch.
+inline bool launchable(uint64_t blocks, uint32_t threads) { return blocks < (1ull << 32) / threads; }
+
 // Lets kernel `fn` take `bytes` of dynamic LDS on the current device; `raised` (one per kernel) remembers the devices it was done on.
 inline hipError_t allow_lds(const void* fn, int bytes, std::atomic<uint64_t>& raised)
 {

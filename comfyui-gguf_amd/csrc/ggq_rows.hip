@@ -22,7 +22,7 @@ int launch_rows(const RowArgs& a, int dtype, hipStream_t s)
     if (span > MAX_DIM) return GGQ_ERR_ARG;
     const uint32_t vecs = (uint32_t)((span + 7) / 8);
     if (vecs > (a.dim % 8 != 0 ? 512u : 1024u)) {
-        if (a.rows > 0x7FFFFFFFull) return GGQ_ERR_ARG;
+        if (!launchable(a.rows, ROW_LONG_THREADS)) return GGQ_ERR_ARG;
         static std::atomic<uint64_t> raised[3];
         hipError_t e = allow_lds(reinterpret_cast<const void*>(LONG_ROWS[dtype]), MAX_DIM * 4, raised[dtype]);
         if (e == hipSuccess) {
@@ -71,13 +71,15 @@ extern "C" int ggq_quantize_rows(const void* x, uint64_t rows, uint32_t cols, vo
     if (rows == 0) return GGQ_OK;
     if (!x || !q || !scale || cols == 0 || q_stride < cols || q_stride % 16 != 0) return GGQ_ERR_ARG;
     if (!aligned_to(x, dtype == GGQ_F32 ? 4 : 2) || !aligned_to(q, 16)) return GGQ_ERR_ALIGN;
-    if (q_stride <= 8192u && rows <= 0x7FFFFFFFull) {
+    const bool solo = q_stride <= 512u;
+    const uint64_t blocks = solo ? rows / 4 + (rows % 4 != 0) : rows;
+    const uint32_t threads = solo ? 256u : (uint32_t)((q_stride <= 8192u ? q_stride : 8192u) + 511u) / 512u * 64u;
+    if (q_stride <= 8192u && launchable(blocks, threads)) {                // more rows than that: dealt out to the teams that fit the chip
         typedef void (*quantize_fn)(const uint8_t*, uint64_t, uint32_t, uint8_t*, uint64_t, float*);
 #define GGQ_QUANTIZE(DT) {{quantize_rows<DT, true, false>, quantize_rows<DT, false, false>}, {quantize_rows<DT, true, true>, quantize_rows<DT, false, true>}}
         static const quantize_fn QUANTIZE[3][2][2] = {GGQ_QUANTIZE(OUT_F16), GGQ_QUANTIZE(OUT_BF16), GGQ_QUANTIZE(OUT_F32)};
-        const bool solo = q_stride <= 512u;
-        hipLaunchKernelGGL(QUANTIZE[dtype][cols % 8 != 0][solo ? 0 : 1], dim3((uint32_t)(solo ? (rows + 3) / 4 : rows)), dim3(solo ? 256u : (uint32_t)(q_stride + 511u) / 512u * 64u), 0,
-                           static_cast<hipStream_t>(hip_stream), static_cast<const uint8_t*>(x), rows, cols, static_cast<uint8_t*>(q), q_stride, scale);
+        hipLaunchKernelGGL(QUANTIZE[dtype][cols % 8 != 0][solo ? 0 : 1], dim3((uint32_t)blocks), dim3(threads), 0, static_cast<hipStream_t>(hip_stream), static_cast<const uint8_t*>(x),
+                           rows, cols, static_cast<uint8_t*>(q), q_stride, scale);
         const hipError_t e = hipGetLastError();
         return e == hipSuccess ? GGQ_OK : hip_fail(e);
     }

@@ -16,6 +16,7 @@ from .norms import MAX_DIM, _on_gpu, _plain, _refuse_grad
 
 MAX_K = 131071                     # |sum| <= 128 * 128 * k stays below 2^31
 FEW = 16384                        # elements of x up to which (and 16 rows) one launch does both: the kernels' I8_FEW
+FEW_ROWS = 16 * ((1 << 23) - 1)    # ... and fewer rows of the weight than this: a workgroup of 512 threads for 16 of them, 2^32 threads a launch
 _quantize_call = _linear_call = _few_call = None
 
 
@@ -32,6 +33,8 @@ def _launch(call, name, device, *args):
             rc = call(*args, _raw_stream(index))
     else:
         rc = call(*args, _raw_stream(index))
+    if rc == _native.GGQ_ERR_ARG:
+        raise GGQUnsupported(f"shape outside what {name} takes")
     if rc:
         _native.check(rc, name)
 
@@ -136,7 +139,7 @@ def _linear_int8(x, weight, weight_scale, bias, x_scale, out_dtype):
     x = _plain(x)
     if x.dtype is torch.int8:
         xq, x_scale = _rows8(x.reshape(m, k) if x.dim() != 2 else x, "x", True), x_scale.reshape(m).contiguous()
-    elif m <= 16 and m * k <= FEW and k % 8 == 0 and out_dtype is x.dtype:
+    elif m <= 16 and m * k <= FEW and k % 8 == 0 and out_dtype is x.dtype and n < FEW_ROWS:
         if not x.is_contiguous() or x.data_ptr() & 15:
             x = x.clone(memory_format=torch.contiguous_format)
         _launch(_few_call, "ggq_linear_int8_few", device, x.data_ptr(), m, weight.data_ptr(), weight.stride(0), weight_scale.data_ptr(), n, k,

@@ -169,6 +169,8 @@ def _block_norm(stream, branch, gate, post_norm, post_weight, norm, weight, bias
                 rc = call(desc, _raw_stream(index))
         else:
             rc = call(desc, _raw_stream(index))
+        if rc == _native.GGQ_ERR_ARG:
+            raise GGQUnsupported("shape outside what ggq_block_norm takes")
         if rc:
             _native.check(rc, "ggq_block_norm")
     return out, ((y, y_scale) if quantize else y)

@@ -218,7 +218,8 @@ uint64_t ggq_linear_mfma_workspace(int qtype, uint32_t rows, uint32_t cols, uint
  * the six may be NULL.  params_f32: bit i set = parameter i (order: post_weight, gate, weight, bias, scale, shift) holds fp32, else `dtype`.
  * y_scale NULL: y is rows x dim of `dtype`.  y_scale given: y is int8 rows y_stride BYTES apart (a multiple of 16, >= dim; bytes past dim are
  * written as 0) with y ~ q * y_scale[row], q = rint(127 y / max|row|), y_scale = max|row| / 127; a row with an infinity or a NaN: q = 0, scale NaN.
- * stream_out may be stream, y may be branch.  GGQ_ERR_ARG: rows longer than 32768 elements.  Arithmetic in fp32 from load to store.
+ * stream_out may be stream, y may be branch.  GGQ_ERR_ARG: rows longer than 32768 elements, or
+ * 2^22 rows and more that are longer than 8192 (4096 where dim is no multiple of 8).  Arithmetic in fp32 from load to store.
  * Replaces: nothing of the reference's own code -- the torch operations that the models it loads run between GGMLOps.Linear calls
  * (ops.py:242-244), and GGMLOps.LayerNorm (ops.py:262-266). */
 typedef struct ggq_norm_desc {
@@ -241,20 +242,21 @@ typedef struct ggq_norm_desc {
 int ggq_block_norm(const ggq_norm_desc* desc, void* hip_stream);
 
 /* Rows of `cols` values of `dtype` in 8 bits with one scale each: q[i, :] = rint(127 x[i, :] / max|x[i, :]|), scale[i] = max|x[i, :]| / 127; layout and
- * special rows as in ggq_block_norm.  Half-way quotients of 16-bit rows go to the even integer exactly. */
+ * special rows as in ggq_block_norm.  Half-way quotients of 16-bit rows go to the even integer exactly.  Limits as there. */
 int ggq_quantize_rows(const void* x, uint64_t rows, uint32_t cols, void* q, uint64_t q_stride, float* scale, int dtype, void* hip_stream);
 
 /* ---- product of 8-bit integers -------------------------------------------------------------------------------------------------------- */
 
 /* y[i, j] = (sum_k xq[i, k] wq[j, k]) * x_scale[i] * w_scale[j] + bias[j], i < m, j < n: xq int8 rows x_stride bytes apart, wq int8 rows w_stride bytes
  * apart (both multiples of 16, both arrays 16-byte aligned), scales fp32, bias (may be NULL) and y (m x n, contiguous) of `dtype`.  The integer sum
- * is exact (int32; k <= 131071: GGQ_ERR_ARG above); scale, bias and the one rounding to `dtype` in fp32.  Bytes past column k of a row are read (up to
+ * is exact (int32; k <= 131071, m and n < 2^31 with fewer than 2^23
+ * tiles of 256 x 256: GGQ_ERR_ARG above); scale, bias and the one rounding to `dtype` in fp32.  Bytes past column k of a row are read (up to
  * the next multiple of 16) but must be 0 in xq where k is no multiple of 16.
  * Replaces, for a weight kept in 8 bits: F.linear of GGMLOps.Linear.forward_ggml_cast_weights (ops.py:242-244). */
 int ggq_linear_int8(const void* xq, uint64_t x_stride, const float* x_scale, uint32_t m, const void* wq, uint64_t w_stride, const float* w_scale, uint32_t n,
                     uint32_t k, const void* bias, void* y, int dtype, void* hip_stream);
 
-/* The same for a few rows of x as they are: m <= 16 rows of `dtype`, m * k <= 16384 (GGQ_ERR_ARG above), contiguous, 16-byte aligned, k % 8 == 0; they are put into
+/* The same for a few rows of x as they are: m <= 16 rows of `dtype`, m * k <= 16384, n < 2^27 - 16 (GGQ_ERR_ARG above), contiguous, 16-byte aligned, k % 8 == 0; they are put into
  * 8 bits on the way, as ggq_quantize_rows does, and the result is that of the two calls. */
 int ggq_linear_int8_few(const void* x, uint32_t m, const void* wq, uint64_t w_stride, const float* w_scale, uint32_t n, uint32_t k, const void* bias, void* y,
                         int dtype, void* hip_stream);

@@ -83,3 +83,19 @@ def test_patched_parameters_are_refused_everywhere(pkg):
         pkg.ops.GGMLMoE(router, *_stacks(), top_k=2)
     with pytest.raises(ValueError, match="patch"):
         pkg.ops.GGMLInt8Linear(torch.ones(64, 8), patched)
+
+
+def test_more_rows_than_a_launch_takes_are_refused(pkg):
+    """At the C entries, before anything is launched (addresses that are never followed): fewer than 2^32 threads are one launch."""
+    import ctypes
+    n, A = pkg._native, 0x10000
+    L = n.lib()
+
+    def norm(**kw):
+        return L.ggq_block_norm(ctypes.byref(n.ggq_norm_desc(**{**dict(stream=A, y=A, rows=1 << 22, dim=8200, rows_per_mod=4, dtype=n.F16, norm=1, post_norm=0, eps=1e-6), **kw})), None)
+    assert norm() == n.GGQ_ERR_ARG and norm(dim=4097) == n.GGQ_ERR_ARG and norm(dim=32768, rows=1 << 40) == n.GGQ_ERR_ARG
+    for cols, stride, rows in ((8200, 8208, 1 << 22), (4105, 8208, 1 << 22), (32768, 32768, 1 << 33)):
+        assert L.ggq_quantize_rows(A, rows, cols, A, stride, A, n.F16, None) == n.GGQ_ERR_ARG
+    for m, rows in ((1 << 31, 1), (1, 1 << 31), ((1 << 32) - 1, 1), (1 << 25, 1 << 24), ((1 << 31) - 1, 257)):
+        assert L.ggq_linear_int8(A, 64, A, m, A, 64, A, rows, 64, None, A, n.F16, None) == n.GGQ_ERR_ARG, (m, rows)
+    assert L.ggq_linear_int8_few(A, 1, A, 64, A, 16 * ((1 << 23) - 1), 64, None, A, n.F16, None) == n.GGQ_ERR_ARG

@@ -369,3 +369,44 @@ def test_a_layer_whose_scores_cancel(pkg, tokens, monkeypatch):
     monkeypatch.setattr(layer, "_expert", lambda stack, e, *a: ran.add(e) or expert(stack, e, *a))
     layer._one_by_one(x)
     assert ran == set(chosen)
+
+
+# ---- more rows than one launch has threads for
+
+def test_quantized_rows_beyond_a_launch(pkg):
+    """2^26 rows and more, a wave each: the same as in two halves."""
+    rows, k = (1 << 26) + 5, 16
+    x = (torch.arange(rows, device=DEV, dtype=torch.int32) % 251).to(torch.bfloat16)[:, None] * torch.tensor([1.0, -0.5] * 8, device=DEV, dtype=torch.bfloat16)
+    x[:, 3] += 7
+    q, scale = pkg.int8.quantize_rows(x)
+    half = rows // 2
+    for part in (slice(0, half), slice(half, rows)):
+        a, b = pkg.int8.quantize_rows(x[part])
+        assert torch.equal(q[part], a) and torch.equal(scale[part], b)
+
+
+def test_products_beyond_a_launch(pkg):
+    """A weight of 2^27 rows for one row and for 20, x of 2^30 rows and more for one row of the weight: every 16 rows (64, with the tiles) took a workgroup."""
+    n = 1 << 27
+    w = torch.zeros(n, 16, dtype=torch.int8, device=DEV)
+    w[:, 0] = (torch.arange(n, device=DEV, dtype=torch.int32) % 127).to(torch.int8)
+    w[:, 5] = 1
+    scale = torch.ones(n, device=DEV)
+    x = torch.zeros(20, 16, device=DEV, dtype=torch.float16)
+    x[:, 0], x[:, 5] = 127, 3
+    x[7, 0] = 0
+    part = pkg.int8.linear_int8(x, w[:254], scale[:254])
+    for m in (1, 20):
+        y = pkg.int8.linear_int8(x[:m], w, scale)
+        assert y.shape == (m, n)
+        whole = n // 127 * 127
+        assert torch.equal(y[:, :whole].view(m, -1, 127), part[:m, None, :127].expand(m, whole // 127, 127)) and torch.equal(y[:, whole:], part[:m, :n - whole])
+    del y, w, scale
+    m = (1 << 30) + 70
+    q = torch.zeros(m, 16, dtype=torch.int8, device=DEV)
+    q[:, 2] = 5
+    q[-1, 2], q[1 << 30, 2] = 9, 11
+    y = pkg.int8.linear_int8(q, torch.full((1, 16), 2, dtype=torch.int8, device=DEV), torch.ones(1, device=DEV), x_scale=torch.ones(m, device=DEV), out_dtype=torch.float16)
+    assert y.shape == (m, 1) and float(y[-1]) == 18 and float(y[1 << 30]) == 22
+    y[-1] = y[1 << 30] = 10
+    assert bool((y == 10).all())
