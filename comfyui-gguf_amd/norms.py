@@ -100,6 +100,16 @@ def _per_sample(v, lead, dim, dtype, device, what, vectors):
     return v, v.stride(0), n, v.dtype is torch.float32
 
 
+def _rows_per_vector(rows, vectors):
+    """Rows that share a modulation vector, in the descriptor's 32 bits.  With one vector for all (stride 0) any number does: vector after vector is the same."""
+    per = max(rows // vectors, 1)
+    if per >> 32:
+        if vectors > 1:
+            raise GGQUnsupported(f"block_norm: {per} rows for each modulation vector, fewer than 2^32")
+        per = (1 << 32) - 1
+    return per
+
+
 def _block_norm(stream, branch, gate, post_norm, post_weight, norm, weight, bias, scale, shift, eps, quantize):
     stream = _on_gpu(stream, "block_norm")
     if stream.dim() == 0 or norm not in NORMS or post_norm not in NORMS:
@@ -163,7 +173,7 @@ def _block_norm(stream, branch, gate, post_norm, post_weight, norm, weight, bias
         index = device.index
         call = _call or _bind()
         desc = _PACK(stream.data_ptr(), at_branch, at_out, at_y, at_y_scale, at_post, at_gate, at_weight, at_bias, at_scale, at_shift,
-                     rows, gate_stride, scale_stride, shift_stride, y_stride, dim, max(rows // vectors, 1), flags, _OUT_CODE[dtype], kind, post_kind, eps)
+                     rows, gate_stride, scale_stride, shift_stride, y_stride, dim, _rows_per_vector(rows, vectors), flags, _OUT_CODE[dtype], kind, post_kind, eps)
         if _cur_device() != index:
             with torch.cuda.device(index):
                 rc = call(desc, _raw_stream(index))

@@ -99,3 +99,14 @@ def test_more_rows_than_a_launch_takes_are_refused(pkg):
     for m, rows in ((1 << 31, 1), (1, 1 << 31), ((1 << 32) - 1, 1), (1 << 25, 1 << 24), ((1 << 31) - 1, 257)):
         assert L.ggq_linear_int8(A, 64, A, m, A, 64, A, rows, 64, None, A, n.F16, None) == n.GGQ_ERR_ARG, (m, rows)
     assert L.ggq_linear_int8_few(A, 1, A, 64, A, 16 * ((1 << 23) - 1), 64, None, A, n.F16, None) == n.GGQ_ERR_ARG
+
+
+def test_rows_beyond_32_bits_per_modulation_vector(pkg):
+    """One vector for all rows is read for all of them, however many; the descriptor's field has 32 bits."""
+    per = pkg.norms._rows_per_vector
+    assert per(6, 1) == 6 and per(6, 3) == 2 and per(0, 1) == 1 and per(2, 2) == 1
+    assert per((1 << 32) - 1, 1) == (1 << 32) - 1
+    assert per(5 << 32, 1) == (1 << 32) - 1
+    assert per(5 << 32, 5 << 3) == 1 << 29
+    with pytest.raises(pkg.dequant.GGQUnsupported):
+        per(5 << 32, 5)

@@ -410,3 +410,18 @@ def test_products_beyond_a_launch(pkg):
     assert y.shape == (m, 1) and float(y[-1]) == 18 and float(y[1 << 30]) == 22
     y[-1] = y[1 << 30] = 10
     assert bool((y == 10).all())
+
+
+def test_norms_of_more_rows_than_32_bits_count(pkg):
+    rows = (1 << 32) + 6
+    x = torch.ones(rows, 1, device=DEV, dtype=torch.bfloat16)
+    x[-3:] = -2.0
+    x[1 << 32] = 0.0
+    r, y = pkg.norms.block_norm(x, scale=torch.full((1,), 2.0, device=DEV), eps=0.0625)
+    assert r.data_ptr() == x.data_ptr()
+    at = [0, (1 << 32) - 1, 1 << 32, (1 << 32) + 1, rows - 3, rows - 1]
+    want = [3 / 1.0625 ** 0.5] * 2 + [0.0, 3 / 1.0625 ** 0.5] + [-6 / 4.0625 ** 0.5] * 2
+    got = torch.stack([y[i, 0] for i in at]).double().cpu()
+    assert bool(((got - torch.tensor(want, dtype=torch.float64)).abs() <= 2.0 ** -8 * torch.tensor(want, dtype=torch.float64).abs()).all())
+    y[-3:], y[1 << 32] = y[0], y[0]
+    assert bool((y == y[0]).all())
