@@ -44,6 +44,14 @@ int launch_rows(const RowArgs& a, int dtype, hipStream_t s)
 
 bool aligned_to(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
+// Whether the rows of two arrays lie on one another, in part (`same`: or wholly).  A row is read before its own place is written, other rows may not be.
+bool on_one_another(const void* a, uint64_t a_row, const void* b, uint64_t b_row, uint64_t rows, bool same)
+{
+    if (!a || !b || (a == b && a_row == b_row && !same)) return false;
+    const unsigned __int128 p = reinterpret_cast<uintptr_t>(a), q = reinterpret_cast<uintptr_t>(b);
+    return p < q + (unsigned __int128)rows * b_row && q < p + (unsigned __int128)rows * a_row;
+}
+
 }  // namespace
 
 extern "C" int ggq_block_norm(const ggq_norm_desc* d, void* hip_stream)
@@ -58,6 +66,10 @@ extern "C" int ggq_block_norm(const ggq_norm_desc* d, void* hip_stream)
     const void* params[6] = {d->post_weight, d->gate, d->weight, d->bias, d->scale, d->shift};
     for (int i = 0; i < 6; i++)
         if (!aligned_to(params[i], (d->params_f32 >> i) & 1u ? 4 : eb)) return GGQ_ERR_ALIGN;
+    const uint64_t in_row = d->dim * eb, y_row = d->y_scale ? d->y_stride : in_row;
+    if (on_one_another(d->y, y_row, d->stream, in_row, d->rows, d->y_scale) || on_one_another(d->y, y_row, d->branch, in_row, d->rows, d->y_scale)) return GGQ_ERR_ARG;
+    if (d->branch && (on_one_another(d->stream_out, in_row, d->stream, in_row, d->rows, false) || on_one_another(d->stream_out, in_row, d->branch, in_row, d->rows, false) ||
+                      on_one_another(d->y, y_row, d->stream_out, in_row, d->rows, true))) return GGQ_ERR_ARG;
     auto b = [](const void* p) { return static_cast<const uint8_t*>(p); };
     RowArgs a{b(d->stream), b(d->branch), static_cast<uint8_t*>(d->stream_out), static_cast<uint8_t*>(d->y), d->y_scale, b(d->post_weight), b(d->gate), b(d->weight),
               b(d->bias), b(d->scale), b(d->shift), d->rows, d->gate_stride, d->scale_stride, d->shift_stride, d->y_stride, d->dim, d->rows_per_mod, d->params_f32,
@@ -71,6 +83,7 @@ extern "C" int ggq_quantize_rows(const void* x, uint64_t rows, uint32_t cols, vo
     if (rows == 0) return GGQ_OK;
     if (!x || !q || !scale || cols == 0 || q_stride < cols || q_stride % 16 != 0) return GGQ_ERR_ARG;
     if (!aligned_to(x, dtype == GGQ_F32 ? 4 : 2) || !aligned_to(q, 16)) return GGQ_ERR_ALIGN;
+    if (on_one_another(q, q_stride, x, (uint64_t)cols * (dtype == GGQ_F32 ? 4 : 2), rows, true)) return GGQ_ERR_ARG;
     const bool solo = q_stride <= 512u;
     const uint64_t blocks = solo ? rows / 4 + (rows % 4 != 0) : rows;
     const uint32_t threads = solo ? 256u : (uint32_t)((q_stride <= 8192u ? q_stride : 8192u) + 511u) / 512u * 64u;

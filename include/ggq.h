@@ -218,7 +218,8 @@ uint64_t ggq_linear_mfma_workspace(int qtype, uint32_t rows, uint32_t cols, uint
  * the six may be NULL.  params_f32: bit i set = parameter i (order: post_weight, gate, weight, bias, scale, shift) holds fp32, else `dtype`.
  * y_scale NULL: y is rows x dim of `dtype`.  y_scale given: y is int8 rows y_stride BYTES apart (a multiple of 16, >= dim; bytes past dim are
  * written as 0) with y ~ q * y_scale[row], q = rint(127 y / max|row|), y_scale = max|row| / 127; a row with an infinity or a NaN: q = 0, scale NaN.
- * stream_out may be stream, y may be branch.  GGQ_ERR_ARG: rows longer than 32768 elements, or
+ * stream_out may be stream or branch, y of `dtype` may be the one of the two that stream_out is not (or stream, without a branch); any other overlap of these
+ * arrays, and 8-bit rows over any of them, is GGQ_ERR_ARG.  GGQ_ERR_ARG: rows longer than 32768 elements, or
  * 2^22 rows and more that are longer than 8192 (4096 where dim is no multiple of 8).  Arithmetic in fp32 from load to store.
  * Replaces: nothing of the reference's own code -- the torch operations that the models it loads run between GGMLOps.Linear calls
  * (ops.py:242-244), and GGMLOps.LayerNorm (ops.py:262-266). */

@@ -110,3 +110,25 @@ def test_rows_beyond_32_bits_per_modulation_vector(pkg):
     assert per(5 << 32, 5 << 3) == 1 << 29
     with pytest.raises(pkg.dequant.GGQUnsupported):
         per(5 << 32, 5)
+
+
+def test_eight_bit_rows_do_not_go_over_the_inputs(pkg):
+    """y may be branch where its rows lie on branch's own; 8-bit rows do not, and another workgroup's would be gone before they are read."""
+    import ctypes
+    n, A = pkg._native, 0x100000
+    base = dict(stream=A, branch=2 * A, stream_out=A, y=3 * A, y_scale=4 * A, rows=4, dim=64, rows_per_mod=4, y_stride=64, dtype=n.F16, norm=1, post_norm=0, eps=1e-6)
+
+    def call(**kw):
+        return n.lib().ggq_block_norm(ctypes.byref(n.ggq_norm_desc(**{**base, **kw})), None)
+    row = 64 * 2
+    for y in (A, 2 * A, A + row, 2 * A + 3 * row, A - 64, 2 * A - 3 * 64, 2 * A - 64 - 48):
+        assert call(y=y) == n.GGQ_ERR_ARG, hex(y)
+    assert call(branch=None, stream_out=None, y=A) == n.GGQ_ERR_ARG
+    assert n.lib().ggq_quantize_rows(A, 4, 64, A, 64, 4 * A, n.F16, None) == n.GGQ_ERR_ARG
+    assert n.lib().ggq_quantize_rows(A, 4, 64, A + 3 * row, 64, 4 * A, n.F16, None) == n.GGQ_ERR_ARG
+    # 16-bit rows: on the input's own rows or apart from it, nothing between
+    for y in (A + row, 2 * A + row, 2 * A - 3 * row, A + 2, 2 * A + 16):
+        assert call(y=y, y_scale=None) == n.GGQ_ERR_ARG, hex(y)
+    for out in (A + row, 2 * A + row, 2 * A + 16):
+        assert call(stream_out=out) == n.GGQ_ERR_ARG, hex(out)
+    assert call(y=A, y_scale=None) == n.GGQ_ERR_ARG and call(y=5 * A, stream_out=5 * A, y_scale=None) == n.GGQ_ERR_ARG          # y on the stream that is stored

@@ -425,3 +425,20 @@ def test_norms_of_more_rows_than_32_bits_count(pkg):
     assert bool(((got - torch.tensor(want, dtype=torch.float64)).abs() <= 2.0 ** -8 * torch.tensor(want, dtype=torch.float64).abs()).all())
     y[-3:], y[1 << 32] = y[0], y[0]
     assert bool((y == y[0]).all())
+
+
+@pytest.mark.parametrize("rows,dim", [(5000, 256), (3000, 2432), (700, 4097), (40, 16384)])
+def test_outputs_on_the_inputs_at_the_c_entry(pkg, rows, dim):
+    """stream_out on stream and y on branch, or the other way round: what the call gives in arrays of their own."""
+    import ctypes
+    n = pkg._native
+    g = torch.Generator(device=DEV)
+    g.manual_seed(103)
+    stream, branch = (torch.randn(rows, dim, device=DEV, generator=g).bfloat16() for _ in range(2))
+    want_r, want_y = pkg.norms.block_norm(stream, branch, post_norm="layer", norm="rms")
+    for swap in (False, True):
+        s, b = stream.clone(), branch.clone()
+        out, y = (b, s) if swap else (s, b)
+        d = n.ggq_norm_desc(stream=s.data_ptr(), branch=b.data_ptr(), stream_out=out.data_ptr(), y=y.data_ptr(), rows=rows, dim=dim, rows_per_mod=rows, dtype=n.BF16, norm=1, post_norm=2, eps=1e-6)
+        assert n.lib().ggq_block_norm(ctypes.byref(d), torch.cuda.current_stream().cuda_stream) == n.GGQ_OK
+        assert torch.equal(out, want_r) and torch.equal(y, want_y)
