@@ -442,3 +442,30 @@ def test_outputs_on_the_inputs_at_the_c_entry(pkg, rows, dim):
         d = n.ggq_norm_desc(stream=s.data_ptr(), branch=b.data_ptr(), stream_out=out.data_ptr(), y=y.data_ptr(), rows=rows, dim=dim, rows_per_mod=rows, dtype=n.BF16, norm=1, post_norm=2, eps=1e-6)
         assert n.lib().ggq_block_norm(ctypes.byref(d), torch.cuda.current_stream().cuda_stream) == n.GGQ_OK
         assert torch.equal(out, want_r) and torch.equal(y, want_y)
+
+
+# ---- many tokens over many spans
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("tokens,experts,top_k", [(20, 8, 2), (33, 4, 2), (48, 8, 2), (64, 8, 2), (64, 16, 4)])
+@pytest.mark.parametrize("up_name,down_name,dim,ff", [("Q4_K", "Q6_K", 2048, 1280), ("Q8_0", "Q5_0", 2112, 1216)])
+def test_more_tokens_on_an_expert_than_columns_in_registers(pkg, kind, tokens, experts, top_k, up_name, down_name, dim, ff):
+    """Evenly spread routes, and all tokens on one expert, over as many pieces of k as every wave takes several of: the sums of the columns that the registers have no room for
+    are kept in LDS, for one matrix and for two."""
+    dtype = DT[kind]
+    g = torch.Generator(device=DEV)
+    g.manual_seed(104)
+    gate, up = (Stack(pkg, up_name, (experts, ff, dim), kind, 90 + i, shrink=0.125) for i in range(2))
+    down = Stack(pkg, down_name, (experts, dim, ff), kind, 92, shrink=0.125)
+    x = (torch.randn(tokens, dim, device=DEV, generator=g) * 0.25).to(dtype)
+    spread = torch.stack([torch.randperm(experts, device=DEV, generator=g)[:top_k] for _ in range(tokens)]).int()
+    one = spread.clone()
+    one[:, 0] = 1
+    one[:, 1] = torch.where(one[:, 1] == 1, -1, one[:, 1])
+    one[5:, 1:] = -1
+    weights = torch.rand(tokens, top_k, device=DEV, generator=g) + 0.25
+    for ids in (spread, one):
+        y = pkg.moe.moe_experts(x, ids, weights, gate.tensor, up.tensor, down.tensor)
+        want, bound = _want(x, ids, weights, gate.dense, up.dense, down.dense, "silu", dtype)
+        assert bool(want.isfinite().all()) and float(want.abs().max()) < 60000
+        _close(y, want, bound, dtype)
