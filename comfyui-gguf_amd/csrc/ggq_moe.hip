@@ -9,15 +9,7 @@ using namespace ggq;
 
 typedef hipError_t (*moe_fn)(MoeArgs, hipStream_t);
 
-// Slots of a wave's ring, given the rest of a workgroup's LDS: three where as many workgroups then still fit a CU (160 KiB) as with two.
 constexpr uint32_t HALF_LDS = 80u * 1024u, ALL_LDS = 160u * 1024u;
-uint32_t ring_slots(uint32_t rest, uint32_t waves, uint32_t slot_bytes)
-{
-    const uint32_t two = rest + waves * 2u * slot_bytes, three = rest + waves * 3u * slot_bytes;
-    if (three <= HALF_LDS) return 3u;
-    if (two <= HALF_LDS) return 2u;
-    return three <= ALL_LDS ? 3u : 2u;
-}
 
 template <class F, int OUT, int MB>
 hipError_t launch_up(MoeArgs a, hipStream_t s)
@@ -26,8 +18,7 @@ hipError_t launch_up(MoeArgs a, hipStream_t s)
     const uint32_t pairs = a.tokens * a.top_k, most = (pairs < a.experts ? pairs : a.experts) * (a.ff / 16u);      // tiles, if every pair chose another expert
     const uint32_t blocks = (a.tokens + 15u) / 16u;
     a.spare = blocks > (uint32_t)MB ? blocks - MB : 0u;
-    a.ring = ring_slots(fixed + MOE_WAVES * mats * a.spare * 1024u, MOE_WAVES, Mf16Geom<F>::SLICE);
-    const uint32_t lds = MOE_WAVES * (mats * a.spare * 1024u + a.ring * Mf16Geom<F>::SLICE);
+    const uint32_t lds = MOE_WAVES * (mats * a.spare * 1024u + MOE_RING * Mf16Geom<F>::SLICE);
     if (fixed + lds > ALL_LDS) return hipErrorInvalidConfiguration;
     static std::atomic<uint64_t> raised{0};
     const hipError_t e = allow_lds(reinterpret_cast<const void*>(&moe_up<F, OUT, MB>), (int)(ALL_LDS - fixed), raised);
@@ -52,8 +43,7 @@ hipError_t launch_down_w(MoeArgs a, hipStream_t s, bool& fits)
     const uint32_t blocks = (2u * a.tokens + 15u) / 16u;
     a.spare = blocks > (uint32_t)MB ? blocks - MB : 0u;
     const uint32_t sums = W * (a.tokens * 64u + a.spare * 1024u);
-    a.ring = ring_slots(fixed + sums, W, Mf16Geom<F>::SLICE);
-    const uint32_t lds = sums + W * a.ring * Mf16Geom<F>::SLICE;
+    const uint32_t lds = sums + W * MOE_RING * Mf16Geom<F>::SLICE;
     fits = fixed + lds <= ALL_LDS;
     if (!fits) return hipSuccess;
     static std::atomic<uint64_t> raised{0};
@@ -163,7 +153,7 @@ extern "C" int ggq_moe_experts(const ggq_moe_desc* d, void* hip_stream)
     if (!aligned16(d->x) || !aligned16(d->gate) || !aligned16(d->up) || !aligned16(d->down) || !aligned16(d->workspace) || !aligned4(d->ids) || !aligned4(d->weights) ||
         (reinterpret_cast<uintptr_t>(d->y) & 7u)) return GGQ_ERR_ALIGN;
     MoeArgs a{static_cast<const uint8_t*>(d->x), d->ids, d->weights, static_cast<const uint8_t*>(d->gate), static_cast<const uint8_t*>(d->up),
-              static_cast<const uint8_t*>(d->down), static_cast<uint8_t*>(d->y), static_cast<uint8_t*>(d->workspace), nullptr, d->tokens, d->top_k, d->experts, d->dim, d->ff, d->act, 1, 0, 2};
+              static_cast<const uint8_t*>(d->down), static_cast<uint8_t*>(d->y), static_cast<uint8_t*>(d->workspace), nullptr, d->tokens, d->top_k, d->experts, d->dim, d->ff, d->act, 1, 0};
     a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(d->workspace) + (((uint64_t)a.tokens * a.top_k * a.ff * 4u + 15u) & ~15ull));
     hipStream_t s = static_cast<hipStream_t>(hip_stream);
     hipError_t e = up->up[d->dtype][column_blocks(a.tokens, a.top_k, a.experts, 1)](a, s);

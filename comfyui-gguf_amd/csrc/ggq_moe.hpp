@@ -216,9 +216,12 @@ GGQ_DEV float moe_act(float g, int act)
     return g * __builtin_amdgcn_rcpf(1.0f + __expf(-2.0f * u));
 }
 
-// A wave's packed bytes go from memory straight into its own ring of LDS slots (LDS-DMA), one 256-element span of 16 rows per slot: row r at r * ROW_STRIDE, an
-// odd number of 16-byte units, from the aligned address below the row's span on (Mf16Geom).  With a ring of three slots two spans are on their way while one is
-// decoded, at no cost in registers; the launch takes two slots where three would leave one workgroup on a CU instead of two.
+// A wave's packed bytes go from memory straight into its own LDS slots (LDS-DMA), one 256-element span of 16 rows per slot: row r at r * ROW_STRIDE, an
+// odd number of 16-byte units, from the aligned address below the row's span on (Mf16Geom).  Two slots: the next span is on its way while one is decoded, at no cost
+// in registers.  (A third slot does not put a second span on its way: loads return in order, and the wait for a span's columns, which are requested after the span
+// behind it, is a wait for that span.  Measured: one token, two of 8 x 10240 x 4096 in Q4_K / Q6_K, bf16, 60.2 us with two slots, 60.7 with three; 7 tokens, eight of 64 x 1024 x 2048,
+// 63.2 and 64.6; 33 tokens, two of 4 x 6848 x 2432 in Q8_0 / Q5_0, 128.3 and 127.3.)
+constexpr uint32_t MOE_RING = 2;
 
 template <class F> struct MoeGeom {
     using G = Mf16Geom<F>;
@@ -328,7 +331,7 @@ struct MoeArgs {
     float* part;                     // [parts][tokens][dim]: moe_down's parts of y (parts > 1)
     uint32_t tokens, top_k, experts, dim, ff;
     int act;
-    uint32_t parts, spare, ring;     // spare: blocks of 16 columns beyond the kernel's MB that the tokens could fill (their sums live in LDS); ring: slots of a wave
+    uint32_t parts, spare;           // spare: blocks of 16 columns beyond the kernel's MB that the tokens could fill (their sums live in LDS)
 };
 
 constexpr int MOE_WAVES = 8;
@@ -414,7 +417,7 @@ template <class F, int OUT, int MB>
 __global__ __launch_bounds__(MOE_WAVES * 64) MOE_OCC(MB) void moe_up(const MoeArgs a)
 {
     using G = Mf16Geom<F>;
-    // per wave: the sums of columns beyond MB blocks ([spare][64] f32x4), then, for all waves, the rings
+    // per wave: the sums of columns beyond MB blocks ([spare][64] f32x4), then, for all waves, their slots
     extern __shared__ __attribute__((aligned(16))) uint8_t dyn[];
     __shared__ MoeTable table;
     __shared__ uint32_t slots_[MOE_WAVES][MOE_MAX_TOKENS];                         // per column: where its hidden row goes (= token * top_k + place)
@@ -433,7 +436,7 @@ __global__ __launch_bounds__(MOE_WAVES * 64) MOE_OCC(MB) void moe_up(const MoeAr
     // this wave's units of a tile: [u0, u1) in steps of `by`, unit u = span u / MATS of matrix u % 2 (or of the wave's own)
     const uint32_t u0 = MATS == 1 ? wave >> 1 : 2u * n_spans * wave / MOE_WAVES, u1 = MATS == 1 ? n_spans : 2u * n_spans * (wave + 1u) / MOE_WAVES, by = MATS == 1 ? MOE_WAVES / 2 : 1;
     auto is_up = [&](uint32_t u) { return MATS == 1 ? wave & 1u : u & 1u; };
-    uint8_t* ring = dyn + MOE_WAVES * MATS * a.spare * 1024u + wave * a.ring * (uint32_t)G::SLICE;
+    uint8_t* ring = dyn + MOE_WAVES * MATS * a.spare * 1024u + wave * MOE_RING * (uint32_t)G::SLICE;
     uint32_t* slots = slots_[wave];
     f32x4* spare = reinterpret_cast<f32x4*>(dyn) + (uint64_t)wave * MATS * a.spare * 64u;
     uint32_t turn = 0;
@@ -458,13 +461,12 @@ __global__ __launch_bounds__(MOE_WAVES * 64) MOE_OCC(MB) void moe_up(const MoeAr
             const uint32_t fs = fu / MATS;
             const bool tail = F::BS == 32 && fs + 1 == n_spans && tail_len != (uint32_t)MF_SPAN;
             moe_request<F>(weights_at(ft, fu), (uint32_t)row_bytes, fs, (tail ? tail_len : (uint32_t)MF_SPAN) / (uint32_t)F::BS * (uint32_t)F::TS, ring + in * G::SLICE);
-            in = in + 1 == a.ring ? 0 : in + 1;
+            in ^= 1u;
             fu += by;
             if (fu >= u1) { fu = u0; ft++; }
             return tail ? 1 : 2;
         };
         request();
-        if (a.ring > 2) request();
         f32x4 acc[MATS][MB];                                                       // acc[0]: of the matrix of this unit, acc[1] of the other
         auto clear = [&]() {
 #pragma unroll
@@ -485,7 +487,7 @@ __global__ __launch_bounds__(MOE_WAVES * 64) MOE_OCC(MB) void moe_up(const MoeAr
             if (request() == 2) moe_wait<(int)MoeGeom<F>::LOADS>();                // all but the span just requested
             else moe_wait<0>();
             uint8_t* slot = ring + out * G::SLICE;
-            out = out + 1 == a.ring ? 0 : out + 1;
+            out ^= 1u;
             const gcptr rows = weights_at(nth * tiles + tile, unit);
             if (F::BS == 32 && span + 1 == n_spans && tail_len != (uint32_t)MF_SPAN) moe_cut<F>(rows, (uint32_t)row_bytes, span, tail_len / (uint32_t)F::BS * (uint32_t)F::TS, slot);
             const uint32_t skew = G::SKEW ? moe_offset(rows, r, (uint32_t)row_bytes, span * G::SPAN_BYTES) & 15u : 0u;
@@ -587,7 +589,7 @@ template <class F, int OUT, int MB, int W>
 __global__ __launch_bounds__(W * 64) MOE_OCC(MB) void moe_down(const MoeArgs a)
 {
     using G = Mf16Geom<F>;
-    // y of each wave ([wave][token][16] floats), sums of columns beyond MB blocks ([wave][spare][64] f32x4), the rings
+    // y of each wave ([wave][token][16] floats), sums of columns beyond MB blocks ([wave][spare][64] f32x4), the slots
     extern __shared__ __attribute__((aligned(16))) uint8_t dyn[];
     __shared__ MoeTable table;
     __shared__ float shares_all[MOE_MAX_TOKENS * MOE_MAX_TOPK];
@@ -608,7 +610,7 @@ __global__ __launch_bounds__(W * 64) MOE_OCC(MB) void moe_down(const MoeArgs a)
     const gcptr base = (gcptr)a.down + (uint64_t)row0 * row_bytes;
     const uint64_t items = (uint64_t)table.n * n_spans, share = blockIdx.y * W + wave, all = (uint64_t)a.parts * W;
     const uint32_t first = (uint32_t)__builtin_amdgcn_readfirstlane((int)(items * share / all)), last = (uint32_t)__builtin_amdgcn_readfirstlane((int)(items * (share + 1) / all));
-    uint8_t* ring = dyn + W * (a.tokens * 64u + a.spare * 1024u) + wave * a.ring * (uint32_t)G::SLICE;
+    uint8_t* ring = dyn + W * (a.tokens * 64u + a.spare * 1024u) + wave * MOE_RING * (uint32_t)G::SLICE;
     uint32_t* slots = slots_[wave];
     float* shares = shares_[wave];
 
@@ -617,13 +619,12 @@ __global__ __launch_bounds__(W * 64) MOE_OCC(MB) void moe_down(const MoeArgs a)
         if (fi >= last) return 0;
         const bool tail = F::BS == 32 && fs + 1 == n_spans && tail_len != (uint32_t)MF_SPAN;
         moe_request<F>(base + (uint64_t)table.list[fn] * expert_bytes, (uint32_t)row_bytes, fs, (tail ? tail_len : (uint32_t)MF_SPAN) / (uint32_t)F::BS * (uint32_t)F::TS, ring + in * G::SLICE);
-        in = in + 1 == a.ring ? 0 : in + 1;
+        in ^= 1u;
         fi++;
         if (++fs == n_spans) { fs = 0; fn++; }
         return tail ? 1 : 2;
     };
     request();
-    if (a.ring > 2) request();
 
     uint32_t item = first, nth = first / n_spans, span = first % n_spans, from = 0, n_cols = 0, blocks = 0;
     gcptr rows = base;
@@ -652,7 +653,7 @@ __global__ __launch_bounds__(W * 64) MOE_OCC(MB) void moe_down(const MoeArgs a)
         if (request() == 2) moe_wait<(int)MoeGeom<F>::LOADS>();                    // all but the span just requested
         else moe_wait<0>();
         uint8_t* slot = ring + out * G::SLICE;
-        out = out + 1 == a.ring ? 0 : out + 1;
+        out ^= 1u;
         if (F::BS == 32 && span + 1 == n_spans && tail_len != (uint32_t)MF_SPAN) moe_cut<F>(rows, (uint32_t)row_bytes, span, tail_len / (uint32_t)F::BS * (uint32_t)F::TS, slot);
         const uint32_t skew = G::SKEW ? moe_offset(rows, r, (uint32_t)row_bytes, span * G::SPAN_BYTES) & 15u : 0u;
         moe_span<F, OUT, MB>(slot + r * G::ROW_STRIDE + skew, x, acc, [](int) {});
