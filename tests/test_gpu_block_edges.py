@@ -469,3 +469,103 @@ def test_more_tokens_on_an_expert_than_columns_in_registers(pkg, kind, tokens, e
         want, bound = _want(x, ids, weights, gate.dense, up.dense, down.dense, "silu", dtype)
         assert bool(want.isfinite().all()) and float(want.abs().max()) < 60000
         _close(y, want, bound, dtype)
+
+
+# ---- calls that stand for themselves
+
+def _q8_rows(pkg, values):
+    """A Q8_0 stack of one expert whose row j holds values[j] in column 0 (at most 127, whole) and values2[j] in column 1."""
+    first, second = values
+    rows = first.numel()
+    b = np.zeros((rows, 2, 34), dtype=np.uint8)
+    b[:, :, :2] = np.array([1.0], dtype=np.float16).view(np.uint8)
+    b[:, 0, 2] = first.numpy().astype(np.int8).view(np.uint8)
+    b[:, 0, 3] = second.numpy().astype(np.int8).view(np.uint8)
+    return pkg.ops.GGMLTensor(torch.from_numpy(b.reshape(-1)).to(DEV), tensor_type=pkg.qtypes.Q.Q8_0, tensor_shape=(1, rows, 64))
+
+
+def test_every_size_of_an_fp16_hidden_value(pkg):
+    """One hidden value per result: silu(g) u with g >= 40, where silu(g) is g to 2^-57.  g and u are products of two numbers of 11 bits, so exact in fp32; h is one fp32 product (and
+    the activation's reciprocal: 4 u), kept to 2^-22, or to 2^-19 beyond 65504, and y is half a step of share * h.  Values on both sides of 65520, where fp16 begins to
+    round to infinity, and up to 2^45, of either sign."""
+    g = torch.tensor([1, 2, 47, 61, 64, 100, 120, 127] * 8, dtype=torch.float32)
+    u = torch.tensor([1] * 8 + [-1] * 8 + [2] * 8 + [-3] * 8 + [16] * 8 + [-64] * 8 + [127] * 8 + [-127] * 8, dtype=torch.float32)
+    none = torch.zeros(64)
+    gate, up = _q8_rows(pkg, (g, none)), _q8_rows(pkg, (none, u))
+    b = np.zeros((64, 2, 34), dtype=np.uint8)
+    b[:, :, :2] = np.array([1.0], dtype=np.float16).view(np.uint8)
+    for i in range(64):
+        b[i, i // 32, 2 + i % 32] = 1
+    down = pkg.ops.GGMLTensor(torch.from_numpy(b.reshape(-1)).to(DEV), tensor_type=pkg.qtypes.Q.Q8_0, tensor_shape=(1, 64, 64))
+    x = torch.zeros(9, 64)
+    x[:, 0] = torch.tensor([1394.0, 546.0, 512.0, 40.0, 16384.0, 60000.0, 1071.0, 1092.0, 515.0])
+    x[:, 1] = torch.tensor([1.0, 1.0, 1.0, 1.0, 16384.0, 60000.0, 1.0, 0.5, 0.25])
+    want = (x[:, :1].double() * g.double()) * (x[:, 1:2].double() * u.double())
+    assert {65518.0, 65520.0, 65536.0} <= set(want.abs().flatten().tolist()) and float(want.abs().max()) > 2.0 ** 45
+    for share in (2.0 ** -31, 2.0 ** -12, 1.0):
+        y = pkg.moe.moe_experts(x.half().to(DEV), torch.zeros(9, 1, dtype=torch.int32, device=DEV), torch.full((9, 1), share, device=DEV), gate, up, down)
+        t = (share * want).abs()
+        fits = t < 65000
+        tol = t * (2.0 ** -11 + torch.where(want.abs() > 65504, 2.0 ** -19, 2.0 ** -22) + 8 * U) + 2.0 ** -25
+        err = (y.double().cpu() - share * want).abs()
+        assert bool((err <= tol)[fits].all()), float((err / tol)[fits].max())
+        assert torch.equal(y.cpu()[t > 66000], torch.sign(want[t > 66000]).half() * float("inf"))
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+def test_a_layer_of_many_experts_in_a_graph(pkg, kind):
+    """The router's two launches and its scratch, hidden values beyond fp16: captured once, replayed on other inputs between eager calls."""
+    dtype = DT[kind]
+    gate, up = (Stack(pkg, "Q4_K", (40, 256, 256), kind, 110 + i).tensor for i in range(2))
+    down = Stack(pkg, "Q6_K", (40, 256, 256), kind, 112, shrink=2.0 ** -10).tensor
+    g = torch.Generator(device=DEV)
+    g.manual_seed(105)
+    router = torch.randn(40, 256, device=DEV, generator=g) * 0.05
+    layer = pkg.ops.GGMLMoE(router, gate, up, down, top_k=3)
+    static = torch.randn(7, 256, device=DEV, generator=g).to(dtype)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        layer(static)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = layer(static)
+    for i in range(5):
+        new = (torch.randn(7, 256, device=DEV, generator=g) * (1.0, 30.0, 0.01, 100.0, 1.0)[i]).to(dtype)
+        static.copy_(new)
+        graph.replay()
+        kept = out.clone()
+        assert torch.equal(kept.nan_to_num(1.5), layer(new).nan_to_num(1.5)) and torch.equal(kept.isnan(), layer(new).isnan())
+        torch.cuda.synchronize()
+
+
+def test_the_longest_sums_in_every_kernel(pkg):
+    """131071 columns at the extremes, for few rows and for many: |sum| = 127 * 128 * 131071 = 0.99 * 2^31, the integers exact."""
+    k = 131071
+    for m, n in ((16, 5), (17, 70), (300, 260)):
+        q = torch.full((m, k), 127, dtype=torch.int8, device=DEV)
+        w = torch.full((n, k), -128, dtype=torch.int8, device=DEV)
+        w[1::2] = 127
+        w[0, :7] = 1
+        y = pkg.int8.linear_int8(q, w, torch.ones(n, device=DEV), x_scale=torch.ones(m, device=DEV), out_dtype=torch.float32)
+        want = w.long().sum(1).mul(127).float()
+        assert torch.equal(y, want[None].expand(m, n))
+
+
+@pytest.mark.parametrize("experts", [5, 20])
+def test_routes_of_as_many_tokens_as_a_call_takes(pkg, experts):
+    g = torch.Generator(device=DEV)
+    g.manual_seed(106)
+    x, w = torch.randn(65535, 8, device=DEV, generator=g).bfloat16(), torch.randn(experts, 8, device=DEV, generator=g).bfloat16()
+    ids, weights = pkg.moe.route(x, w, 3)
+    scores = x.double() @ w.double().t()                        # 8 exact products; their sums in 64 bits differ by the order of adding at most, 2^-50 of the terms
+    p, order = torch.sort(torch.softmax(scores, -1), dim=-1, descending=True, stable=True)
+    top = torch.sort(scores, dim=-1, descending=True)[0]
+    clear = (top.diff(dim=-1).abs()[:, :3] > 2.0 ** -49 * (x.double().abs() @ w.double().abs().t()).amax(-1, keepdim=True)).all(-1)
+    assert int(clear.sum()) > 65000 and torch.equal(ids[clear].long(), order[clear, :3])
+    want = p[:, :3] / p[:, :3].sum(-1, keepdim=True)
+    # |difference of scores| u for its rounding to fp32 (8 products of normal values: below 40), and 16 u for exp, reciprocal, sum and product
+    assert bool(((weights.double() - want).abs() <= want * 64 * U)[clear].all())
+    with pytest.raises(pkg.dequant.GGQUnsupported):
+        pkg.moe.route(torch.cat((x, x[:1])), w, 3)
