@@ -33,35 +33,35 @@ constexpr int MOE_WORDS = MOE_MAX_EXPERTS / 32;
 
 // ---- the router
 
-// Eight products and their sum in fp64: which of two close scores is larger decides which experts run.  A product of 24 x 11 bits is exact there, and that of two
-// bf16 values may leave fp32's range.  (One token, 8 experts x 4096 in bf16: the router 5.6 us, 3.9 with sums of four in fp32, which lose a small term beside a
-// large one.  fp16: 4.9; 4.7 with the products in fp32, where two fp16 values have room.)  RT: the router's type, fp32 in GGUF files.
-template <int OUT, int RT> GGQ_DEV double moe_dot8(const float (&u)[8], const uint8_t* w)
-{
-    float v[8];
-    double p[8];
-    row_load8<RT>(w, 0, 8, v);
-#pragma unroll
-    for (int k = 0; k < 8; k++) p[k] = (double)u[k] * (double)v[k];
-    return ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
-}
-
-// the score of one expert, by one wave, in every lane: pieces of 4 x 512 elements on their way at once
+// The score of one expert, by one wave, in every lane: pieces of 4 x 512 elements on their way at once.  Products and sums in fp64: which of two close scores is
+// larger decides which experts run.  A product of 24 x 11 bits is exact there, and that of two bf16 values may leave fp32's range.  RT: the router's type, fp32 in GGUF
+// files.  What bounds it is the latency of the loads: one token, 8 experts x 4096 in bf16, the router of a layer in turn with its experts takes 4.5 us, and 10.6 where the
+// compiler lets a piece's loads wait for the sums of the one before.
 template <int OUT, int RT> GGQ_DEV double moe_score(const uint8_t* x, const uint8_t* w, uint32_t dim)
 {
-    constexpr uint32_t RB = RT == OUT_F32 ? 4 : 2, U = 4;
+    constexpr uint32_t U = 4;
     double acc = 0.0;
     for (uint32_t i0 = (threadIdx.x & 63u) * 8u; i0 < dim; i0 += 512u * U) {
-        double d[U];
+        RowRaw<OUT> xs[U];
+        RowRaw<RT> ws[U];
 #pragma unroll
         for (uint32_t p = 0; p < U; p++) {
-            const uint32_t i = i0 + 512u * p < dim ? i0 + 512u * p : 0u;
-            float u[8];
-            row_load8<OUT>(x + (uint64_t)i * 2, 0, 8, u);
-            d[p] = moe_dot8<OUT, RT>(u, w + (uint64_t)i * RB);
+            const uint64_t i = i0 + 512u * p < dim ? i0 + 512u * p : 0u;       // past the end: the row's start, not added
+            xs[p] = row_raw<OUT, false>(x + i * 2u, 0, 8);
+            ws[p] = row_raw<RT, false>(w + i * (RT == OUT_F32 ? 4u : 2u), 0, 8);
         }
+        __builtin_amdgcn_sched_barrier(0);                                     // all of them before the first is used
 #pragma unroll
-        for (uint32_t p = 0; p < U; p++) acc += i0 + 512u * p < dim ? d[p] : 0.0;
+        for (uint32_t p = 0; p < U; p++) {
+            float u[8], v[8];
+            double d[8];
+            row_unpack<OUT>(xs[p], u);
+            row_unpack<RT>(ws[p], v);
+#pragma unroll
+            for (int k = 0; k < 8; k++) d[k] = (double)u[k] * (double)v[k];
+            const double sum = ((d[0] + d[1]) + (d[2] + d[3])) + ((d[4] + d[5]) + (d[6] + d[7]));
+            acc += i0 + 512u * p < dim ? sum : 0.0;
+        }
     }
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) acc += __shfl_xor(acc, off, 64);
