@@ -28,6 +28,7 @@ from .qtypes import GGMLQuantizationType, GGML_QUANT_SIZES, HIP_QTYPES
 Q = GGMLQuantizationType
 
 _functorch = getattr(torch._C, "_functorch", None)
+_transform_stack = getattr(_functorch, "peek_interpreter_stack", lambda: None)
 
 TORCH_COMPATIBLE_QTYPES = (None, Q.F32, Q.F16)
 
@@ -67,7 +68,7 @@ def _is_compiling():
 
 def _transforms():
     """(inside torch.func's vmap, inside another of its transforms)."""
-    if _functorch is None or _functorch.peek_interpreter_stack() is None:
+    if _transform_stack() is None:
         return False, False
     keys = [i.key() for i in _functorch.get_interpreter_stack()]
     batched = [k == _functorch.TransformType.Vmap for k in keys]
@@ -77,10 +78,10 @@ def _transforms():
 def _transformed(*tensors):
     """Whether a raw kernel launch would drop something of these tensors or cannot see their memory: a forward-mode tangent; a batch inside vmap; any tensor inside
     jvp, grad and the like, where also those that the call makes are wrapped.  Outside of such calls this is two look-ups."""
-    batched, other = _transforms()
     dual = _forward_ad._current_level >= 0
-    if not (batched or other or dual):
+    if not dual and _transform_stack() is None:
         return False
+    batched, other = _transforms()
     return other or any(isinstance(t, torch.Tensor) and ((batched and _functorch.is_functorch_wrapped_tensor(t)) or (dual and _forward_ad.unpack_dual(t).tangent is not None))
                         for t in tensors)
 

@@ -16,8 +16,8 @@ results are no further from exact than F.linear's (tools/fused_error.py, profile
 import torch
 
 from . import _native
-from .dequant import (GGQUnsupported, _DEVICE_OK, _HIP_TABLE, _OUT_CODE, _as_bytes, _cur_device, _dequantize_op, _device_served, _is_compiling, _qtype_key, _raw_stream,
-                      _transformed, dequantize_tensor, is_quantized)
+from .dequant import (GGQUnsupported, _DEVICE_OK, _HIP_TABLE, _OUT_CODE, _as_bytes, _cur_device, _dequantize_op, _device_served, _is_compiling, _qtype_key, _forward_ad, _raw_stream,
+                      _transform_stack, _transformed, dequantize_tensor, is_quantized)
 
 MAX_ROWS = 4
 _F16, _BF16 = torch.float16, torch.bfloat16
@@ -46,7 +46,7 @@ def _prepare(x, weight, bias, dequant_dtype, what, dtypes, need_cols_256):
         # the result of a raw kernel launch has no grad_fn; the reference's F.linear carries the gradient back to the input and the bias
         # (a LoRA-training node, gradient-based guidance): those calls keep dequantize + F.linear
         raise GGQUnsupported(f"{what}: autograd is recording -- dequantize + F.linear builds the graph")
-    if _transformed(x, bias):
+    if (_transform_stack() is not None or _forward_ad._current_level >= 0) and _transformed(x, bias):
         # nor has it a forward-mode tangent, or a batch of vmap's: the torch operations carry those
         raise GGQUnsupported(f"{what}: inside a torch.func transform or forward-mode autograd")
     if getattr(weight, "patches", None) or (bias is not None and getattr(bias, "patches", None)):

@@ -65,8 +65,8 @@ def quantize_rows(x):
 
 
 def _quantize_rows(x):
-    x = _on_gpu(x, "quantize_rows")
     _refuse_grad("quantize_rows", x)
+    x = _on_gpu(x, "quantize_rows")
     if x.dim() == 0 or not 1 <= x.shape[-1] <= MAX_DIM:
         raise GGQUnsupported(f"quantize_rows: rows of 1 ... {MAX_DIM} elements")
     lead, k = x.shape[:-1], x.shape[-1]
@@ -116,7 +116,7 @@ def _linear_int8(x, weight, weight_scale, bias, x_scale, out_dtype):
             raise GGQUnsupported("linear_int8: results in fp16 / bf16 / fp32")
         if x.device != device or k > MAX_DIM:
             raise GGQUnsupported(f"linear_int8: x on {x.device}, the weight on {device}; rows of at most {MAX_DIM} elements are quantized")
-    _refuse_grad("linear_int8", x, x_scale, weight, weight_scale, bias)
+    _refuse_grad("linear_int8", x, x_scale, weight_scale, bias, packed=(weight,))
     if x.dim() == 0 or x.shape[-1] != k:
         raise GGQUnsupported(f"linear_int8: rows of {k} elements for this weight")
     lead = x.shape[:-1]

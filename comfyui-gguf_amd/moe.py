@@ -52,8 +52,12 @@ def _with_device(device, call, name, *args):
 
 
 def _route(x, router, top_k, renormalize):
-    x, router = _rows16(x, "moe.route"), _rows16(router, "moe.route", True)
     _refuse_grad("moe.route", x, router)
+    return _run_route(_rows16(x, "moe.route"), router, top_k, renormalize)
+
+
+def _run_route(x, router, top_k, renormalize):
+    router = _rows16(router, "moe.route", True)
     tokens, dim = x.shape
     experts = router.shape[0]
     if router.shape[1] != dim or router.dtype not in (x.dtype, torch.float32) or router.device != x.device:
@@ -83,7 +87,6 @@ def _stack(w, what, device):
     if len(shape) != 3:
         raise GGQUnsupported(f"moe_experts: {what} of shape (experts, rows, columns)")
     qid, block, size = ent
-    _refuse_grad("moe_experts", w)
     w = _plain(w)
     if w.device != device or w.dtype is not torch.uint8 or not w.is_contiguous() or w.data_ptr() & 15:
         raise GGQUnsupported(f"moe_experts: packed {what} must be a contiguous, 16-byte aligned byte tensor on {device}")
@@ -109,8 +112,8 @@ def _stacks(x, gate, up, down, activation):
 
 
 def _experts(x, ids, weights, gate, up, down, activation):
+    _refuse_grad("moe_experts", x, weights, packed=(ids, gate, up, down))
     x = _rows16(x, "moe_experts")
-    _refuse_grad("moe_experts", x, ids, weights)
     return _run(x, ids, weights, _stacks(x, gate, up, down, activation), activation)
 
 
@@ -139,6 +142,7 @@ def _run(x, ids, weights, stacks, activation):
 
 
 def _layer(x, router, gate, up, down, top_k, renormalize, activation):
+    _refuse_grad("moe_layer", x, router, packed=(gate, up, down))
     lead = x.shape
     if not lead or not lead[-1]:
         raise GGQUnsupported(f"moe_layer: rows of a tensor, got shape {tuple(lead)}")
@@ -148,7 +152,7 @@ def _layer(x, router, gate, up, down, top_k, renormalize, activation):
     stacks = _stacks(x, gate, up, down, activation)              # refusals come before the router is launched
     if router.shape[0] != stacks[0]:
         raise GGQUnsupported(f"moe_layer: a router of {router.shape[0]} experts, stacks of {stacks[0]}")
-    ids, weights = _route(x, router, top_k, renormalize)
+    ids, weights = _run_route(x, router, top_k, renormalize)
     return _run(x, ids, weights, stacks, activation).reshape(lead)
 
 

@@ -16,7 +16,7 @@ import struct
 import torch
 
 from . import _native
-from .dequant import GGQUnsupported, _DEVICE_OK, _OUT_CODE, _cur_device, _device_served, _is_compiling, _raw_stream, _transformed, dequantize_tensor, is_quantized
+from .dequant import GGQUnsupported, _DEVICE_OK, _OUT_CODE, _cur_device, _device_served, _is_compiling, _forward_ad, _raw_stream, _transform_stack, _transformed, dequantize_tensor, is_quantized
 
 NORMS = {None: 0, "none": 0, "rms": 1, "layer": 2}
 MAX_DIM = 32768                    # elements of a row: they live in the registers or the LDS of one workgroup
@@ -42,9 +42,7 @@ def _plain(t):
 
 
 def _on_gpu(x, what):
-    """x as a plain tensor on a served GPU, of a type that the row kernels take, with memory of its own."""
-    if _transformed(x):
-        raise GGQUnsupported(f"{what}: inside a torch.func transform or forward-mode autograd -- torch's operations carry it on")
+    """x as a plain tensor on a served GPU, of a type that the row kernels take."""
     if not isinstance(x, torch.Tensor) or not x.is_cuda or x.dtype not in _OUT_CODE:
         raise GGQUnsupported(f"{what}: fp16 / bf16 / fp32 tensors on the GPU")
     index = x.device.index
@@ -53,12 +51,13 @@ def _on_gpu(x, what):
     return _plain(x)
 
 
-def _refuse_grad(what, *tensors):
+def _refuse_grad(what, *tensors, packed=()):
+    """Before anything asks a tensor for its memory: inside vmap it has none.  (packed: integers, which require no grad.)"""
     if torch.is_grad_enabled():
         for t in tensors:
             if t is not None and t.requires_grad:
                 raise GGQUnsupported(f"{what}: autograd is recording -- torch's operations build the graph")
-    if _transformed(*tensors):
+    if (_transform_stack() is not None or _forward_ad._current_level >= 0) and _transformed(*tensors, *packed):
         raise GGQUnsupported(f"{what}: inside a torch.func transform or forward-mode autograd -- torch's operations carry it on")
 
 
@@ -111,10 +110,10 @@ def _rows_per_vector(rows, vectors):
 
 
 def _block_norm(stream, branch, gate, post_norm, post_weight, norm, weight, bias, scale, shift, eps, quantize):
+    _refuse_grad("block_norm", stream, branch, gate, post_weight, weight, bias, scale, shift)
     stream = _on_gpu(stream, "block_norm")
     if stream.dim() == 0 or norm not in NORMS or post_norm not in NORMS:
         raise GGQUnsupported(f"block_norm: rows of a tensor, and norms of {sorted(k for k in NORMS if k)} or None")
-    _refuse_grad("block_norm", stream, branch, gate, post_weight, weight, bias, scale, shift)
     kind, post_kind = NORMS[norm], NORMS[post_norm]
     if branch is None and (gate is not None or post_kind or post_weight is not None):
         raise GGQUnsupported("block_norm: gate and post_norm act on branch, which is not given")
@@ -173,7 +172,7 @@ def _block_norm(stream, branch, gate, post_norm, post_weight, norm, weight, bias
         index = device.index
         call = _call or _bind()
         desc = _PACK(stream.data_ptr(), at_branch, at_out, at_y, at_y_scale, at_post, at_gate, at_weight, at_bias, at_scale, at_shift,
-                     rows, gate_stride, scale_stride, shift_stride, y_stride, dim, _rows_per_vector(rows, vectors), flags, _OUT_CODE[dtype], kind, post_kind, eps)
+                     rows, gate_stride, scale_stride, shift_stride, y_stride, dim, (rows // vectors or 1) if rows < 1 << 32 else _rows_per_vector(rows, vectors), flags, _OUT_CODE[dtype], kind, post_kind, eps)
         if _cur_device() != index:
             with torch.cuda.device(index):
                 rc = call(desc, _raw_stream(index))
