@@ -253,7 +253,9 @@ class GGMLMoE(torch.nn.Module):
         from .dequant import GGQUnsupported
         from .moe import MAX_TOKENS, moe_layer
         stacks = self.router, self.gate, self.up, self.down
-        if input.is_cuda and input.numel() <= MAX_TOKENS * input.shape[-1] and any(w.device != input.device for w in stacks):
+        with torch._C.DisableTorchFunctionSubclass():            # (a GGMLTensor's device asked for the long way is 4 us)
+            away = input.is_cuda and input.numel() <= MAX_TOKENS * input.shape[-1] and any(w.device != input.device for w in stacks)
+        if away:
             stacks = [w.to(input.device) for w in stacks]        # weights that are kept elsewhere come over for the call, as GGMLLayer's do (ops.py:209)
         try:
             return moe_layer(input, *stacks, top_k=self.top_k, renormalize=self.renormalize, activation=self.activation)
