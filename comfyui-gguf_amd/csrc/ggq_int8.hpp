@@ -64,8 +64,8 @@ struct I8Args {
 //
 // Measured (4608 x 9728 x 2432 / 4608 x 10240 x 4096, us): fragments read where they are used 151 / 206; tiles in groups of 4 rows of tiles (L2) 126 / 203; read one
 // piece ahead 130 / 193, interleaved 122 / 188; the branches for a partial last step out of the loop, so that the compiler counts the reads in flight
-// instead of waiting for all, 118 / 178 = 1840 / 2172 TOP/s (the library's int8 product on these shapes: 127 / 187).  4 waves of 128 x 128: 137 / 203; 64 bytes
-// of k and 4 buffers: 131 / 204.
+// instead of waiting for all, 118 / 178 = 1840 / 2172 TOP/s (in turn with the library's int8 product, which stores int32: 118 and
+// 118, 179 and 182; 512 x 10240 x 4096: 32 and 39).  4 waves of 128 x 128: 137 / 203; 64 bytes of k and 4 buffers: 131 / 204.
 template <int DT, int TM, int TN, int WM, int WN, int KS, int NB>
 __global__ __launch_bounds__(WM * WN * KS * 64) void linear_i8_tile(const I8Args a)
 {

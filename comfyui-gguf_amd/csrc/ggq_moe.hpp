@@ -70,7 +70,7 @@ template <int OUT, int RT> GGQ_DEV double moe_score(const uint8_t* x, const uint
 
 // The top_k experts of one token and their weights, from the scores in LDS; by the whole workgroup, which has a thread for every expert.  rank_[e] = how many
 // experts come before e.  A NaN comes last and makes all of the token's weights NaN, chosen or not: it is in the softmax's sum (rank_[experts]: whether there
-// is one).  The comparisons of an expert are split over the threads there are.
+// is one).  The comparisons of an expert are split over the threads there are.  Weights are fp32: exp of a difference of fp64 scores, v_exp_f32 and v_rcp_f32 within 2^-23.
 GGQ_DEV void moe_choose(const double* score, uint32_t* rank_, double* chosen, uint32_t experts, uint32_t top_k, int renormalize, int32_t* ids, float* weights)
 {
     const uint32_t padded = (experts + 63u) & ~63u, parts = blockDim.x / padded, t = threadIdx.x % padded, part = threadIdx.x / padded;
@@ -209,6 +209,7 @@ GGQ_DEV void moe_barrier()
     asm volatile("" ::: "memory");
 }
 
+// v_exp_f32 and v_rcp_f32 are within 2^-23 of their value, the exponent's argument within |g| 2^-24: as much as the sums that g comes from.
 GGQ_DEV float moe_act(float g, int act)
 {
     if (act == 0) return g * __builtin_amdgcn_rcpf(1.0f + __expf(-g));                                    // silu

@@ -33,7 +33,8 @@ int launch_rows(const RowArgs& a, int dtype, hipStream_t s)
     }
     const bool solo = vecs <= 64u;
     const uint32_t waves = solo ? 1u : (vecs + 63u) / 64u;
-    // as many teams as the chip holds at 16 waves per CU, each with as few rows as that leaves
+    // as many teams as the chip holds at 16 waves per CU, each with as few rows as that leaves.  (Where dim is no multiple of 8 the registers of fp16 rows, 170 and 161, and of
+    // short bf16 rows, 134, leave 8 ... 12 waves per CU: there the last teams run as a second round.)
     const uint64_t teams = 256u * 16u / waves, per = (a.rows + teams - 1) / teams;
     if (per > 0xFFFFFFFFull) return GGQ_ERR_ARG;
     const uint64_t need = (a.rows + per - 1) / per, grid = solo ? (need + 3) / 4 : need;

@@ -11,7 +11,7 @@
 // Everything between the loads and the stores is fp32 in registers: r is NOT rounded to the stream's type before it is normed (one rounding less than
 // separate kernels make), sums and squares are fp32, the variance is taken about the mean in a second pass over the registers.  The quotient 127 y / a is
 // formed in fp64 and rounded to fp32 before rint: in 16-bit rows |y| = a/2 is common and 63.5 has to be seen as exactly half-way, which a reciprocal in
-// fp32 misses; an fp32 product of two 24-bit values is not exact.
+// fp32 misses; an fp32 product of two 24-bit values is not exact.  (A norm's rows are fp32 and share the code.)
 //
 // What bounds it: HBM.  One pass: stream and branch are read once, r and y written once.  A row lives in the registers of one wave (short rows: no
 // barrier) or of the up to 16 waves of a workgroup, the longest in LDS.
@@ -283,7 +283,9 @@ GGQ_DEV void team_clear(float* red, uint32_t n)
 // is one wave, four teams to a workgroup, no barrier; else a team is a workgroup of up to 16 waves.  The next row's loads are under way while a row is
 // computed, and a sample's factors stay in registers from row to row (read for every row, they would be up to 14 bytes per element from the caches
 // beside the 8 from memory that the row itself moves).
-// Measured: 9216 x 4096 bf16, rms on either side, gate and modulation: 55 us, 5.5 TB/s (a large copy: 4.9); 666 x 2432 fp16, layer norm: 9.0 us; one row of 4096: 3.2 us.
+// Measured: 9216 x 4096 bf16, rms, gate and modulation: 54 us from a kernel's start to its end, 66 us a call back to back in a replayed graph = 4.6 TB/s (a large copy: 6.3);
+// 666 x 2432 fp16, layer norm: 9.1 us; one row of 4096: 3.3 us.  Rows of an odd number of elements go through the checks of every vector's end, in more registers: 36864 x 511
+// fp16 71 us (512: 36), 9216 x 4095 114, and 9216 x 4097 bf16, through LDS, 163 us.  8-bit rows: 4608 x 4096 35 us, 3.7 TB/s, where 16-bit ones move 4.6.
 template <int DT, bool SOLO, bool TAIL>
 __global__ __launch_bounds__(SOLO ? 256 : TAIL ? 512 : 1024) void block_norm(const RowArgs a, uint32_t rows_per_team)
 {

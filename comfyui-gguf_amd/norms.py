@@ -7,7 +7,7 @@ The models that the reference loads run these as separate torch operations aroun
 ``GGMLOps.LayerNorm``, ops.py:262-266).  Here r stays in fp32 registers between the sum and the norm.  ``quantize=True`` returns y as 8-bit rows with a
 scale each, ready for ``int8.linear_int8``.
 
-As the fused linears do, the call raises GGQUnsupported for what the kernel does not take (CPU tensors, other types, a recording autograd); the caller
+As the fused linears do, the call raises GGQUnsupported for what the kernel does not take (CPU tensors, other types, a recording autograd, torch.func's transforms); the caller
 keeps its torch operations then.
 """
 import ctypes

@@ -251,7 +251,8 @@ int ggq_quantize_rows(const void* x, uint64_t rows, uint32_t cols, void* q, uint
 /* y[i, j] = (sum_k xq[i, k] wq[j, k]) * x_scale[i] * w_scale[j] + bias[j], i < m, j < n: xq int8 rows x_stride bytes apart, wq int8 rows w_stride bytes
  * apart (both multiples of 16, both arrays 16-byte aligned), scales fp32, bias (may be NULL) and y (m x n, contiguous) of `dtype`.  The integer sum
  * is exact (int32; k <= 131071, m and n < 2^31 with fewer than 2^23
- * tiles of 256 x 256: GGQ_ERR_ARG above); scale, bias and the one rounding to `dtype` in fp32.  Bytes past column k of a row are read (up to
+ * tiles of 256 x 256: GGQ_ERR_ARG above); x_scale[i] * w_scale[j] (to be neither
+ * infinite nor subnormal), its product with the sum, the bias and the one rounding to `dtype` in fp32.  Bytes past column k of a row are read (up to
  * the next multiple of 16) but must be 0 in xq where k is no multiple of 16.
  * Replaces, for a weight kept in 8 bits: F.linear of GGMLOps.Linear.forward_ggml_cast_weights (ops.py:242-244). */
 int ggq_linear_int8(const void* xq, uint64_t x_stride, const float* x_scale, uint32_t m, const void* wq, uint64_t w_stride, const float* w_scale, uint32_t n,
