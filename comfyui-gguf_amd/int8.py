@@ -157,7 +157,8 @@ def linear_int8(x, weight, weight_scale, bias=None, *, x_scale=None, out_dtype=N
 
     x: (..., k) fp16 / bf16 / fp32 (put into 8 bits row by row), or int8 with ``x_scale`` (the leading dimensions of x, fp32) and ``out_dtype``.
     weight: int8 (n, k), weight_scale: fp32 (n,) -- what ``quantize_rows`` makes of a weight.  Rows of either that are not a multiple of 16 bytes apart, or
-    x rows in 8 bits whose k is no multiple of 16, are copied on every call.  The result has ``out_dtype`` (x's type unless given)."""
+    x rows in 8 bits whose k is no multiple of 16, are copied on every call.  The result has ``out_dtype`` (x's type unless given); a bias of
+    another type is rounded to it."""
     if _is_compiling():
         return _eager_linear(x, weight, weight_scale, bias, x_scale, out_dtype)
     return _linear_int8(x, weight, weight_scale, bias, x_scale, out_dtype)

@@ -12,7 +12,7 @@ re-implemented here.
 """
 import torch
 
-from .dequant import _is_compiling, _transforms, dequantize_tensor, is_quantized
+from .dequant import _is_compiling, _transform_stack, _transforms, dequantize_tensor, is_quantized
 
 
 class GGMLTensor(torch.Tensor):
@@ -264,32 +264,50 @@ class GGMLMoE(torch.nn.Module):
 
     def _one_by_one(self, input):
         x = input.reshape(-1, input.shape[-1])
-        scores = x.double() @ self.router.to(x.device).double().t()                   # moe.route in torch: which of two close scores is larger decides which experts run
-        ids = torch.sort(scores, dim=-1, descending=True, stable=True)[1][:, :self.top_k]
-        share = torch.softmax(scores, -1).gather(-1, ids)
-        share = (share / share.sum(-1, keepdim=True) if self.renormalize else share).float()
+        ids, share = self._route(x)
+        inside = not _is_compiling() and any(_transforms())      # of torch.func's transforms: no value can be looked at
+        y = self._sum_of_experts(x, ids, share, inside, inside and x.dtype is torch.float16)
+        if x.dtype is torch.float16 and not inside and not bool(y.isfinite().all()):
+            y = self._sum_of_experts(x, ids, share, inside, True)
+        return y.to(input.dtype).reshape(input.shape)
+
+    def _route(self, x):
+        """moe.route, in torch where it refuses: scores in 64 bits, as which of two close ones is larger decides which experts run."""
+        from .dequant import GGQUnsupported
+        from .moe import route
+        router = self.router if self.router.device == x.device else self.router.to(x.device)
+        try:
+            return route(x, router, self.top_k, renormalize=self.renormalize)
+        except GGQUnsupported:
+            scores = x.double() @ router.double().t()
+            ids = torch.sort(scores, dim=-1, descending=True, stable=True)[1][:, :self.top_k]
+            share = torch.softmax(scores, -1).gather(-1, ids)
+            return ids, (share / share.sum(-1, keepdim=True) if self.renormalize else share).float()
+
+    def _sum_of_experts(self, x, ids, share, every, in_range):
+        """The experts' results, weighted and added in 32 bits: each for its own tokens, or for all of them (every).  in_range: fp16 hidden values beyond 65504 are divided by a
+        power of two per row -- |act(left)| <= |left| -- which is 1 for the other rows: those have the same bits with and without."""
         act = torch.nn.functional.silu if self.activation == "silu" else (lambda v: torch.nn.functional.gelu(v, approximate="tanh"))
 
         def one(expert, rows, part):
-            """part * what one expert makes of rows, in 32 bits."""
             gate, up, down = (self._expert(w, expert, x.dtype, x.device) for w in (self.gate, self.up, self.down))
             left, right = torch.nn.functional.linear(rows, gate), torch.nn.functional.linear(rows, up)
-            if x.dtype is torch.float16:                 # hidden values beyond 65504: |act(left)| <= |left|, so a power of two per row keeps them in range (1 for the others)
+            if in_range:
                 reach = left.detach().abs().amax(-1, keepdim=True).float() * right.detach().abs().amax(-1, keepdim=True).float()
                 down_by = torch.exp2(torch.ceil(torch.log2(reach / 32768)).clamp_min(0))
                 right, part = (right.float() / down_by).to(x.dtype), part * down_by
             return torch.nn.functional.linear(act(left) * right, down).float() * part
 
         y = torch.zeros(x.shape, dtype=torch.float32, device=x.device)
-        if not _is_compiling() and any(_transforms()):   # inside torch.func's transforms ids cannot be read, and an expert's tokens not picked out: every expert for all
+        if every:
             for expert in range(self.gate.shape[0]):
                 mine = ids == expert
                 y = y + torch.where(mine.any(-1, keepdim=True), one(expert, x, torch.where(mine, share, 0.0).sum(-1, keepdim=True)), 0.0)
-            return y.to(input.dtype).reshape(input.shape)
+            return y
         for expert in torch.unique(ids).tolist():
             token, place = torch.nonzero(ids == expert, as_tuple=True)
             y = y.index_add(0, token, one(expert, x[token], share[token, place][:, None]))
-        return y.to(input.dtype).reshape(input.shape)
+        return y
 
     @staticmethod
     def _expert(stack, expert, dtype, device):
@@ -300,7 +318,13 @@ class GGMLMoE(torch.nn.Module):
             return plain.reshape(stack.shape)[expert].to(device, dtype)
         experts, rows, cols = stack.tensor_shape
         per = plain.numel() // experts
-        with torch._C._DisableFuncTorch():               # a weight is the same inside torch.func's transforms, and has to have memory there
+
+        def unpack():
             one = plain.reshape(-1)[expert * per:(expert + 1) * per].clone()
             one = GGMLTensor(one if one.is_cuda else one.to(device), tensor_type=stack.tensor_type, tensor_shape=(rows, cols))
-            return dequantize_tensor(one, dtype).to(device)
+            dense = dequantize_tensor(one, dtype)
+            return dense if dense.device == device else dense.to(device)
+        if _transform_stack() is None:
+            return unpack()
+        with torch._C._DisableFuncTorch():               # a weight is the same inside torch.func's transforms, and has to have memory there
+            return unpack()

@@ -132,3 +132,16 @@ def test_eight_bit_rows_do_not_go_over_the_inputs(pkg):
     for out in (A + row, 2 * A + row, 2 * A + 16):
         assert call(stream_out=out) == n.GGQ_ERR_ARG, hex(out)
     assert call(y=A, y_scale=None) == n.GGQ_ERR_ARG and call(y=5 * A, stream_out=5 * A, y_scale=None) == n.GGQ_ERR_ARG          # y on the stream that is stored
+
+
+def test_experts_in_torch_are_chosen_by_scores_in_64_bits(pkg):
+    """Small scores beside terms of 2^24 that cancel: 32 bits do not tell them apart.  Each expert's result is its own number."""
+    order = torch.tensor([3, 0, 7, 5, 1, 6, 2, 4])
+    router = torch.zeros(8, 64)
+    for e in range(8):
+        router[e, 4 * e], router[e, 63 - 4 * e], router[e, 4 * e + 1] = 2.0 ** 24, -2.0 ** 24, float(order[e]) * 2.0 ** -3
+    gate, up = torch.full((8, 1, 64), 1.0), torch.full((8, 1, 64), 1.0)
+    down = torch.arange(1.0, 9.0).view(8, 1, 1).expand(8, 64, 1)
+    x = torch.ones(2, 64)
+    y = pkg.ops.GGMLMoE(router, gate, up, down, top_k=1)(x)
+    assert torch.equal(y, torch.full((2, 64), 64.0 * 64.0 * 3))          # silu(64) is 64 in fp32; the third expert has the largest score
